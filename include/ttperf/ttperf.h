@@ -478,6 +478,85 @@ int ttp_capture_end(ttp_ctx* ctx, ttp_graph** out);
 int ttp_graph_launch(ttp_graph* graph);
 int ttp_graph_destroy(ttp_graph* graph);
 
+/* ---- fine-tuning operators ----------------------------------------------------------------
+ * What a fine-tuning step has on both sides of the backward that feeds the store: losses that
+ * give the logits' gradient, and activations kept in 8 bits with the gradients made from them.
+ * No counterpart in the reference, whose losses are a mean squared error and a cross entropy
+ * (autograd/dynamic/ops.hpp:160-173, py/nn.py:180-230) and whose tensors are kept whole.
+ *
+ * Common to all of them: work is queued on the context's stream and nothing waits for it; every
+ * pointer is device memory of the context's device, checked as ttp_upload checks one; what a
+ * call writes must not overlap anything else it is given, but for a result that is exactly its
+ * input (said where allowed).  A refused call changes nothing.  Scratch memory belongs to the
+ * context and grows with the sizes seen: while capturing, a call that would have to grow it is
+ * refused (TTP_ERR_STATE; make the call once before the capture).  Sums, softmax statistics and
+ * products are held in fp32 or more, results rounded once (to nearest even) to their type, and
+ * the same inputs give the same bits. */
+
+/* A matrix of `rows` rows of `cols` contiguous elements of type `dtype` (TTP_DTYPE_*), `stride`
+ * elements from row to row.  Rows may be 0; cols 1 to 2^31 - 1; any address and stride that the
+ * element type is aligned to. */
+typedef struct ttp_matrix {
+    void* data;
+    uint64_t rows, cols, stride;
+    int32_t dtype;
+    int32_t reserved; /* must be 0 */
+} ttp_matrix;
+
+/* Each row's log-probability of its token under softmax(logits row): logps[t] =
+ * z[t,y] - log sum_v exp z[t,v].  targets: one int64 per row; a negative one masks the row (0,
+ * its logits are not read); one past the vocabulary gives NaN.  Logits of -inf have
+ * probability 0; a row with NaN or +inf, or of -inf alone, gives NaN. */
+int ttp_token_logprobs(ttp_ctx* ctx, const ttp_matrix* logits, const int64_t* targets,
+                       float* logps);
+
+/* The preference loss of P pairs of sequences (direct preference optimisation).  Sequence s is
+ * rows starts[s] .. starts[s + 1] - 1 (2 P + 1 int64 in device memory, not decreasing, bounded
+ * to the rows there are; a sequence may be empty); the first P sequences are the chosen ones,
+ * sequence P + p the one rejected against p.  With d_s the sum over a sequence's unmasked rows
+ * of logp - ref_logps (ref_logps null: of logp), and h_p = beta (d_p - d_{P+p}):
+ *   loss = mean_p [ -(1 - eps) log sigmoid(h_p) - eps log sigmoid(-h_p) ],   margins[p] = h_p
+ * grad (null: none): dloss/dlogits times the context's loss scale while loss scaling is on; of
+ * logits' shape and type; zeros on masked rows and on rows in no sequence.  It may be exactly
+ * `logits`.  The sums over a sequence are in fp64. */
+typedef struct ttp_preference_args {
+    const ttp_matrix* logits;
+    const int64_t* targets;  /* rows */
+    const int64_t* starts;   /* 2 * pairs + 1 */
+    const float* ref_logps;  /* rows, or null */
+    uint64_t pairs;          /* 1 to 2^20 */
+    double beta;             /* > 0 */
+    double label_smoothing;  /* eps, in [0, 0.5] */
+    const ttp_matrix* grad;  /* out, or null */
+    float* logps;            /* out: rows */
+    float* margins;          /* out: pairs */
+    float* loss;             /* out: 1 */
+} ttp_preference_args;
+int ttp_preference_loss(ttp_ctx* ctx, const ttp_preference_args* args);
+
+/* The clipped policy loss over single tokens, with a penalty on the distance to a reference:
+ * with r = exp(logp - old_logps), A = advantages and g = ref_logps - logp of each unmasked row,
+ *   loss = 1/D sum [ -min(r A, clamp(r, 1 - clip_low, 1 + clip_high) A) + kl_coef k ],
+ *   k = exp(g) - g - 1,   kl = 1/D sum k   (ref_logps null: k = 0)
+ * D is `denominator`, or the number of unmasked rows (at least 1) where that is 0.
+ * grad: as in ttp_preference_loss. */
+typedef struct ttp_policy_args {
+    const ttp_matrix* logits;
+    const int64_t* targets;    /* rows */
+    const float* old_logps;    /* rows */
+    const float* advantages;   /* rows */
+    const float* ref_logps;    /* rows, or null */
+    double clip_low;           /* in [0, 1] */
+    double clip_high;          /* >= 0 */
+    double kl_coef;            /* >= 0; > 0 needs ref_logps */
+    double denominator;        /* > 0, or 0: the unmasked rows */
+    const ttp_matrix* grad;    /* out, or null */
+    float* logps;              /* out: rows */
+    float* loss;               /* out: 1 */
+    float* kl;                 /* out: 1 */
+} ttp_policy_args;
+int ttp_policy_loss(ttp_ctx* ctx, const ttp_policy_args* args);
+
 /* ---- per-kernel timing (HIP events on the context's stream) ------------------------------ */
 #define TTP_KERNEL_NORM 0   /* grad-norm / inf-check pass and the step's decisions */
 #define TTP_KERNEL_UPDATE 1 /* fused multi-tensor update pass               */

@@ -33,6 +33,7 @@
 #include <vector>
 
 #include "ttperf/ttperf.h"
+#include "context.hpp"
 #include "kernels.hpp"
 
 using ttp::Chunk;
@@ -212,6 +213,9 @@ struct ttp_ctx {
     std::vector<uint32_t> host_tile_base;
     uint32_t* tsum_pending = nullptr;
     bool acc_sums_used = false;
+    void* op_ws = nullptr;  // scratch of the operators' launches (ttpi::workspace)
+    uint64_t op_ws_bytes = 0;
+    bool op_ws_captured = false;  // a captured call uses it: replaced, it is kept
     std::vector<void*> retired;   // replaced buffers that live graphs may still write
 
     // bias-correction tables of every betas pair stepped with (kept, since captured graphs
@@ -942,9 +946,7 @@ int fill_report(ttp_ctx* c, bool norm_ran, ttp_step_report* r) {
 // buffers: the allocation the last of them was found in, which answers for the next one there
 // (a bucket's gradients are mostly slices of one allocation; the runtime's two queries take
 // about a microsecond per buffer).
-struct SeenAlloc {
-    uintptr_t lo = 0, end = 0;
-};
+using ttpi::SeenAlloc;
 int check_device_buffer(const ttp_ctx* c, const void* p, uint64_t bytes, const char* what,
                         SeenAlloc* seen = nullptr) {
     if (!bytes) return TTP_OK;
@@ -983,6 +985,20 @@ int check_index(const ttp_ctx* c, uint32_t i) {
     if (i >= c->tensors.size())
         return fail(TTP_ERR_RANGE, "tensor index " + std::to_string(i) + " out of range");
     return TTP_OK;
+}
+
+// Whether an accumulate's kernel assigns (no grad yet) or adds is fixed when the call is captured.
+// Every launch must therefore find the flag as the capture did: a call earlier in the same
+// capture must have set it (zero_grad with set_to_none, set_has_grad, a gradient upload
+// or an accumulate; zeroing to zeros leaves the flag as the launch finds it).
+int captured_accumulate(const ttp_ctx* c, uint32_t index) {
+    if (!c->capturing || (c->cap_touched[index] & kCapGrad)) return TTP_OK;
+    return fail(TTP_ERR_STATE,
+                "a captured accumulate into tensor " + std::to_string(index) +
+                    " must follow a call of the same capture that sets that tensor's "
+                    "has-grad flag (zero_grad with set_to_none, set_has_grad, a gradient "
+                    "upload or an accumulate): whether it assigns or adds is fixed when it "
+                    "is captured");
 }
 
 // Elements per record of buffer `which`: element e sits at base + (e / kRec) * stride +
@@ -1192,7 +1208,7 @@ void release(ttp_ctx* c) {
     for (void* p : {(void*)c->grad, (void*)c->records, (void*)c->momentum, (void*)c->mom_init,
                     (void*)c->st, (void*)c->slots, (void*)c->partials, (void*)c->tickets,
                     c->staging, (void*)c->tsum, (void*)c->tile_sums, (void*)c->acc_tiles, (void*)c->tile_base,
-                    (void*)c->tsum_pending})
+                    (void*)c->tsum_pending, c->op_ws})
         if (p) (void)hipFree(p);
     for (auto& kv : c->bias_tables) (void)hipFree(kv.second.first);
     free_tables(c->all);
@@ -1213,6 +1229,78 @@ void release(ttp_ctx* c) {
 }
 
 }  // namespace
+
+// =====================================================================================
+// what the operators' files use (context.hpp)
+// =====================================================================================
+namespace ttpi {
+
+int fail(int code, const std::string& msg) { return ::fail(code, msg); }
+
+int hip_failed(hipError_t e, const char* what) {
+    clear_hip_error();
+    return ::fail(e == hipErrorOutOfMemory ? TTP_ERR_OOM : TTP_ERR_HIP,
+                  std::string(what) + ": " + hipGetErrorString(e));
+}
+
+int begin(ttp_ctx* c, Op* op) {
+    int rc = check_ctx(c);
+    if (rc) return rc;
+    if ((rc = set_dev(c))) return rc;
+    *op = {c->stream, c->num_cus, c->scaler.enabled ? &c->st->scale : nullptr, c->tickets};
+    return TTP_OK;
+}
+
+int device_buffer(const ttp_ctx* c, const void* p, uint64_t bytes, const char* what,
+                  SeenAlloc* seen) {
+    if (bytes && !p) return ::fail(TTP_ERR_INVALID, std::string("null pointer for ") + what);
+    return check_device_buffer(c, p, bytes, what, seen);
+}
+
+int workspace(ttp_ctx* c, uint64_t bytes, void** p) {
+    if (bytes > c->op_ws_bytes) {
+        int rc;
+        const char* what = "a first operator call of this size (allocates its scratch memory)";
+        if ((rc = no_capture(c, what)) || (rc = no_stream_capture(c, what))) return rc;
+        // half as much again, so that slowly growing sizes do not allocate every time
+        const uint64_t grown = (bytes + bytes / 2 + 4095) / 4096 * 4096;
+        HIP_TRY(hipStreamSynchronize(c->stream));  // queued calls may still use the old memory
+        if (c->op_ws) {
+            if (c->op_ws_captured)
+                c->retired.push_back(c->op_ws);  // used on replay
+            else
+                HIP_TRY(hipFree(c->op_ws));
+        }
+        c->op_ws = nullptr;
+        c->op_ws_bytes = 0;
+        c->op_ws_captured = false;
+        HIP_TRY(hipMalloc(&c->op_ws, grown));
+        c->op_ws_bytes = grown;
+    }
+    if (c->stream && !c->op_ws_captured) {  // the context's capture, or its caller's
+        hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+        HIP_TRY(hipStreamIsCapturing(c->stream, &status));
+        c->op_ws_captured = status != hipStreamCaptureStatusNone;
+    }
+    *p = c->op_ws;
+    return TTP_OK;
+}
+
+int grad_target(ttp_ctx* c, uint32_t index, GradTarget* out) {
+    int rc = check_index(c, index);
+    if (rc) return rc;
+    if ((rc = captured_accumulate(c, index))) return rc;
+    const TensorRec& t = c->tensors[index];
+    *out = {(char*)c->grad + t.offset * grad_esize(c), t.numel, bf16_grads(c), !t.has_grad};
+    return TTP_OK;
+}
+
+void grad_written(ttp_ctx* c, uint32_t index) {
+    set_grad_flag(c, index, true);
+    set_fresh(c, index, false);
+}
+
+}  // namespace ttpi
 
 // =====================================================================================
 // C ABI
@@ -1678,17 +1766,7 @@ int ttp_accumulate_grad(ttp_ctx* c, uint32_t index, const void* src, uint64_t n,
                                      "optionally | TTP_ACCUM_SUMSQ");
     if (kind != TTP_HOST && kind != TTP_DEVICE) return fail(TTP_ERR_INVALID, "bad memory kind");
     if (kind == TTP_HOST && (rc = no_capture(c, "accumulating a host gradient"))) return rc;
-    // Whether the kernel assigns (no grad yet) or adds is fixed when the call is captured.
-    // Every launch must therefore find the flag as the capture did: a call earlier in the same
-    // capture must have set it (zero_grad with set_to_none, set_has_grad, a gradient upload
-    // or an accumulate; zeroing to zeros leaves the flag as the launch finds it).
-    if (c->capturing && !(c->cap_touched[index] & kCapGrad))
-        return fail(TTP_ERR_STATE,
-                    "a captured accumulate into tensor " + std::to_string(index) +
-                        " must follow a call of the same capture that sets that tensor's "
-                        "has-grad flag (zero_grad with set_to_none, set_has_grad, a gradient "
-                        "upload or an accumulate): whether it assigns or adds is fixed when it "
-                        "is captured");
+    if ((rc = captured_accumulate(c, index))) return rc;
     TensorRec& t = c->tensors[index];
     if (n != t.numel)
         return fail(TTP_ERR_RANGE, "tensor " + std::to_string(index) + " has " +
@@ -1810,13 +1888,7 @@ int ttp_accumulate_grad_multi(ttp_ctx* c, const uint32_t* indices, const void* c
         if (seen[i]) return fail(TTP_ERR_INVALID, "tensor index " + std::to_string(i) +
                                                       " listed twice");
         seen[i] = 1;
-        if (c->capturing && !(c->cap_touched[i] & kCapGrad))
-            return fail(TTP_ERR_STATE,
-                        "a captured accumulate into tensor " + std::to_string(i) +
-                            " must follow a call of the same capture that sets that tensor's "
-                            "has-grad flag (zero_grad with set_to_none, set_has_grad, a "
-                            "gradient upload or an accumulate): whether it assigns or adds is "
-                            "fixed when it is captured");
+        if ((rc = captured_accumulate(c, i))) return rc;
         const TensorRec& t = c->tensors[i];
         if (!t.numel) continue;
         if (!srcs[k]) return fail(TTP_ERR_INVALID, "null source for tensor " + std::to_string(i));

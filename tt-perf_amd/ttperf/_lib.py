@@ -60,8 +60,30 @@ class StepReport(C.Structure):
         return {k: getattr(self, k) for k, _ in self._fields_ if k != "reserved"}
 
 
-# name -> (restype, argtypes); the ABI surface the header declares
 _P = C.c_void_p
+
+
+class Matrix(C.Structure):
+    _fields_ = [("data", _P), ("rows", C.c_uint64), ("cols", C.c_uint64),
+                ("stride", C.c_uint64), ("dtype", C.c_int32), ("reserved", C.c_int32)]
+
+
+class PreferenceArgs(C.Structure):
+    _fields_ = [("logits", C.POINTER(Matrix)), ("targets", _P), ("starts", _P),
+                ("ref_logps", _P), ("pairs", C.c_uint64), ("beta", C.c_double),
+                ("label_smoothing", C.c_double), ("grad", C.POINTER(Matrix)), ("logps", _P),
+                ("margins", _P), ("loss", _P)]
+
+
+class PolicyArgs(C.Structure):
+    _fields_ = [("logits", C.POINTER(Matrix)), ("targets", _P), ("old_logps", _P),
+                ("advantages", _P), ("ref_logps", _P), ("clip_low", C.c_double),
+                ("clip_high", C.c_double), ("kl_coef", C.c_double),
+                ("denominator", C.c_double), ("grad", C.POINTER(Matrix)), ("logps", _P),
+                ("loss", _P), ("kl", _P)]
+
+
+# name -> (restype, argtypes); the ABI surface the header declares
 SIGNATURES = {
     "ttp_device_count": (C.c_int, [C.POINTER(C.c_int)]),
     "ttp_create": (C.c_int, [C.c_int, C.POINTER(TensorDesc), C.c_uint32, C.c_int, C.POINTER(_P)]),
@@ -110,6 +132,9 @@ SIGNATURES = {
     "ttp_capture_end": (C.c_int, [_P, C.POINTER(_P)]),
     "ttp_graph_launch": (C.c_int, [_P]),
     "ttp_graph_destroy": (C.c_int, [_P]),
+    "ttp_token_logprobs": (C.c_int, [_P, C.POINTER(Matrix), _P, _P]),
+    "ttp_preference_loss": (C.c_int, [_P, C.POINTER(PreferenceArgs)]),
+    "ttp_policy_loss": (C.c_int, [_P, C.POINTER(PolicyArgs)]),
     "ttp_timing_enable": (C.c_int, [_P, C.c_int]),
     "ttp_timing_collect": (C.c_int, [_P, C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_uint64)]),
     "ttp_last_error": (C.c_char_p, []),

@@ -1,0 +1,219 @@
+"""The fine-tuning operators of a ParamStore: losses over logits with their gradient.
+
+They take and give torch tensors on the store's device.  Results are new tensors unless given;
+work is queued on the store's stream, ordered with torch's current stream as the store's other
+device work is (no synchronisation when both share one stream, see ParamStore.set_stream).
+While the store captures a graph, every result has to be given (an earlier call's, `out=`), and
+the graph reads and writes the tensors in place at every launch.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Any, NamedTuple, Optional
+
+from . import _lib as L
+
+
+class PreferenceLoss(NamedTuple):
+    """loss (), margins (pairs,) and logps (rows,) in float32, and the logits' gradient (or
+    None)."""
+    loss: Any
+    margins: Any
+    logps: Any
+    grad: Optional[Any]
+
+
+class PolicyLoss(NamedTuple):
+    """loss (), kl () and logps (rows,) in float32, and the logits' gradient (or None)."""
+    loss: Any
+    kl: Any
+    logps: Any
+    grad: Optional[Any]
+
+
+def _matrix(t):
+    """The C view of a 2-D tensor whose rows are contiguous."""
+    import torch
+    rows, cols = t.shape
+    stride = t.stride(0) if rows > 1 else cols
+    return L.Matrix(data=t.data_ptr(), rows=rows, cols=cols, stride=stride, reserved=0,
+                    dtype=L.DTYPE_BF16 if t.dtype == torch.bfloat16 else L.DTYPE_F32)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+class Operators:
+    """Mixed into ParamStore."""
+
+    def _rows_of(self, t, what):
+        """A 2-D view of a float32 or bfloat16 device tensor: all but its last dimension are
+        rows (a tensor of one dimension is one row).  Nothing is copied: a layout that is no
+        matrix of contiguous rows is refused."""
+        import torch
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or \
+                t.dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError(f"{what} must be a float32 or bfloat16 tensor on the GPU")
+        if t.device.index != self.device:
+            raise ValueError(f"{what} is on {t.device}, the store on cuda:{self.device}")
+        t = t.detach()
+        if t.dim() == 0 or t.shape[-1] == 0:
+            raise ValueError(f"{what} has no columns")
+        if t.dim() != 2:
+            try:
+                t = t.view(-1, t.shape[-1])
+            except RuntimeError:
+                raise ValueError(f"{what} must be a matrix of contiguous rows (or a view as "
+                                 "one): make it contiguous first") from None
+        if t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or
+                          (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
+            raise ValueError(f"{what} must have contiguous rows that do not overlap: make it "
+                             "contiguous first")
+        return t
+
+    def _vector_of(self, t, n, dtype, what):
+        """A contiguous 1-D device tensor of n elements of `dtype` (a copy where it is not)."""
+        import torch
+        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype:
+            raise ValueError(f"{what} must be a {str(dtype)[6:]} tensor on the GPU")
+        if t.device.index != self.device:
+            raise ValueError(f"{what} is on {t.device}, the store on cuda:{self.device}")
+        if t.numel() != n:
+            raise ValueError(f"{what}: expected {n} elements, got {t.numel()}")
+        t = t.detach()
+        if self._in_capture and not t.is_contiguous():
+            raise ValueError(f"{what} must be contiguous while capturing")
+        return t.contiguous().view(-1)
+
+    def _result(self, given, shape, dtype, what):
+        """The tensor to write: `given`, checked, or a new one."""
+        import torch
+        if given is None:
+            if self._in_capture:
+                raise ValueError(f"{what} has to be given while capturing")
+            return torch.empty(shape, dtype=dtype, device=f"cuda:{self.device}")
+        if not isinstance(given, torch.Tensor) or not given.is_cuda or given.dtype != dtype or \
+                given.device.index != self.device or tuple(given.shape) != tuple(shape) or \
+                not given.is_contiguous():
+            raise ValueError(f"{what} must be a contiguous {str(dtype)[6:]} tensor of shape "
+                             f"{tuple(shape)} on cuda:{self.device}")
+        return given.detach()
+
+    def _queue(self, tensors, call):
+        """Queue `call` behind torch's work on `tensors`, which it reads and writes."""
+        if self._in_capture:
+            L.check(call())
+            return
+        kept = self._before_device_sources(tensors)
+        L.check(call())
+        self._after_device_sources(kept)
+
+    def _gradient(self, grad, logits, want):
+        """(what the caller gets back, its matrix) of a loss's gradient: `grad` True for a new
+        tensor like the logits, a tensor to write it to (the logits themselves too), False for
+        none."""
+        import torch
+        if grad is False or grad is None:
+            return None, None
+        if grad is True:
+            if want is not None:
+                grad = want
+            else:
+                if self._in_capture:
+                    raise ValueError("the gradient has to be given while capturing")
+                grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        if not isinstance(grad, torch.Tensor) or grad.dtype != logits.dtype or \
+                grad.shape != logits.shape:
+            raise ValueError("the gradient must be a tensor of the logits' shape and type")
+        return grad, self._rows_of(grad, "the gradient")
+
+    def token_logprobs(self, logits, targets, *, out=None):
+        """Each row's log-probability of its token under softmax(logits): float32, of targets'
+        shape.  logits: (..., V) float32 or bfloat16; targets: int64, a negative one masks its
+        row (0).  A token past the vocabulary gives NaN.  (ttp_token_logprobs)"""
+        import torch
+        z = self._rows_of(logits, "the logits")
+        y = self._vector_of(targets, z.shape[0], torch.int64, "the targets")
+        out = self._result(out, targets.shape, torch.float32, "out")
+        m = _matrix(z)
+        self._queue((z, y, out), lambda: L.lib.ttp_token_logprobs(
+            self._h, C.byref(m), y.data_ptr(), out.data_ptr()))
+        return out
+
+    def preference_loss(self, logits, targets, starts, ref_logps=None, *, beta=0.1,
+                        label_smoothing=0.0, grad=True, out=None):
+        """The preference loss of P pairs of sequences, and its gradient for the logits.
+
+        Sequence s is rows starts[s] to starts[s + 1] (starts: int64, 2 P + 1 of them on the GPU,
+        not decreasing); the first P sequences are the chosen ones, sequence P + p the one
+        rejected against p.  With d the sum of logps - ref_logps over a sequence's unmasked rows
+        (targets < 0: masked) and margins = beta (d_chosen - d_rejected):
+
+            loss = mean(-(1 - eps) log sigmoid(margins) - eps log sigmoid(-margins))
+
+        grad: True (a new tensor), False (none), or the tensor to write it to, which may be
+        `logits` itself.  While loss scaling is on the gradient is the scaled loss's, by the
+        store's own scale; the loss is not scaled.  logits.backward(r.grad) continues in torch.
+        out: an earlier call's result, whose tensors are written again.  (ttp_preference_loss)"""
+        import torch
+        z = self._rows_of(logits, "the logits")
+        rows = z.shape[0]
+        y = self._vector_of(targets, rows, torch.int64, "the targets")
+        if not isinstance(starts, torch.Tensor) or starts.numel() < 3 or starts.numel() % 2 == 0:
+            raise ValueError("starts must hold 2 * pairs + 1 row numbers")
+        pairs = starts.numel() // 2
+        at = self._vector_of(starts, 2 * pairs + 1, torch.int64, "starts")
+        ref = None if ref_logps is None else self._vector_of(
+            ref_logps, rows, torch.float32, "ref_logps")
+        loss = self._result(out and out.loss, (), torch.float32, "the loss")
+        margins = self._result(out and out.margins, (pairs,), torch.float32, "the margins")
+        logps = self._result(out and out.logps, targets.shape, torch.float32, "the logps")
+        given, g = self._gradient(grad, logits, out and out.grad)
+        m, gm = _matrix(z), None if g is None else _matrix(g)
+        args = L.PreferenceArgs(
+            logits=C.pointer(m), targets=y.data_ptr(), starts=at.data_ptr(), ref_logps=_ptr(ref),
+            pairs=pairs, beta=beta, label_smoothing=label_smoothing,
+            grad=None if gm is None else C.pointer(gm), logps=logps.data_ptr(),
+            margins=margins.data_ptr(), loss=loss.data_ptr())
+        used = [t for t in (z, y, at, ref, g, logps, margins, loss) if t is not None]
+        self._queue(used, lambda: L.lib.ttp_preference_loss(self._h, C.byref(args)))
+        return PreferenceLoss(loss, margins, logps, given)
+
+    def policy_loss(self, logits, targets, old_logps, advantages, ref_logps=None, *, clip=0.2,
+                    kl_coef=0.0, denominator=None, grad=True, out=None):
+        """The clipped policy loss over single tokens, and its gradient for the logits.
+
+        With r = exp(logp - old_logps), A = advantages, g = ref_logps - logp of each unmasked row
+        (targets < 0: masked), k = exp(g) - g - 1 (0 without ref_logps):
+
+            loss = sum(-min(r A, clamp(r, 1 - clip[0], 1 + clip[1]) A) + kl_coef k) / D
+            kl   = sum(k) / D
+
+        clip: one number or (low, high).  denominator: D; None: the number of unmasked rows (at
+        least 1).  grad and out as in preference_loss.  (ttp_policy_loss)"""
+        import torch
+        low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)
+        if denominator is not None and not denominator > 0:
+            raise ValueError("denominator must be positive")
+        z = self._rows_of(logits, "the logits")
+        rows = z.shape[0]
+        y = self._vector_of(targets, rows, torch.int64, "the targets")
+        old = self._vector_of(old_logps, rows, torch.float32, "old_logps")
+        adv = self._vector_of(advantages, rows, torch.float32, "advantages")
+        ref = None if ref_logps is None else self._vector_of(
+            ref_logps, rows, torch.float32, "ref_logps")
+        loss = self._result(out and out.loss, (), torch.float32, "the loss")
+        kl = self._result(out and out.kl, (), torch.float32, "kl")
+        logps = self._result(out and out.logps, targets.shape, torch.float32, "the logps")
+        given, g = self._gradient(grad, logits, out and out.grad)
+        m, gm = _matrix(z), None if g is None else _matrix(g)
+        args = L.PolicyArgs(
+            logits=C.pointer(m), targets=y.data_ptr(), old_logps=old.data_ptr(),
+            advantages=adv.data_ptr(), ref_logps=_ptr(ref), clip_low=low, clip_high=high,
+            kl_coef=kl_coef, denominator=denominator or 0.0,
+            grad=None if gm is None else C.pointer(gm), logps=logps.data_ptr(),
+            loss=loss.data_ptr(), kl=kl.data_ptr())
+        used = [t for t in (z, y, old, adv, ref, g, logps, loss, kl) if t is not None]
+        self._queue(used, lambda: L.lib.ttp_policy_loss(self._h, C.byref(args)))
+        return PolicyLoss(loss, kl, logps, given)

@@ -19,6 +19,7 @@ import weakref
 import numpy as np
 
 from . import _lib as L
+from .operators import Operators
 
 
 def _is_torch(x):
@@ -279,7 +280,7 @@ class _StepSlots:
         opt._saved_t.pop(self, None)
 
 
-class ParamStore(_StepSlots):
+class ParamStore(_StepSlots, Operators):
     """One context: tensors laid out 64-element aligned in caller order.
 
     shapes : list of shapes (tuples) or element counts
