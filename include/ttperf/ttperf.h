@@ -557,6 +557,43 @@ typedef struct ttp_policy_args {
 } ttp_policy_args;
 int ttp_policy_loss(ttp_ctx* ctx, const ttp_policy_args* args);
 
+/* An activation of rows x cols kept in 8 bits for the backward: blocks of 32 columns of one row
+ * (the last one may be shorter) share a power of two, so that every kept value is exact in bf16.
+ * values: rows x W bytes, W = cols rounded up to 32 (zeros behind the last column), 16-byte
+ * aligned; scales: rows x W / 32 bytes.  Element (t, i) stands for
+ *   v 2^(scales[t][i / 32] - 127),  v = values[t][i] as int8 (TTP_CHECKPOINT_INT8, |v| <= 127) or
+ *                                   as fp8 e4m3 (TTP_CHECKPOINT_E4M3, |v| <= 448)
+ * with the least such power that holds the block's largest magnitude (not below 2^-126 for int8,
+ * 2^-117 for e4m3: blocks that small lose bits), and v rounded to nearest even.  A block that
+ * holds an infinity or a NaN gets the scale 255 and stands for NaN, so that an overflow reaches
+ * the gradients. */
+#define TTP_CHECKPOINT_INT8 0
+#define TTP_CHECKPOINT_E4M3 1
+#define TTP_CHECKPOINT_BLOCK 32
+typedef struct ttp_checkpoint8 {
+    void* values;
+    void* scales;
+    uint64_t rows, cols;
+    int32_t format;   /* TTP_CHECKPOINT_* */
+    int32_t reserved; /* must be 0 */
+} ttp_checkpoint8;
+/* x into `kept`. */
+int ttp_checkpoint8_pack(ttp_ctx* ctx, const ttp_matrix* x, const ttp_checkpoint8* kept);
+/* The values `kept` stands for (exact in bf16 and fp32). */
+int ttp_checkpoint8_restore(ttp_ctx* ctx, const ttp_checkpoint8* kept, const ttp_matrix* x);
+
+/* GELU that keeps its input in 8 bits.  approximate: TTP_GELU_ERF, x Phi(x), or TTP_GELU_TANH,
+ * x/2 (1 + tanh(sqrt(2/pi) (x + 0.044715 x^3))) (GPT-2's).
+ * Forward: y = gelu(x) from the whole x, and x into `kept`, in one pass.  y has x's type and may
+ * be exactly x.  Backward: dx = dy gelu'(xhat) from the kept values xhat; dx has dy's type and may
+ * be exactly dy. */
+#define TTP_GELU_ERF 0
+#define TTP_GELU_TANH 1
+int ttp_gelu_checkpoint8(ttp_ctx* ctx, const ttp_matrix* x, int approximate, const ttp_matrix* y,
+                         const ttp_checkpoint8* kept);
+int ttp_gelu_backward8(ttp_ctx* ctx, const ttp_checkpoint8* kept, int approximate,
+                       const ttp_matrix* dy, const ttp_matrix* dx);
+
 /* ---- per-kernel timing (HIP events on the context's stream) ------------------------------ */
 #define TTP_KERNEL_NORM 0   /* grad-norm / inf-check pass and the step's decisions */
 #define TTP_KERNEL_UPDATE 1 /* fused multi-tensor update pass               */

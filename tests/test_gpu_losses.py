@@ -7,7 +7,7 @@ Tolerances, from the arithmetic (u = 2^-24):
          off, which the terms that matter (z near m) do not show:
          u (|z_y - m| + |log s| + V / 256 + 64)
   grad   c ([v = y] - p): p is off by the exponent's argument (|z_v - m| 3 u) and s; c by the
-         rows' sums; rounded once to its type: 2^-9 relative in bf16, u in fp32
+         rows' sums; rounded once to its type: 2^-8 relative in bf16, u in fp32
 """
 import math
 

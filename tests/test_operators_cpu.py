@@ -9,13 +9,13 @@ import pytest
 from conftest import REPO
 from test_isa_cpu import HIPCC, PKG, scc_reads_live_into_a_block
 
-OPERATOR_FILES = ("losses",)
+OPERATOR_FILES = ("losses", "checkpoint8")
 
 
 def test_struct_layouts_match_the_header(tmp_path):
     from ttperf import _lib as L
     structs = {"ttp_matrix": L.Matrix, "ttp_preference_args": L.PreferenceArgs,
-               "ttp_policy_args": L.PolicyArgs}
+               "ttp_policy_args": L.PolicyArgs, "ttp_checkpoint8": L.Checkpoint8}
     lines = ['#include <stdio.h>', '#include <stddef.h>', '#include "ttperf/ttperf.h"',
              "int main(void) {"]
     for cname, ct in structs.items():
@@ -43,6 +43,12 @@ def test_a_null_context_is_refused():
     assert L.lib.ttp_token_logprobs(None, C.byref(m), None, None) == L.ERR_INVALID
     assert L.lib.ttp_preference_loss(None, C.byref(L.PreferenceArgs())) == L.ERR_INVALID
     assert L.lib.ttp_policy_loss(None, C.byref(L.PolicyArgs())) == L.ERR_INVALID
+    k = L.Checkpoint8()
+    assert L.lib.ttp_checkpoint8_pack(None, C.byref(m), C.byref(k)) == L.ERR_INVALID
+    assert L.lib.ttp_checkpoint8_restore(None, C.byref(k), C.byref(m)) == L.ERR_INVALID
+    assert L.lib.ttp_gelu_checkpoint8(None, C.byref(m), 0, C.byref(m), C.byref(k)) == \
+        L.ERR_INVALID
+    assert L.lib.ttp_gelu_backward8(None, C.byref(k), 0, C.byref(m), C.byref(m)) == L.ERR_INVALID
 
 
 @pytest.mark.parametrize("name", OPERATOR_FILES)

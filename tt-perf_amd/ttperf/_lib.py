@@ -24,6 +24,9 @@ ACCUM_SUMSQ = 0x100
 ACCUM_MULTI_MAX = 64  # tensors per ttp_accumulate_grad_multi call
 ZERO_NO_FILL = 0x100  # OR'd into zero_grad's set_to_none: flags only
 STEP_SLOTS = 64  # step counts ttp_swap_step keeps
+CHECKPOINT_INT8, CHECKPOINT_E4M3 = 0, 1
+CHECKPOINT_BLOCK = 32  # columns that share a scale
+GELU_ERF, GELU_TANH = 0, 1
 STEP_TENSOR_SUMS = 1
 STEP_DEFER_SCALE = 2
 KERNEL_NORM, KERNEL_UPDATE = 0, 1
@@ -83,6 +86,11 @@ class PolicyArgs(C.Structure):
                 ("loss", _P), ("kl", _P)]
 
 
+class Checkpoint8(C.Structure):
+    _fields_ = [("values", _P), ("scales", _P), ("rows", C.c_uint64), ("cols", C.c_uint64),
+                ("format", C.c_int32), ("reserved", C.c_int32)]
+
+
 # name -> (restype, argtypes); the ABI surface the header declares
 SIGNATURES = {
     "ttp_device_count": (C.c_int, [C.POINTER(C.c_int)]),
@@ -135,6 +143,12 @@ SIGNATURES = {
     "ttp_token_logprobs": (C.c_int, [_P, C.POINTER(Matrix), _P, _P]),
     "ttp_preference_loss": (C.c_int, [_P, C.POINTER(PreferenceArgs)]),
     "ttp_policy_loss": (C.c_int, [_P, C.POINTER(PolicyArgs)]),
+    "ttp_checkpoint8_pack": (C.c_int, [_P, C.POINTER(Matrix), C.POINTER(Checkpoint8)]),
+    "ttp_checkpoint8_restore": (C.c_int, [_P, C.POINTER(Checkpoint8), C.POINTER(Matrix)]),
+    "ttp_gelu_checkpoint8": (C.c_int, [_P, C.POINTER(Matrix), C.c_int, C.POINTER(Matrix),
+                                       C.POINTER(Checkpoint8)]),
+    "ttp_gelu_backward8": (C.c_int, [_P, C.POINTER(Checkpoint8), C.c_int, C.POINTER(Matrix),
+                                     C.POINTER(Matrix)]),
     "ttp_timing_enable": (C.c_int, [_P, C.c_int]),
     "ttp_timing_collect": (C.c_int, [_P, C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_uint64)]),
     "ttp_last_error": (C.c_char_p, []),

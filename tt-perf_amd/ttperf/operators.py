@@ -1,4 +1,5 @@
-"""The fine-tuning operators of a ParamStore: losses over logits with their gradient.
+"""The fine-tuning operators of a ParamStore: losses over logits with their gradient, activations
+kept in 8 bits and the gradients made from them.
 
 They take and give torch tensors on the store's device.  Results are new tensors unless given;
 work is queued on the store's stream, ordered with torch's current stream as the store's other
@@ -29,6 +30,35 @@ class PolicyLoss(NamedTuple):
     kl: Any
     logps: Any
     grad: Optional[Any]
+
+
+class Checkpoint8:
+    """An activation kept in 8 bits (ttp_checkpoint8): `values` (rows, cols rounded up to 32) and
+    `scales` (rows, that / 32), both uint8; element i of a row is values[i] (int8, or fp8 e4m3)
+    times 2^(scales[i // 32] - 127).  `shape` and `dtype` are the activation's own."""
+
+    __slots__ = ("values", "scales", "shape", "dtype", "format", "rows", "cols")
+
+    def __init__(self, values, scales, shape, dtype, fmt):
+        self.values, self.scales = values, scales
+        self.shape, self.dtype, self.format = tuple(shape), dtype, fmt
+        self.cols = self.shape[-1]
+        self.rows = values.shape[0]
+
+    def _c(self):
+        return L.Checkpoint8(values=self.values.data_ptr(), scales=self.scales.data_ptr(),
+                             rows=self.rows, cols=self.cols,
+                             format=_FORMATS[self.format], reserved=0)
+
+
+_FORMATS = {"int8": L.CHECKPOINT_INT8, "e4m3": L.CHECKPOINT_E4M3}
+_APPROXIMATE = {"none": L.GELU_ERF, "tanh": L.GELU_TANH}
+
+
+def _choice(table, key, what):
+    if key not in table:
+        raise ValueError(f"{what} must be one of {', '.join(map(repr, table))}")
+    return table[key]
 
 
 def _matrix(t):
@@ -217,3 +247,88 @@ class Operators:
         used = [t for t in (z, y, old, adv, ref, g, logps, loss, kl) if t is not None]
         self._queue(used, lambda: L.lib.ttp_policy_loss(self._h, C.byref(args)))
         return PolicyLoss(loss, kl, logps, given)
+
+    # ---- activations kept in 8 bits ------------------------------------------------------------
+    def _kept_of(self, x, fmt, out, shape):
+        """The checkpoint to write for the matrix `x`: `out`, checked, or a new one."""
+        import torch
+        _choice(_FORMATS, fmt, "fmt")
+        rows, cols = x.shape
+        blocks = -(-cols // L.CHECKPOINT_BLOCK)
+        if out is not None and (not isinstance(out, Checkpoint8) or out.format != fmt or
+                                out.shape != tuple(shape)):
+            raise ValueError(f"out must be a checkpoint of shape {tuple(shape)} in {fmt}")
+        values = self._result(out and out.values, (rows, blocks * L.CHECKPOINT_BLOCK),
+                              torch.uint8, "the checkpoint")
+        scales = self._result(out and out.scales, (rows, blocks), torch.uint8, "the checkpoint")
+        return out or Checkpoint8(values, scales, shape, x.dtype, fmt)
+
+    @staticmethod
+    def _check_kept(kept):
+        if not isinstance(kept, Checkpoint8):
+            raise ValueError("a Checkpoint8 is needed (checkpoint8, gelu_checkpoint8)")
+
+    def checkpoint8(self, x, *, fmt="int8", out=None):
+        """x (..., cols), float32 or bfloat16, kept in 8 bits: a Checkpoint8.  Blocks of 32 columns
+        share a power of two; fmt "int8" keeps 7 bits beside the sign of a block's largest value,
+        "e4m3" 4 significant bits of every value.  A block with an infinity or a NaN stands for
+        NaN.  out: a Checkpoint8 to write again.  (ttp_checkpoint8_pack)"""
+        m = self._rows_of(x, "the activation")
+        kept = self._kept_of(m, fmt, out, x.shape)
+        a, k = _matrix(m), kept._c()
+        self._queue((m, kept.values, kept.scales), lambda: L.lib.ttp_checkpoint8_pack(
+            self._h, C.byref(a), C.byref(k)))
+        return kept
+
+    def restore8(self, kept, *, dtype=None, out=None):
+        """The values a Checkpoint8 stands for, in its activation's shape and type (or `dtype`:
+        float32 or bfloat16; exact in both).  (ttp_checkpoint8_restore)"""
+        import torch
+        self._check_kept(kept)
+        dtype = dtype or (kept.dtype if out is None else out.dtype)
+        if dtype not in (torch.float32, torch.bfloat16):
+            raise ValueError("dtype must be torch.float32 or torch.bfloat16")
+        out = self._result(out, kept.shape, dtype, "out")
+        m = self._rows_of(out, "out")
+        a, k = _matrix(m), kept._c()
+        self._queue((kept.values, kept.scales, m), lambda: L.lib.ttp_checkpoint8_restore(
+            self._h, C.byref(k), C.byref(a)))
+        return out
+
+    def gelu_checkpoint8(self, x, *, fmt="int8", approximate="none", out=None, kept=None):
+        """(gelu(x), x as a Checkpoint8) in one pass.  approximate: "none" (x Phi(x)) or "tanh"
+        (GPT-2's), as torch.nn.functional.gelu.  out: where to put gelu(x), x itself too; kept: a
+        Checkpoint8 to write again.  (ttp_gelu_checkpoint8)"""
+        approx = _choice(_APPROXIMATE, approximate, "approximate")
+        m = self._rows_of(x, "the input")
+        if out is None:
+            out = self._result(None, x.shape, x.dtype, "out")
+        y = self._like(out, x, "out")
+        kept = self._kept_of(m, fmt, kept, x.shape)
+        a, b, k = _matrix(m), _matrix(y), kept._c()
+        self._queue((m, y, kept.values, kept.scales), lambda: L.lib.ttp_gelu_checkpoint8(
+            self._h, C.byref(a), approx, C.byref(b), C.byref(k)))
+        return out, kept
+
+    def gelu_backward8(self, kept, dy, *, approximate="none", out=None):
+        """dy gelu'(x) from the x that gelu_checkpoint8 kept.  out: where to put it, dy itself
+        too.  (ttp_gelu_backward8)"""
+        approx = _choice(_APPROXIMATE, approximate, "approximate")
+        self._check_kept(kept)
+        g = self._rows_of(dy, "dy")
+        if tuple(dy.shape) != kept.shape:
+            raise ValueError(f"dy has shape {tuple(dy.shape)}, the checkpoint {kept.shape}")
+        if out is None:
+            out = self._result(None, dy.shape, dy.dtype, "out")
+        d = self._like(out, dy, "out")
+        a, b, k = _matrix(g), _matrix(d), kept._c()
+        self._queue((kept.values, kept.scales, g, d), lambda: L.lib.ttp_gelu_backward8(
+            self._h, C.byref(k), approx, C.byref(a), C.byref(b)))
+        return out
+
+    def _like(self, out, x, what):
+        """The matrix of a result that has x's shape and type."""
+        import torch
+        if not isinstance(out, torch.Tensor) or out.dtype != x.dtype or out.shape != x.shape:
+            raise ValueError(f"{what} must be a tensor of the input's shape and type")
+        return self._rows_of(out, what)
