@@ -594,6 +594,18 @@ int ttp_gelu_checkpoint8(ttp_ctx* ctx, const ttp_matrix* x, int approximate, con
 int ttp_gelu_backward8(ttp_ctx* ctx, const ttp_checkpoint8* kept, int approximate,
                        const ttp_matrix* dy, const ttp_matrix* dx);
 
+/* A linear layer's gradients from its input kept in 8 bits, into the store's gradients as
+ * ttp_accumulate_grad puts them (assigned where the tensor has none, else added in fp32 and
+ * rounded once; the same rule for captured calls; a current gradient sum becomes stale):
+ *   weight (+)= xhat^T dy  (cols x outs; transposed: outs x cols),   bias (+)= sum of dy's rows
+ * xhat: the values `kept` stands for (rows x cols); dy: rows x outs, of either type whatever the
+ * store's.  Products are exact (an fp32 dy goes in as three bf16 parts), sums in fp32.
+ * bias: a tensor index, or TTP_NO_TENSOR. */
+#define TTP_NO_TENSOR 0xFFFFFFFFu
+int ttp_accumulate_linear_grad8(ttp_ctx* ctx, uint32_t weight, uint32_t bias,
+                                const ttp_checkpoint8* kept, const ttp_matrix* dy,
+                                int transposed);
+
 /* ---- per-kernel timing (HIP events on the context's stream) ------------------------------ */
 #define TTP_KERNEL_NORM 0   /* grad-norm / inf-check pass and the step's decisions */
 #define TTP_KERNEL_UPDATE 1 /* fused multi-tensor update pass               */

@@ -9,7 +9,7 @@ import pytest
 from conftest import REPO
 from test_isa_cpu import HIPCC, PKG, scc_reads_live_into_a_block
 
-OPERATOR_FILES = ("losses", "checkpoint8")
+OPERATOR_FILES = ("losses", "checkpoint8", "linear_grad8")
 
 
 def test_struct_layouts_match_the_header(tmp_path):
@@ -47,6 +47,8 @@ def test_a_null_context_is_refused():
     assert L.lib.ttp_checkpoint8_pack(None, C.byref(m), C.byref(k)) == L.ERR_INVALID
     assert L.lib.ttp_checkpoint8_restore(None, C.byref(k), C.byref(m)) == L.ERR_INVALID
     assert L.lib.ttp_gelu_checkpoint8(None, C.byref(m), 0, C.byref(m), C.byref(k)) == \
+        L.ERR_INVALID
+    assert L.lib.ttp_accumulate_linear_grad8(None, 0, 1, C.byref(k), C.byref(m), 0) == \
         L.ERR_INVALID
     assert L.lib.ttp_gelu_backward8(None, C.byref(k), 0, C.byref(m), C.byref(m)) == L.ERR_INVALID
 

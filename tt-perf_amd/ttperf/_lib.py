@@ -27,6 +27,7 @@ STEP_SLOTS = 64  # step counts ttp_swap_step keeps
 CHECKPOINT_INT8, CHECKPOINT_E4M3 = 0, 1
 CHECKPOINT_BLOCK = 32  # columns that share a scale
 GELU_ERF, GELU_TANH = 0, 1
+NO_TENSOR = 0xFFFFFFFF
 STEP_TENSOR_SUMS = 1
 STEP_DEFER_SCALE = 2
 KERNEL_NORM, KERNEL_UPDATE = 0, 1
@@ -149,6 +150,8 @@ SIGNATURES = {
                                        C.POINTER(Checkpoint8)]),
     "ttp_gelu_backward8": (C.c_int, [_P, C.POINTER(Checkpoint8), C.c_int, C.POINTER(Matrix),
                                      C.POINTER(Matrix)]),
+    "ttp_accumulate_linear_grad8": (C.c_int, [_P, C.c_uint32, C.c_uint32, C.POINTER(Checkpoint8),
+                                              C.POINTER(Matrix), C.c_int]),
     "ttp_timing_enable": (C.c_int, [_P, C.c_int]),
     "ttp_timing_collect": (C.c_int, [_P, C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_uint64)]),
     "ttp_last_error": (C.c_char_p, []),

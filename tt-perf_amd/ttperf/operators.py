@@ -326,6 +326,22 @@ class Operators:
             self._h, C.byref(k), approx, C.byref(a), C.byref(b)))
         return out
 
+    def accumulate_linear_grad8(self, index, kept, dy, *, bias=None, transposed=False):
+        """Add a linear layer's gradients to the store's: tensor `index` receives xhat^T dy
+        (cols x outs, the layout of py/nn.py:36; transposed=True: outs x cols, torch.nn.Linear's)
+        and tensor `bias` the sum of dy's rows, with xhat what the Checkpoint8 `kept` of the
+        layer's input stands for and dy (..., outs), float32 or bfloat16.  As accumulate_grad: the
+        first gradient of a tensor is assigned, a further one added in fp32 and rounded once.
+        (ttp_accumulate_linear_grad8)"""
+        self._check_kept(kept)
+        g = self._rows_of(dy, "dy")
+        if tuple(dy.shape[:-1]) != kept.shape[:-1]:
+            raise ValueError(f"dy has shape {tuple(dy.shape)}, the checkpoint {kept.shape}")
+        a, k = _matrix(g), kept._c()
+        self._queue((kept.values, kept.scales, g), lambda: L.lib.ttp_accumulate_linear_grad8(
+            self._h, index, L.NO_TENSOR if bias is None else bias, C.byref(k), C.byref(a),
+            1 if transposed else 0))
+
     def _like(self, out, x, what):
         """The matrix of a result that has x's shape and type."""
         import torch
