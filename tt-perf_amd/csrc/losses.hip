@@ -18,6 +18,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "context.hpp"
 #include "device.hpp"
@@ -29,43 +30,95 @@ namespace {
 
 // ---- (maximum, sum of exponentials) ---------------------------------------------------------
 struct Stat {
-    float m, s;  // s = sum exp(z - m); nothing yet: (-inf, 0)
+    float m, s;  // s = sum exp(z - m); nothing: (-inf, 0)
 };
 // What the exponents are taken from: an all -inf part has the sum 0, not exp(-inf + inf).
 __device__ __forceinline__ float stat_base(float m) { return m == -INFINITY ? 0.0f : m; }
+// exp(z - base).  The difference first: one fused operation on z log2 e would leave the rounding
+// of base log2 e in every row, and overflow at the type's lowest value.
+__device__ __forceinline__ float power(float z, float base) {
+    return exp2_fast((z - base) * kLog2e);
+}
 
-__device__ __forceinline__ Stat join(Stat a, Stat b) {
-    const float m = fmaxf(a.m, b.m), base = stat_base(m);
-    return {m, a.s * exp2_fast((a.m - base) * kLog2e) + b.s * exp2_fast((b.m - base) * kLog2e)};
+// The wave's sum or maximum in every lane, by a butterfly without LDS permutes (see wave_sum).
+template <int kCtrl>
+__device__ __forceinline__ float dpp(float x) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), kCtrl,
+                                                                 0xF, 0xF, true));
 }
-template <int N>
-__device__ __forceinline__ Stat join(Stat a, const float (&v)[N]) {
-    float m = a.m;
-#pragma unroll
-    for (int k = 0; k < N; ++k) m = fmaxf(m, v[k]);  // (skips NaN, which the sum then holds)
-    const float base = stat_base(m);
-    float s = a.s * exp2_fast((a.m - base) * kLog2e);
-#pragma unroll
-    for (int k = 0; k < N; ++k) s += exp2_fast((v[k] - base) * kLog2e);
-    return {m, s};
+template <class F>
+__device__ __forceinline__ float wave_all(float x, F&& f) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                    false);
+    x = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false,
+                                                    false);
+    x = f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+    x = f(x, dpp<0x128>(x));  // row_ror:8
+    x = f(x, dpp<0x124>(x));  // row_ror:4
+    x = f(x, dpp<0x4E>(x));   // quad_perm:[2,3,0,1]
+    return f(x, dpp<0xB1>(x));  // quad_perm:[1,0,3,2]
 }
-__device__ __forceinline__ Stat shfl_xor(Stat a, int off) {
-    return {__shfl_xor(a.m, off), __shfl_xor(a.s, off)};
+__device__ __forceinline__ float wave_max(float x) {
+    return wave_all(x, [](float a, float b) { return fmaxf(a, b); });
 }
-// The block's, in every lane of it.
-template <int kThreads>
-__device__ __forceinline__ Stat block_join(Stat a, Stat* lds) {
+__device__ __forceinline__ float wave_add(float x) {
+    return wave_all(x, [](float a, float b) { return a + b; });
+}
+
+constexpr uint32_t kNone16 = 0xFF80FF80u, kNone32 = 0xFF800000u;  // -inf
+template <class T>
+__device__ __forceinline__ u32x4 no_logits() {
+    const uint32_t n = sizeof(T) == 2 ? kNone16 : kNone32;
+    return u32x4{n, n, n, n};
+}
+
+// A wave's statistics of its lanes' kLoads chunks and one more logit each (-inf where a lane has
+// none): the wave's maximum first, so that no sum has to be rescaled.  kLean: the chunks are
+// unpacked again for the sum (kept from the maximum, their values take twice the registers).
+template <class T, int kLoads, bool kLean>
+__device__ __forceinline__ Stat wave_stat(u32x4* w, float extra) {
+    constexpr int P = kPer<T>;
+    float m = extra;
 #pragma unroll
-    for (int off = 32; off; off >>= 1) a = join(a, shfl_xor(a, off));
-    if constexpr (kThreads > 64) {
-        if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = a;
-        __syncthreads();
-        a = lds[0];
+    for (int k = 0; k < kLoads; ++k) {
+        float v[P];
+        unpack(w[k], v, (const T*)nullptr);
 #pragma unroll
-        for (int w = 1; w < kThreads / 64; ++w) a = join(a, lds[w]);
-        __syncthreads();
+        for (int j = 0; j < P; ++j) m = fmaxf(m, v[j]);  // (skips NaN, which the sum then holds)
     }
-    return a;
+    m = wave_max(m);
+    if constexpr (kLean) {
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k) asm volatile("" : "+v"(w[k]));
+    }
+    const float base = stat_base(m);
+    float s = power(extra, base);
+#pragma unroll
+    for (int k = 0; k < kLoads; ++k) {
+        float v[P];
+        unpack(w[k], v, (const T*)nullptr);
+#pragma unroll
+        for (int j = 0; j < P; ++j) s += power(v[j], base);
+    }
+    return {m, wave_add(s)};
+}
+
+// A row's parts 0 .. splits - 1 together, f(k) giving part k: `lanes` lanes (a power of two, at
+// most a wave) take every lanes-th, each in order.  The result is in all of them.
+template <class F>
+__device__ __forceinline__ Stat join_parts(uint32_t splits, uint32_t lanes, F&& f) {
+    const uint32_t p = threadIdx.x % lanes;
+    float m = -INFINITY, s = 0.0f;
+    for (uint32_t k = p; k < splits; k += lanes) m = fmaxf(m, f(k).m);
+    for (uint32_t off = lanes / 2; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, (int)off));
+    const float base = stat_base(m);
+    for (uint32_t k = p; k < splits; k += lanes) {
+        const Stat x = f(k);
+        s += x.s * power(x.m, base);
+    }
+    for (uint32_t off = lanes / 2; off; off >>= 1) s += __shfl_xor(s, (int)off);
+    return {m, s};
 }
 
 // ---- a row's part of the loss ---------------------------------------------------------------
@@ -89,11 +142,12 @@ struct RowArgs {
     float clip_lo, clip_hi, kl_coef;
 };
 
+// The token's logit; past the vocabulary NaN.  (A masked row's is not asked for.)
 template <class T>
-__device__ __forceinline__ float row_logp(const RowArgs& a, uint64_t row, int64_t y, Stat st) {
-    if (y < 0) return 0.0f;
-    if (y >= (int64_t)a.cols) return NAN;
-    const float zy = widen(((const T*)a.z)[row * a.stride + (uint64_t)y]);
+__device__ __forceinline__ float token_logit(const RowArgs& a, uint64_t row, int64_t y) {
+    return y < (int64_t)a.cols ? widen(((const T*)a.z)[row * a.stride + (uint64_t)y]) : NAN;
+}
+__device__ __forceinline__ float row_logp(float zy, Stat st) {
     return (zy - st.m) - logf(st.s);
 }
 
@@ -127,7 +181,7 @@ __device__ __forceinline__ PolicyRow policy_row(const RowArgs& a, uint64_t row, 
 template <class T, Loss kLoss>
 __device__ __forceinline__ void finish_row(const RowArgs& a, uint64_t row, Stat st) {
     const int64_t y = a.targets[row];
-    const float logp = row_logp<T>(a, row, y, st);
+    const float logp = y < 0 ? 0.0f : row_logp(token_logit<T>(a, row, y), st);
     a.logps[row] = logp;
     if constexpr (kLoss == kPreference) {
         a.part[row] = y < 0 ? 0.0 : (double)logp - (a.ref ? (double)a.ref[row] : 0.0);
@@ -144,79 +198,125 @@ __device__ __forceinline__ void finish_row(const RowArgs& a, uint64_t row, Stat 
 }
 
 // ---- row_scores_kernel ------------------------------------------------------------------------
+// A row is cut into 16-byte chunks from its first element on, its last elements (fewer than a
+// chunk) by themselves, and the chunks into parts of 256, one wave's four loads per lane.  Which
+// lane takes what, and in which order sums are joined, depends on the number of columns alone: a
+// row's bits do not depend on where it lies.
 constexpr int kRowBlock = 256;
-constexpr int kAhead = 4;  // 16-byte loads in flight per lane
+constexpr int kLoads = 4;
+constexpr uint32_t kPart = kLoads * 64;
 
-// The statistics of z[lo, hi) (each lane its share); hi - lo a whole number of 16-byte chunks but
-// for the row's last part.
-template <class T, int kThreads>
-__device__ __forceinline__ Stat part_stats(const T* z, uint32_t lo, uint32_t hi) {
-    constexpr int P = kPer<T>;
-    const uint32_t chunks = (hi - lo) / P;
-    Stat st = {-INFINITY, 0.0f};
-    uint32_t c = threadIdx.x;
-    for (; c + (kAhead - 1) * kThreads < chunks; c += kAhead * kThreads) {
-        u32x4 w[kAhead];
+// One part on its way through a wave: where it is, whether its row counts, its logits.
+template <class T>
+struct Part {
+    uint64_t row;
+    uint32_t part;
+    bool live;
+    u32x4 w[kLoads];
+    float extra;
+
+    __device__ __forceinline__ void look(const RowArgs& a) {
+        live = row < a.rows && a.targets[row] >= 0;  // a masked row's logits are not read
+    }
+    // (kOnce: no gradient kernel reads them again soon)
+    template <bool kOnce>
+    __device__ __forceinline__ void load(const RowArgs& a, uint32_t splits) {
+        constexpr int P = kPer<T>;
+        const uint32_t chunks = a.cols / P, lane = threadIdx.x & 63;
+        const T* z = (const T*)a.z + row * a.stride;
+        extra = -INFINITY;
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) w[k] = load16(z + lo + (uint64_t)(c + k * kThreads) * P);
+        for (int k = 0; k < kLoads; ++k) w[k] = no_logits<T>();
+        if (!live) return;
 #pragma unroll
-        for (int k = 0; k < kAhead; ++k) {
-            float v[P];
-            unpack(w[k], v, z);
-            st = join(st, v);
+        for (int k = 0; k < kLoads; ++k) {
+            const uint32_t c = part * kPart + k * 64 + lane;
+            const T* p = z + (uint64_t)c * P;
+            if (c < chunks) w[k] = kOnce ? load16_once(p) : load16(p);
         }
+        const uint32_t e = chunks * P + lane;
+        if (part + 1 == splits && e < a.cols) extra = widen(z[e]);
     }
-    for (; c < chunks; c += kThreads) {
-        float v[P];
-        unpack(load16(z + lo + (uint64_t)c * P), v, z);
-        st = join(st, v);
-    }
-    const uint32_t at = lo + chunks * P + threadIdx.x;
-    if (at < hi) {
-        const float v[1] = {widen(z[at])};
-        st = join(st, v);
-    }
-    return st;
-}
+};
 
-// Block b: part b % splits of row b / splits (b + k gridDim.x: of a further row).  splits > 1:
-// every block has one item, and the launch's last block joins the parts of all rows.
+// Wave i: part i % splits of row i / splits, and on by the launch's waves.  With `last_joins`
+// (every wave then has one part) the launch's last block joins the rows' parts, else
+// finish_rows_kernel does; rows of one part are finished at once.
+// Bound by reading the logits.  Parts rather than rows per block: the waves in flight then sweep a
+// narrow window of memory.
 template <class T, Loss kLoss>
 __global__ __launch_bounds__(kRowBlock) void row_scores_kernel(RowArgs a, uint32_t splits,
-                                                               uint32_t per, double* parts,
+                                                               uint32_t lanes, double* parts,
+                                                               uint32_t last_joins,
                                                                uint32_t* tickets) {
-    __shared__ Stat lds[kRowBlock / 64];
-    __shared__ uint32_t last;
-    const uint64_t items = a.rows * splits;
-    for (uint64_t i = blockIdx.x; i < items; i += gridDim.x) {
-        const uint64_t row = i / splits;
-        const uint32_t part = (uint32_t)(i - row * splits);
-        Stat st = {-INFINITY, 0.0f};
-        if (a.targets[row] >= 0) {  // a masked row's logits are not read
-            const uint32_t lo = part * per;
-            const uint32_t hi = part + 1 == splits ? a.cols : lo + per;
-            st = part_stats<T, kRowBlock>((const T*)a.z + row * a.stride, lo, hi);
-            st = block_join<kRowBlock>(st, lds);
+    constexpr uint32_t kWaves = kRowBlock / 64;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    // a step of all the launch's waves, as rows and parts: no division per part
+    const uint32_t step = gridDim.x * kWaves;
+    const uint32_t step_rows = step / splits, step_parts = step - step_rows * splits;
+    const auto advance = [&](Part<T>& p) {
+        p.row += step_rows;
+        p.part += step_parts;
+        if (p.part >= splits) {
+            p.part -= splits;
+            p.row += 1;
         }
-        if (threadIdx.x == 0) {
+        p.look(a);
+    };
+    // the next part's logits and the one after's target are on their way while one is summed
+    Part<T> now, next;
+    const uint32_t first = blockIdx.x * kWaves + wave;
+    now.row = first / splits;
+    now.part = first - (uint32_t)now.row * splits;
+    now.look(a);
+    next.row = now.row;
+    next.part = now.part;
+    advance(next);
+    constexpr bool kOnce = kLoss == kScore;
+    now.template load<kOnce>(a, splits);
+    while (now.row < a.rows) {
+        next.template load<kOnce>(a, splits);
+        Stat st = {-INFINITY, 0.0f};
+        if (now.live) st = wave_stat<T, kLoads, false>(now.w, now.extra);
+        if ((threadIdx.x & 63) == 0) {
             if (splits == 1)
-                finish_row<T, kLoss>(a, row, st);
+                finish_row<T, kLoss>(a, now.row, st);
             else
-                st_device(parts + i, __builtin_bit_cast(double, st));
+                st_device(parts + now.row * splits + now.part, __builtin_bit_cast(double, st));
         }
+        now = next;
+        advance(next);
     }
-    if (splits == 1 || !is_last_block(tickets, &last)) return;
-    // `lanes` lanes per row (a power of two, at most a wave), each one part
-    uint32_t lanes = 1;
-    while (lanes < splits) lanes *= 2;
-    const uint32_t p = threadIdx.x % lanes, step = kRowBlock / lanes;
-    for (uint64_t base = 0; base < a.rows; base += step) {
-        const uint64_t row = base + threadIdx.x / lanes;
-        Stat st = {-INFINITY, 0.0f};
-        if (row < a.rows && p < splits)
-            st = __builtin_bit_cast(Stat, ld_device(parts + row * splits + p));
-        for (uint32_t off = lanes / 2; off; off >>= 1) st = join(st, shfl_xor(st, (int)off));
-        if (row < a.rows && p == 0) finish_row<T, kLoss>(a, row, st);
+    if (!last_joins) return;
+    __shared__ uint32_t last;
+    // every wave's parts are at memory before the block takes its ticket
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (!is_last_block(tickets, &last)) return;
+    const uint32_t rows = kRowBlock / lanes;
+    for (uint64_t base = 0; base < a.rows; base += rows) {
+        const uint64_t row = min(base + threadIdx.x / lanes, a.rows - 1);
+        const Stat st = join_parts(splits, lanes, [&](uint32_t k) {
+            return __builtin_bit_cast(Stat, ld_device(parts + row * splits + k));
+        });
+        if (base + threadIdx.x / lanes < a.rows && threadIdx.x % lanes == 0)
+            finish_row<T, kLoss>(a, row, st);
+    }
+}
+template <class T, Loss kLoss>
+__global__ __launch_bounds__(kRowBlock) void finish_rows_kernel(RowArgs a, uint32_t splits,
+                                                                uint32_t lanes,
+                                                                const double* parts) {
+    const uint32_t rows = kRowBlock / lanes;
+    for (uint64_t base = (uint64_t)blockIdx.x * rows; base < a.rows;
+         base += (uint64_t)gridDim.x * rows) {
+        const uint64_t row = min(base + threadIdx.x / lanes, a.rows - 1);
+        const Stat st = join_parts(splits, lanes, [&](uint32_t k) {
+            return __builtin_bit_cast(Stat, parts[row * splits + k]);
+        });
+        if (base + threadIdx.x / lanes < a.rows && threadIdx.x % lanes == 0)
+            finish_row<T, kLoss>(a, row, st);
     }
 }
 
@@ -281,7 +381,7 @@ constexpr uint32_t kSumBlocks = 64;
 struct SumArgs {
     const int64_t* targets;
     uint64_t rows, per;  // rows per block
-    const double *part, *part_kl;
+    const double *part, *part_kl;  // null: the norm alone
     double* sums;      // 3 per block
     double denominator;  // 0: the unmasked rows
     const float* loss_scale;
@@ -295,8 +395,10 @@ __global__ __launch_bounds__(kBlock) void row_sums_kernel(SumArgs a, uint32_t* t
     double x[3] = {0.0, 0.0, 0.0};
     for (uint64_t t = lo + threadIdx.x; t < hi; t += kBlock) {
         x[0] += a.targets[t] >= 0 ? 1.0 : 0.0;
-        x[1] += a.part[t];
-        x[2] += a.part_kl[t];
+        if (a.part) {
+            x[1] += a.part[t];
+            x[2] += a.part_kl[t];
+        }
     }
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
@@ -311,8 +413,10 @@ __global__ __launch_bounds__(kBlock) void row_sums_kernel(SumArgs a, uint32_t* t
     }
     if (threadIdx.x == 0) {
         const double d = a.denominator > 0.0 ? a.denominator : fmax(x[0], 1.0);
-        *a.loss = (float)(x[1] / d);
-        *a.kl = (float)(x[2] / d);
+        if (a.part) {
+            *a.loss = (float)(x[1] / d);
+            *a.kl = (float)(x[2] / d);
+        }
         *a.norm = (float)((a.loss_scale ? (double)*a.loss_scale : 1.0) / d);
     }
 }
@@ -328,97 +432,297 @@ struct GradArgs {
     const float* coef;
     const float* norm;  // null: 1
 };
-// Block b: part b % splits of row b / splits.  Each element is read before it is written by the
-// same lane, so the gradient may take the logits' place.
+constexpr int kGradBlock = 256;
+constexpr uint32_t kGradPart = 512;  // chunks of a part: two for each lane
+// The row's values: f exp(z - m), f = -c / s.
 template <class T>
-__global__ __launch_bounds__(kRowBlock) void row_grads_kernel(GradArgs a, uint32_t splits,
-                                                              uint32_t per) {
-    constexpr int P = kPer<T>;
-    const uint64_t items = a.rows * splits;
+__device__ __forceinline__ u32x4 grad16(u32x4 w, const T* type, float f, float m) {
+    float v[kPer<T>];
+    unpack(w, v, type);
+#pragma unroll
+    for (int k = 0; k < kPer<T>; ++k) v[k] = f * power(v[k], m);
+    return pack(v, type);
+}
+
+// Block b: part b % splits of row b / splits (kLanes 64: four rows per block, of at most 128
+// chunks).  Each element is read before it is written by the same lane, so the gradient may take
+// the logits' place.
+template <class T, int kLanes>
+__global__ __launch_bounds__(kGradBlock) void row_grads_kernel(GradArgs a, uint32_t splits) {
+    constexpr int P = kPer<T>, kRows = kGradBlock / kLanes, kLoads = 2;
+    const uint32_t t = threadIdx.x % kLanes, chunks = a.cols / P;
+    const uint64_t items = (a.rows + kRows - 1) / kRows * splits;
     for (uint64_t i = blockIdx.x; i < items; i += gridDim.x) {
-        const uint64_t row = i / splits;
-        const uint32_t part = (uint32_t)(i - row * splits);
-        const uint32_t lo = part * per, hi = part + 1 == splits ? a.cols : lo + per;
-        const uint32_t chunks = (hi - lo) / P;
-        const T* z = (const T*)a.z + row * a.z_stride + lo;
-        T* g = (T*)a.g + row * a.g_stride + lo;
+        const uint64_t group = i / splits;
+        const uint32_t part = (uint32_t)(i - group * splits);
+        const uint64_t row = group * kRows + __builtin_amdgcn_readfirstlane(threadIdx.x / kLanes);
+        if (kRows > 1 && row >= a.rows) continue;
+        const T* z = (const T*)a.z + row * a.z_stride;
+        T* g = (T*)a.g + row * a.g_stride;
         const int64_t y = a.targets[row];
         const float c = a.coef[row] * (a.norm ? *a.norm : 1.0f);
         const Stat st = a.stats[row];
-        const uint32_t tail = chunks * P + threadIdx.x;
+        const uint32_t first = part * kGradPart + t;
+        const uint32_t e = part + 1 == splits ? chunks * P + t : a.cols;
         if (y < 0 || c == 0.0f) {
             // a row that does not count, or not at all (c = 0, of a masked row, of one in no
             // sequence, of a clipped ratio): zeros, also where its logits are not finite
-            for (uint32_t k = threadIdx.x; k < chunks; k += kRowBlock)
-                store16(g + (uint64_t)k * P, u32x4{0, 0, 0, 0});
-            if (tail < hi - lo) narrow(0.0f, g + tail);
+#pragma unroll
+            for (int k = 0; k < kLoads; ++k)
+                if (first + k * kLanes < chunks)
+                    store16_once(g + (uint64_t)(first + k * kLanes) * P, u32x4{0, 0, 0, 0});
+            if (e < a.cols) narrow(0.0f, g + e);
             continue;
         }
-        // past the vocabulary (its logp and c are NaN): no element
-        const uint32_t at = y < (int64_t)a.cols ? (uint32_t)y - lo : ~0u;
         const float f = -c / st.s;
-        for (uint32_t k = threadIdx.x; k < chunks; k += kRowBlock) {
-            float v[P];
-            unpack(load16(z + (uint64_t)k * P), v, z);
+        u32x4 w[kLoads];
+        float zy = 0.0f;
+        // the token's chunk (this lane's, or none of its): c more, in fp32
+        const uint64_t cy = (uint64_t)y / P;
+        const bool own = y < (int64_t)a.cols && cy < chunks &&
+                         (cy == first || cy == first + (uint64_t)kLanes);
 #pragma unroll
-            for (int j = 0; j < P; ++j) {
-                v[j] = f * exp2_fast((v[j] - st.m) * kLog2e);
-                if (k * P + j == at) v[j] += c;
+        for (int k = 0; k < kLoads; ++k)
+            if (first + k * kLanes < chunks)
+                w[k] = load16_once(z + (uint64_t)(first + k * kLanes) * P);
+        if (own) zy = widen(z[y]);
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k)
+            if (first + k * kLanes < chunks)
+                store16_once(g + (uint64_t)(first + k * kLanes) * P, grad16(w[k], z, f, st.m));
+        if (own) narrow(f * power(zy, st.m) + c, g + y);
+        if (e < a.cols) {
+            const float v = f * power(widen(z[e]), st.m);
+            narrow((int64_t)e == y ? v + c : v, g + e);
+        }
+    }
+}
+
+// ---- policy_rows_kernel -------------------------------------------------------------------------
+// The policy loss and its gradient in one pass: a row's logits stay in kThreads lanes' registers
+// (kChunks 16-byte chunks each) from the statistics to the gradient, which needs nothing of other
+// rows but their number (a.norm, known before).  One row per kThreads lanes; without a gradient
+// (o.g null) the losses alone.  The statistics are taken and joined part by part as
+// row_scores_kernel and its joins do, so that a token's log-probability has the same bits here as
+// there: the first step on a rollout finds ratios of exactly 1.
+template <class T, int kThreads, int kChunks>
+__global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void policy_rows_kernel(RowArgs a,
+                                                                                     GradArgs o) {
+    constexpr int P = kPer<T>;
+    constexpr bool kWaves = kThreads == 64;  // a row is a wave, and one part
+    constexpr int kRows = kWaves ? 4 : 1;
+    constexpr uint32_t kGroups = kThreads / 64;
+    constexpr int kParts = (kChunks + kLoads - 1) / kLoads;  // of a wave
+    static_assert(kChunks % kLoads == 0 || kParts == 1);
+    __shared__ Stat lds[kWaves ? 1 : kGroups * kParts];
+    __shared__ float token;  // (a row per block) the token's logit, read before its place is written
+    const uint32_t t = threadIdx.x % kThreads, lane = t & 63, chunks = a.cols / P;
+    // (the same in a wave: its addresses are one scalar and 32 bits per lane)
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint64_t row = (uint64_t)blockIdx.x * kRows + (kWaves ? wave : 0);
+    if (row >= a.rows) return;  // (whole waves, and only where a row is a wave)
+    const T* z = (const T*)a.z + row * a.stride;
+    T* g = (T*)o.g + row * o.g_stride;
+    const int64_t y = a.targets[row];
+    const uint32_t splits = kWaves ? 1 : (chunks + kPart - 1) / kPart;
+    // chunk k of this lane; and for the lanes of the last part's wave the row's last elements
+    const auto chunk = [&](int k) {
+        return kWaves ? lane + k * 64
+                      : (wave + k / kLoads * kGroups) * kPart + k % kLoads * 64 + lane;
+    };
+    const uint32_t e = kWaves || (splits - 1) % kGroups == wave ? chunks * P + lane : a.cols;
+    // f(k, its bytes from the row's start) for this lane's chunks in the row
+    const auto each = [&](auto&& f) {
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k)
+            if (chunk(k) < chunks) f(k, chunk(k) * 16);
+    };
+    const auto zeros = [&]() {
+        each([&](int, uint32_t b) { store16_once((T*)((char*)g + b), u32x4{0, 0, 0, 0}); });
+        if (e < a.cols) narrow(0.0f, g + e);
+    };
+    if (y < 0) {
+        if (t == 0) {
+            a.logps[row] = 0.0f;
+            a.part[row] = a.part_kl[row] = 0.0;
+        }
+        if (o.g) zeros();
+        return;
+    }
+    u32x4 w[kChunks];
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k) w[k] = no_logits<T>();
+    each([&](int k, uint32_t b) { w[k] = load16_once((const T*)((const char*)z + b)); });
+    const float ze = e < a.cols ? widen(z[e]) : -INFINITY;
+    float zy = 0.0f;
+    if (kWaves || t == 0) zy = token_logit<T>(a, row, y);
+    Stat st;
+    if constexpr (kWaves) {
+        st = wave_stat<T, kChunks, true>(w, ze);
+    } else {
+        if (t == 0) token = zy;
+#pragma unroll
+        for (int j = 0; j < kParts; ++j) {
+            const uint32_t part = wave + j * kGroups;
+            if (part < splits) {
+                st = wave_stat<T, kLoads, true>(w + kLoads * j,
+                                                part + 1 == splits ? ze : -INFINITY);
+                if (lane == 0) lds[part] = st;
             }
-            store16(g + (uint64_t)k * P, pack(v, z));
         }
-        if (tail < hi - lo) {
-            float v = f * exp2_fast((widen(z[tail]) - st.m) * kLog2e);
-            if (tail == at) v += c;
-            narrow(v, g + tail);
-        }
+        __syncthreads();
+        zy = token;
+        uint32_t lanes = 1;
+        while (lanes < splits && lanes < 64) lanes *= 2;
+        st = join_parts(splits, lanes, [&](uint32_t k) { return lds[k]; });
+    }
+    // every lane for itself: a second wait for one lane's result costs more
+    const float logp = row_logp(zy, st);
+    const PolicyRow p = policy_row(a, row, logp);
+    if (t == 0) {
+        a.logps[row] = logp;
+        a.part[row] = (double)p.loss;
+        a.part_kl[row] = (double)p.kl;
+    }
+    if (!o.g) return;
+    const float c = p.coef * *o.norm;
+    if (c == 0.0f) {
+        zeros();
+        return;
+    }
+    const float f = -c / st.s;
+    // the packed registers are unpacked once more: kept from before, the values would take two
+    // to four times the registers
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k) asm volatile("" : "+v"(w[k]));
+    // a row off the 16-byte grid: its stores share cache lines, which L2 puts together
+    if ((uintptr_t)g % 16 == 0)
+        each([&](int k, uint32_t b) {
+            store16_once((T*)((char*)g + b), grad16(w[k], z, f, st.m));
+        });
+    else
+        each([&](int k, uint32_t b) {
+            store16((T*)((char*)g + b), grad16(w[k], z, f, st.m));
+        });
+    if (e < a.cols) {
+        const float v = f * power(ze, st.m);
+        narrow((int64_t)e == y ? v + c : v, g + e);
+    }
+    // the token's own: c more, in fp32, by the lane that has written its chunk
+    const uint64_t cy = (uint64_t)y / P;
+    if (cy < chunks) {
+        const uint32_t x = (uint32_t)cy;
+        const uint32_t owner = kWaves ? x % 64 : x / kPart % kGroups * 64 + x % 64;
+        if (owner == t) narrow(f * power(zy, st.m) + c, g + y);
     }
 }
 
 // ---- launches -----------------------------------------------------------------------------------
 uint32_t grid_of(uint64_t items) { return (uint32_t)std::min<uint64_t>(items, 1u << 22); }
 
-// Rows are split over the vocabulary until the launch has about four blocks for each CU; a part
-// is a whole number of 16-byte chunks, 8 KiB at least, a row in 64 parts at most.
-struct Split {
-    uint32_t splits, per;
-};
-Split split_rows(uint64_t rows, uint32_t cols, uint32_t size, int cus) {
-    const uint64_t row_bytes = (uint64_t)cols * size;
-    uint64_t n = rows ? std::max<uint64_t>((uint64_t)cus * 4 / rows, 1) : 1;
-    n = std::max<uint64_t>(std::min({n, (uint64_t)64, row_bytes / 8192}), 1);
-    const uint32_t unit = 16 / size;
-    const uint32_t per = (uint32_t)(((cols + n - 1) / n + unit - 1) / unit * unit);
-    const uint32_t splits = std::max<uint32_t>((cols + per - 1) / per, 1);
-    return {splits, per};
+uint32_t row_chunks(uint32_t cols, int dtype) {
+    return cols / (16 / (uint32_t)ttpi::elem_size(dtype));
 }
 
-template <Loss kLoss>
-int launch_scores(const ttpi::Op& op, const RowArgs& a, int dtype, Split sp, double* parts) {
+// Up to 1024 parts in all are joined by the launch's last block (a row of 50257 bf16: one launch
+// instead of two), more by a launch of their own.
+struct Split {
+    uint32_t splits, lanes;
+    bool last_joins;
+    uint64_t parts;  // scratch entries
+};
+Split split_rows(uint64_t rows, uint32_t cols, int dtype) {
+    const uint32_t chunks = row_chunks(cols, dtype);
+    if (chunks <= kPart) return {1, 1, false, 0};
+    const uint32_t splits = (chunks + kPart - 1) / kPart;
+    uint32_t lanes = 1;
+    while (lanes < splits && lanes < 64) lanes *= 2;
+    return {splits, lanes, rows * splits <= 1024, rows * splits};
+}
+
+template <Loss kLoss, class T>
+int launch_scores_of(const ttpi::Op& op, const RowArgs& a, Split sp, double* parts) {
     if (!a.rows) return TTP_OK;
-    const dim3 grid(grid_of(a.rows * sp.splits)), block(kRowBlock);
+    // (four rounds of blocks that fit the GPU at once: each wave starts its next part while it
+    // sums one, and the rounds even out what masked rows leave)
+    const dim3 block(kRowBlock), grid((uint32_t)std::min<uint64_t>((a.rows * sp.splits + 3) / 4,
+                                                                   (uint64_t)op.num_cus * 32));
     (void)hipGetLastError();
-    if (dtype == TTP_DTYPE_BF16)
-        hipLaunchKernelGGL((row_scores_kernel<uint16_t, kLoss>), grid, block, 0, op.stream, a,
-                           sp.splits, sp.per, parts, op.tickets);
-    else
-        hipLaunchKernelGGL((row_scores_kernel<float, kLoss>), grid, block, 0, op.stream, a,
-                           sp.splits, sp.per, parts, op.tickets);
+    hipLaunchKernelGGL((row_scores_kernel<T, kLoss>), grid, block, 0, op.stream, a, sp.splits,
+                       sp.lanes, parts, sp.last_joins ? 1u : 0u, op.tickets);
+    TTPI_HIP(hipGetLastError());
+    if (sp.splits == 1 || sp.last_joins) return TTP_OK;
+    const uint64_t per_block = kRowBlock / sp.lanes;
+    hipLaunchKernelGGL((finish_rows_kernel<T, kLoss>),
+                       dim3(grid_of((a.rows + per_block - 1) / per_block)), block, 0, op.stream, a,
+                       sp.splits, sp.lanes, (const double*)parts);
     TTPI_HIP(hipGetLastError());
     return TTP_OK;
 }
+template <Loss kLoss>
+int launch_scores(const ttpi::Op& op, const RowArgs& a, int dtype, Split sp, double* parts) {
+    return dtype == TTP_DTYPE_BF16 ? launch_scores_of<kLoss, uint16_t>(op, a, sp, parts)
+                                   : launch_scores_of<kLoss, float>(op, a, sp, parts);
+}
 
-int launch_grads(const ttpi::Op& op, const GradArgs& a, int dtype) {
+template <class T>
+int launch_grads_of(const ttpi::Op& op, const GradArgs& a) {
     if (!a.rows) return TTP_OK;
-    const Split sp = split_rows(a.rows, a.cols, (uint32_t)ttpi::elem_size(dtype), op.num_cus);
-    const dim3 grid(grid_of(a.rows * sp.splits)), block(kRowBlock);
+    const uint32_t chunks = a.cols / kPer<T>;
     (void)hipGetLastError();
-    if (dtype == TTP_DTYPE_BF16)
-        hipLaunchKernelGGL(row_grads_kernel<uint16_t>, grid, block, 0, op.stream, a, sp.splits,
-                           sp.per);
-    else
-        hipLaunchKernelGGL(row_grads_kernel<float>, grid, block, 0, op.stream, a, sp.splits,
-                           sp.per);
+    if (chunks <= 128) {
+        hipLaunchKernelGGL((row_grads_kernel<T, 64>), dim3(grid_of((a.rows + 3) / 4)),
+                           dim3(kGradBlock), 0, op.stream, a, 1u);
+    } else {
+        const uint32_t splits = (chunks + kGradPart - 1) / kGradPart;
+        hipLaunchKernelGGL((row_grads_kernel<T, kGradBlock>), dim3(grid_of(a.rows * splits)),
+                           dim3(kGradBlock), 0, op.stream, a, splits);
+    }
+    TTPI_HIP(hipGetLastError());
+    return TTP_OK;
+}
+int launch_grads(const ttpi::Op& op, const GradArgs& a, int dtype) {
+    return dtype == TTP_DTYPE_BF16 ? launch_grads_of<uint16_t>(op, a)
+                                   : launch_grads_of<float>(op, a);
+}
+
+// The one-pass policy kernel's shape for rows of `chunks` chunks: f<lanes, chunks per lane>, or
+// false where no shape holds them.  1024 lanes, two rows or one on a CU (16384 rows of 50257 bf16
+// every 50304, so on the 16-byte grid: 575 us, 618 with 256 lanes; 1021 rows of 50257 fp32: 85.5
+// us, 88 with 512), but where rows lie anywhere and three of them fit a CU's registers, 256 lanes
+// (the same rows every 50257: 733 us, 765 with 1024 lanes).
+template <class F>
+bool policy_shape(uint32_t chunks, bool on_grid, F&& f) {
+#define TTP_SHAPE(T, C)                                                 \
+    if (chunks <= T * C) {                                              \
+        f(std::integral_constant<int, T>{}, std::integral_constant<int, C>{}); \
+        return true;                                                    \
+    }
+    TTP_SHAPE(64, 1)
+    TTP_SHAPE(64, 4)
+    TTP_SHAPE(256, 4)
+    TTP_SHAPE(256, 8)
+    TTP_SHAPE(256, 16)
+    if (!on_grid) {
+        TTP_SHAPE(256, 28)
+    }
+    TTP_SHAPE(1024, 8)
+    TTP_SHAPE(1024, 12)
+    TTP_SHAPE(1024, 16)
+    TTP_SHAPE(1024, 20)
+#undef TTP_SHAPE
+    return false;
+}
+template <class T>
+int launch_policy(const ttpi::Op& op, const RowArgs& a, const GradArgs& g) {
+    (void)hipGetLastError();
+    const bool on_grid = ((uintptr_t)a.z | a.stride * sizeof(T)) % 16 == 0;
+    policy_shape(a.cols / kPer<T>, on_grid, [&](auto lanes, auto chunks) {
+        constexpr int kLanes = lanes, kChunks = chunks, kRows = kLanes < 256 ? 256 / kLanes : 1;
+        hipLaunchKernelGGL((policy_rows_kernel<T, kLanes, kChunks>),
+                           dim3((uint32_t)((a.rows + kRows - 1) / kRows)),
+                           dim3(kLanes < 256 ? 256 : kLanes), 0, op.stream, a, g);
+    });
     TTPI_HIP(hipGetLastError());
     return TTP_OK;
 }
@@ -453,10 +757,9 @@ int ttp_token_logprobs(ttp_ctx* ctx, const ttp_matrix* logits, const int64_t* ta
         if ((rc = b.matrix(logits, rows, logits->cols, "the logits", false))) return rc;
         if ((rc = b.array(targets, rows, 8, "the targets", false))) return rc;
         if ((rc = b.array(logps, rows, 4, "the log-probabilities", true))) return rc;
-        const Split sp = split_rows(rows, (uint32_t)logits->cols,
-                                    (uint32_t)ttpi::elem_size(logits->dtype), op.num_cus);
+        const Split sp = split_rows(rows, (uint32_t)logits->cols, logits->dtype);
         void* parts = nullptr;
-        if (sp.splits > 1 && (rc = ttpi::workspace(ctx, rows * sp.splits * 8, &parts))) return rc;
+        if (sp.parts && (rc = ttpi::workspace(ctx, sp.parts * 8, &parts))) return rc;
         RowArgs a{};
         a.z = logits->data;
         a.rows = rows;
@@ -499,12 +802,11 @@ int ttp_preference_loss(ttp_ctx* ctx, const ttp_preference_args* p) {
         if ((rc = b.array(p->margins, p->pairs, 4, "the margins", true))) return rc;
         if ((rc = b.array(p->loss, 1, 4, "the loss", true))) return rc;
 
-        const Split sp = split_rows(rows, (uint32_t)cols,
-                                    (uint32_t)ttpi::elem_size(p->logits->dtype), op.num_cus);
+        const Split sp = split_rows(rows, (uint32_t)cols, p->logits->dtype);
         Scratch s;
         const uint64_t part = s.add(rows * 8), stats = s.add(rows * 8), coef = s.add(rows * 4),
                        pair_loss = s.add(p->pairs * 8),
-                       parts = s.add(sp.splits > 1 ? rows * sp.splits * 8 : 0);
+                       parts = s.add(sp.parts * 8);
         void* ws;
         if ((rc = ttpi::workspace(ctx, s.bytes, &ws))) return rc;
         char* w = (char*)ws;
@@ -581,12 +883,11 @@ int ttp_policy_loss(ttp_ctx* ctx, const ttp_policy_args* p) {
         if ((rc = b.array(p->loss, 1, 4, "the loss", true))) return rc;
         if ((rc = b.array(p->kl, 1, 4, "the mean k", true))) return rc;
 
-        const Split sp = split_rows(rows, (uint32_t)cols,
-                                    (uint32_t)ttpi::elem_size(p->logits->dtype), op.num_cus);
+        const Split sp = split_rows(rows, (uint32_t)cols, p->logits->dtype);
         Scratch s;
         const uint64_t part = s.add(rows * 8), part_kl = s.add(rows * 8), stats = s.add(rows * 8),
                        coef = s.add(rows * 4), sums = s.add(kSumBlocks * 3 * 8),
-                       norm = s.add(4), parts = s.add(sp.splits > 1 ? rows * sp.splits * 8 : 0);
+                       norm = s.add(4), parts = s.add(sp.parts * 8);
         void* ws;
         if ((rc = ttpi::workspace(ctx, s.bytes, &ws))) return rc;
         char* w = (char*)ws;
@@ -608,9 +909,6 @@ int ttp_policy_loss(ttp_ctx* ctx, const ttp_policy_args* p) {
         a.clip_lo = (float)(1.0 - p->clip_low);
         a.clip_hi = (float)(1.0 + p->clip_high);
         a.kl_coef = (float)p->kl_coef;
-        if ((rc = launch_scores<kPolicy>(op, a, p->logits->dtype, sp, (double*)(w + parts))))
-            return rc;
-
         SumArgs sa{};
         sa.targets = p->targets;
         sa.rows = rows;
@@ -618,22 +916,41 @@ int ttp_policy_loss(ttp_ctx* ctx, const ttp_policy_args* p) {
             (uint32_t)std::max<uint64_t>(std::min<uint64_t>((rows + kBlock - 1) / kBlock,
                                                             kSumBlocks), 1);
         sa.per = (rows + blocks - 1) / blocks;
-        sa.part = a.part;
-        sa.part_kl = a.part_kl;
         sa.sums = (double*)(w + sums);
         sa.denominator = p->denominator;
         sa.loss_scale = op.loss_scale;
         sa.loss = p->loss;
         sa.kl = p->kl;
         sa.norm = (float*)(w + norm);
-        (void)hipGetLastError();
-        hipLaunchKernelGGL(row_sums_kernel, dim3(blocks), dim3(kBlock), 0, op.stream, sa,
-                           op.tickets);
-        TTPI_HIP(hipGetLastError());
-        if (!p->grad) return TTP_OK;
-        GradArgs g{a.z,    p->grad->data, rows,    a.stride, p->grad->stride,
-                   a.cols, p->targets,    a.stats, a.coef,   sa.norm};
-        return launch_grads(op, g, p->logits->dtype);
+        const auto launch_sums = [&]() -> int {
+            (void)hipGetLastError();
+            hipLaunchKernelGGL(row_sums_kernel, dim3(blocks), dim3(kBlock), 0, op.stream, sa,
+                               op.tickets);
+            TTPI_HIP(hipGetLastError());
+            return TTP_OK;
+        };
+        GradArgs g{a.z,    p->grad ? p->grad->data : nullptr, rows, a.stride,
+                   p->grad ? p->grad->stride : 0, a.cols, p->targets, a.stats, a.coef, sa.norm};
+        // One pass where a row fits the registers of a block and the rows one launch: the number
+        // of rows that count first, the losses' sums behind it.
+        const bool one_pass =
+            rows && rows <= (1u << 21) &&
+            policy_shape(row_chunks((uint32_t)cols, p->logits->dtype), true, [](auto, auto) {});
+        if (one_pass) {
+            if (p->grad && (rc = launch_sums())) return rc;
+            rc = p->logits->dtype == TTP_DTYPE_BF16 ? launch_policy<uint16_t>(op, a, g)
+                                                    : launch_policy<float>(op, a, g);
+            if (rc) return rc;
+            sa.part = a.part;
+            sa.part_kl = a.part_kl;
+            return launch_sums();
+        }
+        if ((rc = launch_scores<kPolicy>(op, a, p->logits->dtype, sp, (double*)(w + parts))))
+            return rc;
+        sa.part = a.part;
+        sa.part_kl = a.part_kl;
+        if ((rc = launch_sums())) return rc;
+        return p->grad ? launch_grads(op, g, p->logits->dtype) : TTP_OK;
     });
 }
 

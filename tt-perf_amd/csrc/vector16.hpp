@@ -61,6 +61,15 @@ template <class T>
 __device__ __forceinline__ void store16(T* p, u32x4 w) {
     *reinterpret_cast<u32x4_any*>(p) = w;
 }
+// the same for what is read once, or not read again soon
+template <class T>
+__device__ __forceinline__ u32x4 load16_once(const T* p) {
+    return __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
+}
+template <class T>
+__device__ __forceinline__ void store16_once(T* p, u32x4 w) {
+    __builtin_nontemporal_store(static_cast<u32x4_any>(w), reinterpret_cast<u32x4_any*>(p));
+}
 
 }  // namespace
 }  // namespace ttp

@@ -14,6 +14,13 @@ from typing import Any, NamedTuple, Optional
 
 from . import _lib as L
 
+try:
+    import torch
+except ImportError:  # the optimizers do without it; the operators take its tensors
+    torch = None
+else:
+    _ROW_TYPES = (torch.bfloat16, torch.float32)
+
 
 class PreferenceLoss(NamedTuple):
     """loss (), margins (pairs,) and logps (rows,) in float32, and the logits' gradient (or
@@ -46,9 +53,8 @@ class Checkpoint8:
         self.rows = values.shape[0]
 
     def _c(self):
-        return L.Checkpoint8(values=self.values.data_ptr(), scales=self.scales.data_ptr(),
-                             rows=self.rows, cols=self.cols,
-                             format=_FORMATS[self.format], reserved=0)
+        return L.Checkpoint8(self.values.data_ptr(), self.scales.data_ptr(), self.rows, self.cols,
+                             _FORMATS[self.format], 0)
 
 
 _FORMATS = {"int8": L.CHECKPOINT_INT8, "e4m3": L.CHECKPOINT_E4M3}
@@ -63,11 +69,9 @@ def _choice(table, key, what):
 
 def _matrix(t):
     """The C view of a 2-D tensor whose rows are contiguous."""
-    import torch
     rows, cols = t.shape
-    stride = t.stride(0) if rows > 1 else cols
-    return L.Matrix(data=t.data_ptr(), rows=rows, cols=cols, stride=stride, reserved=0,
-                    dtype=L.DTYPE_BF16 if t.dtype == torch.bfloat16 else L.DTYPE_F32)
+    return L.Matrix(t.data_ptr(), rows, cols, t.stride(0) if rows > 1 else cols,
+                    L.DTYPE_BF16 if t.element_size() == 2 else L.DTYPE_F32, 0)
 
 
 def _ptr(t):
@@ -75,75 +79,74 @@ def _ptr(t):
 
 
 class Operators:
-    """Mixed into ParamStore."""
+    """Mixed into ParamStore.  (What runs on every call asks as little as it can: a call over one
+    row took 16 us of host time and takes HOST_US.)"""
 
     def _rows_of(self, t, what):
         """A 2-D view of a float32 or bfloat16 device tensor: all but its last dimension are
         rows (a tensor of one dimension is one row).  Nothing is copied: a layout that is no
         matrix of contiguous rows is refused."""
-        import torch
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or \
-                t.dtype not in (torch.float32, torch.bfloat16):
+        if not isinstance(t, torch.Tensor) or t.dtype not in _ROW_TYPES or not t.is_cuda:
             raise ValueError(f"{what} must be a float32 or bfloat16 tensor on the GPU")
-        if t.device.index != self.device:
+        if t.get_device() != self.device:
             raise ValueError(f"{what} is on {t.device}, the store on cuda:{self.device}")
-        t = t.detach()
-        if t.dim() == 0 or t.shape[-1] == 0:
+        shape = t.shape
+        if not shape or shape[-1] == 0:
             raise ValueError(f"{what} has no columns")
-        if t.dim() != 2:
+        if len(shape) != 2:
             try:
-                t = t.view(-1, t.shape[-1])
+                t = t.detach().view(-1, shape[-1])
             except RuntimeError:
                 raise ValueError(f"{what} must be a matrix of contiguous rows (or a view as "
                                  "one): make it contiguous first") from None
-        if t.numel() and ((t.shape[1] > 1 and t.stride(1) != 1) or
-                          (t.shape[0] > 1 and t.stride(0) < t.shape[1])):
-            raise ValueError(f"{what} must have contiguous rows that do not overlap: make it "
-                             "contiguous first")
+        if not t.is_contiguous():
+            (rows, cols), (pitch, one) = t.shape, t.stride()
+            if (cols > 1 and one != 1) or (rows > 1 and pitch < cols):
+                raise ValueError(f"{what} must have contiguous rows that do not overlap: make it "
+                                 "contiguous first")
         return t
 
     def _vector_of(self, t, n, dtype, what):
-        """A contiguous 1-D device tensor of n elements of `dtype` (a copy where it is not)."""
-        import torch
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype:
+        """A contiguous device tensor of n elements of `dtype` (a copy where it is not)."""
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype or not t.is_cuda:
             raise ValueError(f"{what} must be a {str(dtype)[6:]} tensor on the GPU")
-        if t.device.index != self.device:
+        if t.get_device() != self.device:
             raise ValueError(f"{what} is on {t.device}, the store on cuda:{self.device}")
         if t.numel() != n:
             raise ValueError(f"{what}: expected {n} elements, got {t.numel()}")
-        t = t.detach()
-        if self._in_capture and not t.is_contiguous():
+        if t.is_contiguous():
+            return t
+        if self._in_capture:
             raise ValueError(f"{what} must be contiguous while capturing")
-        return t.contiguous().view(-1)
+        return t.detach().contiguous()
 
-    def _result(self, given, shape, dtype, what):
-        """The tensor to write: `given`, checked, or a new one."""
-        import torch
+    def _result(self, given, like, shape, dtype, what):
+        """The tensor to write: `given`, checked, or a new one on the device of `like`."""
         if given is None:
             if self._in_capture:
                 raise ValueError(f"{what} has to be given while capturing")
-            return torch.empty(shape, dtype=dtype, device=f"cuda:{self.device}")
-        if not isinstance(given, torch.Tensor) or not given.is_cuda or given.dtype != dtype or \
-                given.device.index != self.device or tuple(given.shape) != tuple(shape) or \
+            return like.new_empty(shape, dtype=dtype)
+        if not isinstance(given, torch.Tensor) or given.dtype != dtype or not given.is_cuda or \
+                given.get_device() != self.device or given.shape != torch.Size(shape) or \
                 not given.is_contiguous():
             raise ValueError(f"{what} must be a contiguous {str(dtype)[6:]} tensor of shape "
                              f"{tuple(shape)} on cuda:{self.device}")
-        return given.detach()
+        return given
 
-    def _queue(self, tensors, call):
-        """Queue `call` behind torch's work on `tensors`, which it reads and writes."""
+    def _queue(self, tensors, call, *args):
+        """Queue the library's `call` behind torch's work on `tensors`: what it reads, and the
+        results that were given (a new one is torch's on its current stream already)."""
         if self._in_capture:
-            L.check(call())
+            L.check(call(self._h, *args))
             return
         kept = self._before_device_sources(tensors)
-        L.check(call())
+        L.check(call(self._h, *args))
         self._after_device_sources(kept)
 
     def _gradient(self, grad, logits, want):
         """(what the caller gets back, its matrix) of a loss's gradient: `grad` True for a new
         tensor like the logits, a tensor to write it to (the logits themselves too), False for
         none."""
-        import torch
         if grad is False or grad is None:
             return None, None
         if grad is True:
@@ -152,7 +155,7 @@ class Operators:
             else:
                 if self._in_capture:
                     raise ValueError("the gradient has to be given while capturing")
-                grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+                grad = logits.new_empty(logits.shape)
         if not isinstance(grad, torch.Tensor) or grad.dtype != logits.dtype or \
                 grad.shape != logits.shape:
             raise ValueError("the gradient must be a tensor of the logits' shape and type")
@@ -162,14 +165,12 @@ class Operators:
         """Each row's log-probability of its token under softmax(logits): float32, of targets'
         shape.  logits: (..., V) float32 or bfloat16; targets: int64, a negative one masks its
         row (0).  A token past the vocabulary gives NaN.  (ttp_token_logprobs)"""
-        import torch
         z = self._rows_of(logits, "the logits")
         y = self._vector_of(targets, z.shape[0], torch.int64, "the targets")
-        out = self._result(out, targets.shape, torch.float32, "out")
-        m = _matrix(z)
-        self._queue((z, y, out), lambda: L.lib.ttp_token_logprobs(
-            self._h, C.byref(m), y.data_ptr(), out.data_ptr()))
-        return out
+        result = self._result(out, z, targets.shape, torch.float32, "out")
+        self._queue((z, y) if out is None else (z, y, out), L.lib.ttp_token_logprobs,
+                    _matrix(z), y.data_ptr(), result.data_ptr())
+        return result
 
     def preference_loss(self, logits, targets, starts, ref_logps=None, *, beta=0.1,
                         label_smoothing=0.0, grad=True, out=None):
@@ -186,7 +187,6 @@ class Operators:
         `logits` itself.  While loss scaling is on the gradient is the scaled loss's, by the
         store's own scale; the loss is not scaled.  logits.backward(r.grad) continues in torch.
         out: an earlier call's result, whose tensors are written again.  (ttp_preference_loss)"""
-        import torch
         z = self._rows_of(logits, "the logits")
         rows = z.shape[0]
         y = self._vector_of(targets, rows, torch.int64, "the targets")
@@ -196,9 +196,9 @@ class Operators:
         at = self._vector_of(starts, 2 * pairs + 1, torch.int64, "starts")
         ref = None if ref_logps is None else self._vector_of(
             ref_logps, rows, torch.float32, "ref_logps")
-        loss = self._result(out and out.loss, (), torch.float32, "the loss")
-        margins = self._result(out and out.margins, (pairs,), torch.float32, "the margins")
-        logps = self._result(out and out.logps, targets.shape, torch.float32, "the logps")
+        loss = self._result(out and out.loss, z, (), torch.float32, "the loss")
+        margins = self._result(out and out.margins, z, (pairs,), torch.float32, "the margins")
+        logps = self._result(out and out.logps, z, targets.shape, torch.float32, "the logps")
         given, g = self._gradient(grad, logits, out and out.grad)
         m, gm = _matrix(z), None if g is None else _matrix(g)
         args = L.PreferenceArgs(
@@ -206,8 +206,12 @@ class Operators:
             pairs=pairs, beta=beta, label_smoothing=label_smoothing,
             grad=None if gm is None else C.pointer(gm), logps=logps.data_ptr(),
             margins=margins.data_ptr(), loss=loss.data_ptr())
-        used = [t for t in (z, y, at, ref, g, logps, margins, loss) if t is not None]
-        self._queue(used, lambda: L.lib.ttp_preference_loss(self._h, C.byref(args)))
+        used = [t for t in (z, y, at, ref) if t is not None]
+        if given is not None and grad is not True:
+            used.append(g)
+        if out is not None:
+            used += [t for t in out if t is not None]
+        self._queue(used, L.lib.ttp_preference_loss, args)
         return PreferenceLoss(loss, margins, logps, given)
 
     def policy_loss(self, logits, targets, old_logps, advantages, ref_logps=None, *, clip=0.2,
@@ -222,7 +226,6 @@ class Operators:
 
         clip: one number or (low, high).  denominator: D; None: the number of unmasked rows (at
         least 1).  grad and out as in preference_loss.  (ttp_policy_loss)"""
-        import torch
         low, high = clip if isinstance(clip, (tuple, list)) else (clip, clip)
         if denominator is not None and not denominator > 0:
             raise ValueError("denominator must be positive")
@@ -233,9 +236,9 @@ class Operators:
         adv = self._vector_of(advantages, rows, torch.float32, "advantages")
         ref = None if ref_logps is None else self._vector_of(
             ref_logps, rows, torch.float32, "ref_logps")
-        loss = self._result(out and out.loss, (), torch.float32, "the loss")
-        kl = self._result(out and out.kl, (), torch.float32, "kl")
-        logps = self._result(out and out.logps, targets.shape, torch.float32, "the logps")
+        loss = self._result(out and out.loss, z, (), torch.float32, "the loss")
+        kl = self._result(out and out.kl, z, (), torch.float32, "kl")
+        logps = self._result(out and out.logps, z, targets.shape, torch.float32, "the logps")
         given, g = self._gradient(grad, logits, out and out.grad)
         m, gm = _matrix(z), None if g is None else _matrix(g)
         args = L.PolicyArgs(
@@ -244,23 +247,27 @@ class Operators:
             kl_coef=kl_coef, denominator=denominator or 0.0,
             grad=None if gm is None else C.pointer(gm), logps=logps.data_ptr(),
             loss=loss.data_ptr(), kl=kl.data_ptr())
-        used = [t for t in (z, y, old, adv, ref, g, logps, loss, kl) if t is not None]
-        self._queue(used, lambda: L.lib.ttp_policy_loss(self._h, C.byref(args)))
+        used = [t for t in (z, y, old, adv, ref) if t is not None]
+        if given is not None and grad is not True:
+            used.append(g)
+        if out is not None:
+            used += [t for t in out if t is not None]
+        self._queue(used, L.lib.ttp_policy_loss, args)
         return PolicyLoss(loss, kl, logps, given)
 
     # ---- activations kept in 8 bits ------------------------------------------------------------
     def _kept_of(self, x, fmt, out, shape):
         """The checkpoint to write for the matrix `x`: `out`, checked, or a new one."""
-        import torch
         _choice(_FORMATS, fmt, "fmt")
         rows, cols = x.shape
         blocks = -(-cols // L.CHECKPOINT_BLOCK)
         if out is not None and (not isinstance(out, Checkpoint8) or out.format != fmt or
                                 out.shape != tuple(shape)):
             raise ValueError(f"out must be a checkpoint of shape {tuple(shape)} in {fmt}")
-        values = self._result(out and out.values, (rows, blocks * L.CHECKPOINT_BLOCK),
+        values = self._result(out and out.values, x, (rows, blocks * L.CHECKPOINT_BLOCK),
                               torch.uint8, "the checkpoint")
-        scales = self._result(out and out.scales, (rows, blocks), torch.uint8, "the checkpoint")
+        scales = self._result(out and out.scales, x, (rows, blocks), torch.uint8,
+                              "the checkpoint")
         return out or Checkpoint8(values, scales, shape, x.dtype, fmt)
 
     @staticmethod
@@ -275,25 +282,23 @@ class Operators:
         NaN.  out: a Checkpoint8 to write again.  (ttp_checkpoint8_pack)"""
         m = self._rows_of(x, "the activation")
         kept = self._kept_of(m, fmt, out, x.shape)
-        a, k = _matrix(m), kept._c()
-        self._queue((m, kept.values, kept.scales), lambda: L.lib.ttp_checkpoint8_pack(
-            self._h, C.byref(a), C.byref(k)))
+        self._queue((m,) if out is None else (m, out.values, out.scales),
+                    L.lib.ttp_checkpoint8_pack, _matrix(m), kept._c())
         return kept
 
     def restore8(self, kept, *, dtype=None, out=None):
         """The values a Checkpoint8 stands for, in its activation's shape and type (or `dtype`:
         float32 or bfloat16; exact in both).  (ttp_checkpoint8_restore)"""
-        import torch
         self._check_kept(kept)
         dtype = dtype or (kept.dtype if out is None else out.dtype)
         if dtype not in (torch.float32, torch.bfloat16):
             raise ValueError("dtype must be torch.float32 or torch.bfloat16")
-        out = self._result(out, kept.shape, dtype, "out")
-        m = self._rows_of(out, "out")
-        a, k = _matrix(m), kept._c()
-        self._queue((kept.values, kept.scales, m), lambda: L.lib.ttp_checkpoint8_restore(
-            self._h, C.byref(k), C.byref(a)))
-        return out
+        result = self._result(out, kept.values, kept.shape, dtype, "out")
+        m = self._rows_of(result, "out")
+        used = (kept.values, kept.scales)
+        self._queue(used if out is None else used + (out,), L.lib.ttp_checkpoint8_restore,
+                    kept._c(), _matrix(m))
+        return result
 
     def gelu_checkpoint8(self, x, *, fmt="int8", approximate="none", out=None, kept=None):
         """(gelu(x), x as a Checkpoint8) in one pass.  approximate: "none" (x Phi(x)) or "tanh"
@@ -301,13 +306,17 @@ class Operators:
         Checkpoint8 to write again.  (ttp_gelu_checkpoint8)"""
         approx = _choice(_APPROXIMATE, approximate, "approximate")
         m = self._rows_of(x, "the input")
+        used = [m]
+        if kept is not None:
+            self._check_kept(kept)
+            used += [kept.values, kept.scales]
         if out is None:
-            out = self._result(None, x.shape, x.dtype, "out")
+            out = self._result(None, x, x.shape, x.dtype, "out")
+        else:
+            used.append(out)
         y = self._like(out, x, "out")
         kept = self._kept_of(m, fmt, kept, x.shape)
-        a, b, k = _matrix(m), _matrix(y), kept._c()
-        self._queue((m, y, kept.values, kept.scales), lambda: L.lib.ttp_gelu_checkpoint8(
-            self._h, C.byref(a), approx, C.byref(b), C.byref(k)))
+        self._queue(used, L.lib.ttp_gelu_checkpoint8, _matrix(m), approx, _matrix(y), kept._c())
         return out, kept
 
     def gelu_backward8(self, kept, dy, *, approximate="none", out=None):
@@ -318,12 +327,13 @@ class Operators:
         g = self._rows_of(dy, "dy")
         if tuple(dy.shape) != kept.shape:
             raise ValueError(f"dy has shape {tuple(dy.shape)}, the checkpoint {kept.shape}")
+        used = [kept.values, kept.scales, g]
         if out is None:
-            out = self._result(None, dy.shape, dy.dtype, "out")
+            out = self._result(None, dy, dy.shape, dy.dtype, "out")
+        else:
+            used.append(out)
         d = self._like(out, dy, "out")
-        a, b, k = _matrix(g), _matrix(d), kept._c()
-        self._queue((kept.values, kept.scales, g, d), lambda: L.lib.ttp_gelu_backward8(
-            self._h, C.byref(k), approx, C.byref(a), C.byref(b)))
+        self._queue(used, L.lib.ttp_gelu_backward8, kept._c(), approx, _matrix(g), _matrix(d))
         return out
 
     def accumulate_linear_grad8(self, index, kept, dy, *, bias=None, transposed=False):
@@ -337,14 +347,12 @@ class Operators:
         g = self._rows_of(dy, "dy")
         if tuple(dy.shape[:-1]) != kept.shape[:-1]:
             raise ValueError(f"dy has shape {tuple(dy.shape)}, the checkpoint {kept.shape}")
-        a, k = _matrix(g), kept._c()
-        self._queue((kept.values, kept.scales, g), lambda: L.lib.ttp_accumulate_linear_grad8(
-            self._h, index, L.NO_TENSOR if bias is None else bias, C.byref(k), C.byref(a),
-            1 if transposed else 0))
+        self._queue((kept.values, kept.scales, g), L.lib.ttp_accumulate_linear_grad8, index,
+                    L.NO_TENSOR if bias is None else bias, kept._c(), _matrix(g),
+                    1 if transposed else 0)
 
     def _like(self, out, x, what):
         """The matrix of a result that has x's shape and type."""
-        import torch
         if not isinstance(out, torch.Tensor) or out.dtype != x.dtype or out.shape != x.shape:
             raise ValueError(f"{what} must be a tensor of the input's shape and type")
         return self._rows_of(out, what)
