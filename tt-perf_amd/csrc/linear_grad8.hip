@@ -30,15 +30,17 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
-// kA x kB of the gradient per block, kN rows per step, kWA x kWB waves
-template <int A, int B, int N, int WA, int WB>
+// kA x kB of the gradient per block, kN rows per step; kWA x kWB waves over the tile, and kWN over
+// the rows of a step: each of the kWN sums its share, and they are added up at the end.
+template <int A, int B, int N, int WA, int WB, int WN, int D>
 struct Tile {
-    static constexpr int kA = A, kB = B, kN = N, kWA = WA, kWB = WB;
-    static constexpr int kThreads = 64 * WA * WB;
+    static constexpr int kA = A, kB = B, kN = N, kWA = WA, kWB = WB, kWN = WN, kDepth = D;
+    static constexpr int kThreads = 64 * WA * WB * WN;
     static constexpr int kFA = A / WA / 32, kFB = B / WB / 32;  // 32 x 32 fragments of a wave
     // LDS rows are 64 bytes longer than the tile: the four rows that a transposing load takes at
     // once lie in different banks
-    static constexpr int kPitchA = A + 32, kPitchB = B + 32;  // bf16 elements
+    static constexpr int kPad = 32;
+    static constexpr int kPitchA = A + kPad, kPitchB = B + kPad;  // bf16 elements
 };
 
 struct LinearArgs {
@@ -98,22 +100,24 @@ __device__ __forceinline__ void split3(float a, float b, uint32_t (&p)[3]) {
     }
 }
 
-// Columns c .. c + 7 of a row, past the end 0
+// 8 columns of a row of dy
 template <class G>
 struct Chunk8;
 template <>
 struct Chunk8<uint16_t> {
     u32x4 w;
-    __device__ __forceinline__ void load(const uint16_t* row, uint32_t c, uint32_t cols, bool live) {
-        w = u32x4{0, 0, 0, 0};
-        if (!live || c >= cols) return;
-        if (c + 8 <= cols) {
-            w = load16(row + c);
-        } else {
+    __device__ __forceinline__ void load(const uint16_t* p) { w = load16(p); }
+    __device__ __forceinline__ void clear() { w = u32x4{0, 0, 0, 0}; }
+    __device__ __forceinline__ void keep(int n) {  // the first n, then 0
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (c + k < cols) w[k / 2] |= (uint32_t)row[c + k] << (16 * (k % 2));
-        }
+        for (int k = 0; k < 4; ++k)
+            w[k] = 2 * k + 1 < n ? w[k] : 2 * k < n ? w[k] & 0xFFFFu : 0u;
+    }
+    __device__ __forceinline__ void load_some(const uint16_t* p, int n) {  // the first n, then 0
+        w = u32x4{0, 0, 0, 0};
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (k < n) w[k / 2] |= (uint32_t)p[k] << (16 * (k % 2));
     }
     __device__ __forceinline__ float value(int k) const {
         return k % 2 ? bf16_hi(w[k / 2]) : bf16_lo(w[k / 2]);
@@ -122,30 +126,26 @@ struct Chunk8<uint16_t> {
 };
 template <>
 struct Chunk8<float> {
-    float v[8];
-    __device__ __forceinline__ void load(const float* row, uint32_t c, uint32_t cols, bool live) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] = 0.0f;
-        if (!live || c >= cols) return;
-        if (c + 8 <= cols) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const u32x4 w = load16(row + c + 4 * h);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) v[4 * h + k] = __uint_as_float(w[k]);
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-                if (c + k < cols) v[k] = row[c + k];
-        }
+    u32x4 w[2];
+    __device__ __forceinline__ void load(const float* p) {
+        w[0] = load16(p);
+        w[1] = load16(p + 4);
     }
-    __device__ __forceinline__ float value(int k) const { return v[k]; }
+    __device__ __forceinline__ void clear() { w[0] = w[1] = u32x4{0, 0, 0, 0}; }
+    __device__ __forceinline__ void keep(int n) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k / 4][k % 4] = k < n ? w[k / 4][k % 4] : 0u;
+    }
+    __device__ __forceinline__ void load_some(const float* p, int n) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k / 4][k % 4] = k < n ? __float_as_uint(p[k]) : 0u;
+    }
+    __device__ __forceinline__ float value(int k) const { return __uint_as_float(w[k / 4][k % 4]); }
     __device__ __forceinline__ void planes(u32x4 (&p)[3]) const {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             uint32_t three[3];
-            split3(v[2 * k], v[2 * k + 1], three);
+            split3(value(2 * k), value(2 * k + 1), three);
 #pragma unroll
             for (int j = 0; j < 3; ++j) p[j][k] = three[j];
         }
@@ -218,16 +218,22 @@ __device__ __forceinline__ void put_bias(const LinearArgs& a, uint32_t o, float 
 }
 
 template <class G, int kFormat, class T>
-__global__ __launch_bounds__(T::kThreads, 2) void linear_grad_kernel(LinearArgs a) {
+__global__ __launch_bounds__(T::kThreads, T::kThreads == 512 ? 1 : 2) void linear_grad_kernel(
+    LinearArgs a) {
     constexpr int kPlanes = sizeof(G) == 2 ? 1 : 3;
     constexpr int kSizeA = T::kN * T::kPitchA, kSizeB = T::kN * T::kPitchB;
     constexpr int kBuffer = kSizeA + kPlanes * kSizeB;
     constexpr int kChunksA = T::kN * T::kA / 16 / T::kThreads;  // per lane and step
     constexpr int kChunksB = T::kN * T::kB / 8 / T::kThreads;
-    static_assert(kChunksA >= 1 && kChunksB >= 1 && T::kThreads % (T::kB / 8) == 0);
+    static_assert(kChunksA >= 1 && kChunksB >= 1 && T::kThreads % (T::kB / 8) == 0 &&
+                  T::kThreads % (T::kA / 16) == 0 && T::kN % (16 * T::kWN) == 0);
+    constexpr int kRowsA = T::kThreads / (T::kA / 16), kRowsB = T::kThreads / (T::kB / 8);
+    constexpr int kPairs = T::kWA * T::kWB;  // waves over the tile
     constexpr int kOutPitch = 36;  // floats; a wave's 32 x 32 of the gradient on its way out
-    constexpr int kOut = T::kWA * T::kWB * 32 * kOutPitch * 2;
-    __shared__ __align__(16) short lds[2 * kBuffer > kOut ? 2 * kBuffer : kOut];
+    constexpr int kOut = kPairs * 32 * kOutPitch * 2;
+    constexpr int kAdd = T::kWN > 1 ? kPairs * T::kFB * 64 * 16 * 2 : 0;  // see below
+    constexpr int kMost = 2 * kBuffer > kOut ? 2 * kBuffer : kOut;
+    __shared__ __align__(16) short lds[kMost > kAdd ? kMost : kAdd];
 
     const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
     const uint32_t part = id / (a.tiles_a * a.tiles_b), tile = id % (a.tiles_a * a.tiles_b);
@@ -236,52 +242,83 @@ __global__ __launch_bounds__(T::kThreads, 2) void linear_grad_kernel(LinearArgs 
     const uint32_t rows = (uint32_t)(row0 >= a.rows ? 0 : min(a.per, a.rows - row0));
     const bool bias = a.db && a0 == 0;
 
-    const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
-    const int wa = wave / T::kWB * (T::kA / T::kWA), wb = wave % T::kWB * (T::kB / T::kWB);
+    const int t = threadIdx.x, lane = t & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int pair = wave % kPairs, share = wave / kPairs;
+    const int wa = pair / T::kWB * (T::kA / T::kWA), wb = pair % T::kWB * (T::kB / T::kWB);
 
-    const uint32_t colb = t % (T::kB / 8) * 8;  // this lane's columns of dy, of the tile
-    u32x4 ra[kChunksA];
-    uint32_t rs[kChunksA];
-    Chunk8<G> rb[kChunksB];
-    const auto load = [&](uint32_t step) {
-        const uint32_t n0 = step * T::kN;
+    // this lane's chunks: columns ca of xhat (of the tile), rows ta + k kRowsA; and of dy
+    const uint32_t ca = t % (T::kA / 16) * 16, ta = t / (T::kA / 16);
+    const uint32_t cb = t % (T::kB / 8) * 8, tb = t / (T::kB / 8);
+    const uint8_t* pa = a.values + (row0 + ta) * a.width + a0 + ca;
+    const uint8_t* ps = a.scales + (row0 + ta) * (a.width / 32) + (a0 + ca) / 32;
+    const G* pb = (const G*)a.dy + (row0 + tb) * a.dy_stride + b0 + cb;
+    const uint64_t next_a = (uint64_t)T::kN * a.width, next_b = (uint64_t)T::kN * a.dy_stride;
+    const bool inside = a0 + T::kA <= a.width && b0 + T::kB <= a.outs;
+    const int some_b = b0 + cb >= a.outs ? 0 : (int)min(a.outs - b0 - cb, 8u);
+    struct Loads {
+        u32x4 a[kChunksA];
+        uint32_t s[kChunksA];
+        Chunk8<G> b[kChunksB];
+    };
+    const auto load = [&](Loads& r, uint32_t step) {
+        const uint32_t left = rows - step * T::kN;
+        if (inside && left >= T::kN) {
 #pragma unroll
-        for (int k = 0; k < kChunksA; ++k) {
-            const uint32_t e = t + k * T::kThreads;
-            const uint32_t n = n0 + e / (T::kA / 16), c = a0 + e % (T::kA / 16) * 16;
-            ra[k] = u32x4{0, 0, 0, 0};
-            rs[k] = 1;
-            if (n < rows && c < a.width) {
-                const uint64_t at = (row0 + n) * a.width + c;
-                ra[k] = *reinterpret_cast<const u32x4*>(a.values + at);
-                rs[k] = a.scales[at / 32];
+            for (int k = 0; k < kChunksB; ++k) r.b[k].load(pb + (uint64_t)(k * kRowsB) * a.dy_stride);
+#pragma unroll
+            for (int k = 0; k < kChunksA; ++k) {
+                r.a[k] = *reinterpret_cast<const u32x4*>(pa + (uint64_t)(k * kRowsA) * a.width);
+                r.s[k] = ps[(uint64_t)(k * kRowsA) * (a.width / 32)];
+            }
+        } else {  // columns or rows past the end count 0
+#pragma unroll
+            for (int k = 0; k < kChunksB; ++k) {
+                const G* p = pb + (uint64_t)(k * kRowsB) * a.dy_stride;
+                const int n = tb + k * kRowsB < left ? some_b : 0;
+                // a row's last chunk reaches into the next row, where there is one (of 8 or more)
+                const bool spill = a.outs >= 8 && row0 + step * T::kN + tb + k * kRowsB + 1 < a.rows;
+                if (n == 8 || (n && spill)) {
+                    r.b[k].load(p);
+                    if (n < 8) r.b[k].keep(n);
+                } else if (n) {
+                    r.b[k].load_some(p, n);
+                } else {
+                    r.b[k].clear();
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < kChunksA; ++k) {
+                r.a[k] = u32x4{0, 0, 0, 0};
+                r.s[k] = 1;
+                if (ta + k * kRowsA < left && a0 + ca < a.width) {
+                    r.a[k] =
+                        *reinterpret_cast<const u32x4*>(pa + (uint64_t)(k * kRowsA) * a.width);
+                    r.s[k] = ps[(uint64_t)(k * kRowsA) * (a.width / 32)];
+                }
             }
         }
-#pragma unroll
-        for (int k = 0; k < kChunksB; ++k) {
-            const uint32_t n = n0 + (t + k * T::kThreads) / (T::kB / 8);
-            rb[k].load((const G*)a.dy + (row0 + n) * a.dy_stride, b0 + colb, a.outs, n < rows);
-        }
+        pa += next_a;
+        ps += next_a / 32;
+        pb += next_b;
     };
-    const auto store = [&](short* buffer) {
+    const auto store = [&](const Loads& r, short* buffer) {
 #pragma unroll
         for (int k = 0; k < kChunksA; ++k) {
-            const uint32_t e = t + k * T::kThreads;
             u32x4 w[2];
-            widen16<kFormat>(ra[k], rs[k], w);
-            short* p = buffer + e / (T::kA / 16) * T::kPitchA + e % (T::kA / 16) * 16;
+            widen16<kFormat>(r.a[k], r.s[k], w);
+            short* p = buffer + (ta + k * kRowsA) * T::kPitchA + ca;
             *reinterpret_cast<u32x4*>(p) = w[0];
             *reinterpret_cast<u32x4*>(p + 8) = w[1];
         }
 #pragma unroll
         for (int k = 0; k < kChunksB; ++k) {
-            const uint32_t e = t + k * T::kThreads;
             u32x4 w[kPlanes];
-            rb[k].planes(w);
+            r.b[k].planes(w);
 #pragma unroll
             for (int j = 0; j < kPlanes; ++j)
                 *reinterpret_cast<u32x4*>(buffer + kSizeA + j * kSizeB +
-                                          e / (T::kB / 8) * T::kPitchB + colb) = w[j];
+                                          (tb + k * kRowsB) * T::kPitchB + cb) = w[j];
         }
     };
 
@@ -292,106 +329,184 @@ __global__ __launch_bounds__(T::kThreads, 2) void linear_grad_kernel(LinearArgs 
         for (int j = 0; j < T::kFB; ++j) acc[i][j] = f32x16{};
     // the bias: this lane's rows of its columns, in two levels (sums of many steps by themselves)
     float near[8] = {}, far[8] = {};
+    const auto sum_bias = [&](const Loads& r, uint32_t s) {
+#pragma unroll
+        for (int k = 0; k < kChunksB; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) near[j] += r.b[k].value(j);
+        if ((s & 15) == 15)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                far[j] += near[j];
+                near[j] = 0.0f;
+            }
+    };
 
-    const uint32_t steps = (rows + T::kN - 1) / T::kN;
-    if (steps) {
-        load(0);
-        store(lds);
-    }
-    for (uint32_t s = 0; s < steps; ++s) {
-        __syncthreads();
-        if (bias) {
+    // A step is two rounds of 16 rows, whose operands are in registers before the step begins: step
+    // s + 1 goes to the other LDS buffer behind round 0's instructions, its rounds' operands come
+    // back behind round 1's, and step s + 2's loads from memory are in flight meanwhile.
+    static_assert(T::kN / T::kWN == 32);
+    struct Round {
+        bf16x8 a[T::kFA], b[kPlanes][T::kFB];
+    } round[2];
+    const auto fetch = [&](const short* buffer, int r) {
+        const int n = share * 32 + r * 16;
 #pragma unroll
-            for (int k = 0; k < kChunksB; ++k)
+        for (int i = 0; i < T::kFA; ++i)
+            round[r].a[i] = fragment(buffer, T::kPitchA, n, wa + 32 * i);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) near[j] += rb[k].value(j);
-            if ((s & 15) == 15)
+        for (int p = 0; p < kPlanes; ++p)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    far[j] += near[j];
-                    near[j] = 0.0f;
-                }
-        }
-        if (s + 1 < steps) load(s + 1);
-        const short* buffer = lds + (s & 1) * kBuffer;
+            for (int j = 0; j < T::kFB; ++j)
+                round[r].b[p][j] =
+                    fragment(buffer + kSizeA + p * kSizeB, T::kPitchB, n, wb + 32 * j);
+    };
+    const auto multiply = [&](int r) {
 #pragma unroll
-        for (int n = 0; n < T::kN; n += 16) {
-            bf16x8 fa[T::kFA];
+        for (int p = 0; p < kPlanes; ++p)
 #pragma unroll
             for (int i = 0; i < T::kFA; ++i)
-                fa[i] = fragment(buffer, T::kPitchA, n, wa + 32 * i);
-#pragma unroll
-            for (int p = 0; p < kPlanes; ++p) {
-                bf16x8 fb[T::kFB];
 #pragma unroll
                 for (int j = 0; j < T::kFB; ++j)
-                    fb[j] = fragment(buffer + kSizeA + p * kSizeB, T::kPitchB, n, wb + 32 * j);
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+                        round[r].a[i], round[r].b[p][j], acc[i][j], 0, 0, 0);
+    };
+    const uint32_t steps = (rows + T::kN - 1) / T::kN;
+    // kDepth sets of loads in flight: step s uses set s % kDepth, and step s + kDepth's follow it
+    Loads loads[T::kDepth];
+    const auto advance = [&](Loads& r, uint32_t s) {
+        short* next = lds + (s & 1) * kBuffer;  // step s: loaded, now into LDS
+        multiply(0);
+        store(r, next);
+        // the next step's conversions between the matrix instructions, not behind them
 #pragma unroll
-                for (int i = 0; i < T::kFA; ++i)
-#pragma unroll
-                    for (int j = 0; j < T::kFB; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[i], fb[j],
-                                                                            acc[i][j], 0, 0, 0);
-            }
+        for (int k = 0; k < T::kFA * T::kFB; ++k) {
+            __builtin_amdgcn_sched_group_barrier(0x008, kPlanes, 0);  // matrix
+            __builtin_amdgcn_sched_group_barrier(0x002, 6 * kPlanes, 0);  // vector
+            __builtin_amdgcn_sched_group_barrier(0x200, kPlanes, 0);  // LDS writes
         }
-        if (s + 1 < steps) store(lds + ((s + 1) & 1) * kBuffer);
+        if (bias) sum_bias(r, s);
+        if (s + T::kDepth < steps) load(r, s + T::kDepth);
+        __syncthreads();
+        fetch(next, 0);
+        multiply(1);
+        fetch(next, 1);
+    };
+    if (steps) {
+#pragma unroll
+        for (int d = 0; d < T::kDepth; ++d)
+            if ((uint32_t)d < steps) load(loads[d], d);
+        store(loads[0], lds);
+        if (bias) sum_bias(loads[0], 0);
+        if (T::kDepth < steps) load(loads[0], T::kDepth);
+        __syncthreads();
+        fetch(lds, 0);
+        fetch(lds, 1);
+        for (uint32_t s = 1; s < steps; s += T::kDepth)
+#pragma unroll
+            for (int d = 1; d <= T::kDepth; ++d)
+                if (s + d - 1 < steps) advance(loads[d % T::kDepth], s + d - 1);
+        multiply(0);
+        multiply(1);
     }
     __syncthreads();
+
+    if constexpr (T::kWN > 1) {
+        // the shares' sums, one row of fragments at a time: the others' go through LDS, in order
+        f32x4* parts = reinterpret_cast<f32x4*>(lds) + pair * T::kFB * 64 * 4;
+#pragma unroll
+        for (int i = 0; i < T::kFA; ++i)
+#pragma unroll
+            for (int h = 1; h < T::kWN; ++h) {
+                if (share == h) {
+#pragma unroll
+                    for (int j = 0; j < T::kFB; ++j)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            parts[(j * 4 + k) * 64 + lane] =
+                                f32x4{acc[i][j][4 * k], acc[i][j][4 * k + 1],
+                                      acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
+                }
+                __syncthreads();
+                if (share == 0) {
+#pragma unroll
+                    for (int j = 0; j < T::kFB; ++j)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const f32x4 v = parts[(j * 4 + k) * 64 + lane];
+#pragma unroll
+                            for (int m = 0; m < 4; ++m) acc[i][j][4 * k + m] += v[m];
+                        }
+                }
+                __syncthreads();
+            }
+    }
 
     // out, 32 x 32 at a time through this wave's LDS: the gradient's rows are columns of xhat,
     // or of dy where the weight is transposed
-    float* out = reinterpret_cast<float*>(lds) + wave * 32 * kOutPitch;
-    const uint32_t rows_out = a.transposed ? a.outs : a.cols;
-    const uint32_t cols_out = a.transposed ? a.cols : a.outs;
+    if (share == 0) {
+        float* out = reinterpret_cast<float*>(lds) + pair * 32 * kOutPitch;
+        const uint32_t rows_out = a.transposed ? a.outs : a.cols;
+        const uint32_t cols_out = a.transposed ? a.cols : a.outs;
 #pragma unroll
-    for (int i = 0; i < T::kFA; ++i)
+        for (int i = 0; i < T::kFA; ++i)
 #pragma unroll
-        for (int j = 0; j < T::kFB; ++j) {
-            // lane: column lane % 32 of dy, rows 8 (k / 4) + 4 (lane / 32) + k % 4 of xhat
+            for (int j = 0; j < T::kFB; ++j) {
+                // lane: column lane % 32 of dy, rows 8 (k / 4) + 4 (lane / 32) + k % 4 of xhat
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const int x = 8 * (k / 4) + 4 * (lane >> 5) + k % 4, y = lane & 31;
-                out[(a.transposed ? y : x) * kOutPitch + (a.transposed ? x : y)] = acc[i][j][k];
-            }
-            __builtin_amdgcn_wave_barrier();
-            const uint32_t xa = a0 + wa + 32 * i, yb = b0 + wb + 32 * j;
-            const uint32_t r = (a.transposed ? yb : xa) + lane / 2;
-            const uint32_t c = (a.transposed ? xa : yb) + lane % 2 * 16;
-            float v[16];
+                for (int k = 0; k < 16; ++k) {
+                    const int x = 8 * (k / 4) + 4 * (lane >> 5) + k % 4, y = lane & 31;
+                    out[(a.transposed ? y : x) * kOutPitch + (a.transposed ? x : y)] =
+                        acc[i][j][k];
+                }
+                __builtin_amdgcn_wave_barrier();
+                const uint32_t xa = a0 + wa + 32 * i, yb = b0 + wb + 32 * j;
+                const uint32_t r = (a.transposed ? yb : xa) + lane / 2;
+                const uint32_t c = (a.transposed ? xa : yb) + lane % 2 * 16;
+                float v[16];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const f32x4 q = *reinterpret_cast<const f32x4*>(out + lane / 2 * kOutPitch +
-                                                                lane % 2 * 16 + 4 * k);
+                for (int k = 0; k < 4; ++k) {
+                    const f32x4 q = *reinterpret_cast<const f32x4*>(out + lane / 2 * kOutPitch +
+                                                                    lane % 2 * 16 + 4 * k);
 #pragma unroll
-                for (int m = 0; m < 4; ++m) v[4 * k + m] = q[m];
-            }
-            __builtin_amdgcn_wave_barrier();
-            if (r < rows_out && c < cols_out) {
-                const uint64_t at = (uint64_t)r * cols_out + c;
-                const uint32_t n = min(16u, cols_out - c);
-                if (a.parts == 1) {
-                    put(a, at, n, v);
-                } else {
-                    float* p = a.dw_parts + (uint64_t)part * rows_out * cols_out + at;
+                    for (int m = 0; m < 4; ++m) v[4 * k + m] = q[m];
+                }
+                __builtin_amdgcn_wave_barrier();
+                if (r < rows_out && c < cols_out) {
+                    const uint64_t at = (uint64_t)r * cols_out + c;
+                    const uint32_t n = min(16u, cols_out - c);
+                    if (a.parts == 1) {
+                        put(a, at, n, v);
+                    } else {
+                        float* p = a.dw_parts + (uint64_t)part * rows_out * cols_out + at;
+                        if (n == 16) {
 #pragma unroll
-                    for (int k = 0; k < 16; ++k)
-                        if (k < (int)n) p[k] = v[k];
+                            for (int k = 0; k < 4; ++k) {
+                                const float w[4] = {v[4 * k], v[4 * k + 1], v[4 * k + 2],
+                                                    v[4 * k + 3]};
+                                store16(p + 4 * k, pack(w, p));
+                            }
+                        } else {
+#pragma unroll
+                            for (int k = 0; k < 16; ++k)
+                                if (k < (int)n) p[k] = v[k];
+                        }
+                    }
                 }
             }
-        }
+    }
     if (!bias) return;
     __syncthreads();
     // the lanes that share columns, in order
-    constexpr int kLanes = T::kThreads / (T::kB / 8);
-    float* sums = reinterpret_cast<float*>(lds);  // kLanes x kB
+    float* sums = reinterpret_cast<float*>(lds);  // kRowsB x kB
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sums[t / (T::kB / 8) * T::kB + colb + j] = far[j] + near[j];
+    for (int j = 0; j < 8; ++j) sums[tb * T::kB + cb + j] = far[j] + near[j];
     __syncthreads();
     for (int c = t; c < T::kB; c += T::kThreads) {
         if (b0 + c >= a.outs) break;
         float v = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kLanes; ++k) v += sums[k * T::kB + c];
+        for (int k = 0; k < kRowsB; ++k) v += sums[k * T::kB + c];
         if (a.parts == 1)
             put_bias(a, b0 + c, v);
         else
@@ -399,32 +514,67 @@ __global__ __launch_bounds__(T::kThreads, 2) void linear_grad_kernel(LinearArgs 
     }
 }
 
-// The parts' sums, in order, into the gradients: four elements of the weight per lane, then the
-// bias.
+// The parts' sums, in order, into the gradients: four neighbouring elements of the weight per lane,
+// then the bias.  Bound by reading the parts.
 constexpr int kJoinBlock = 256;
+template <class O>
 __global__ __launch_bounds__(kJoinBlock) void join_parts_kernel(LinearArgs a) {
-    const uint64_t n = (uint64_t)a.cols * a.outs, total = n + (a.db ? a.outs : 0);
+    const uint64_t n = (uint64_t)a.cols * a.outs, quads = n / 4;
+    const uint64_t rest = n - quads * 4, total = quads + rest + (a.db ? a.outs : 0);
+    O* dw = (O*)a.dw;
     for (uint64_t i = (uint64_t)blockIdx.x * kJoinBlock + threadIdx.x; i < total;
          i += (uint64_t)gridDim.x * kJoinBlock) {
-        const bool weight = i < n;
-        const float* p = weight ? a.dw_parts + i : a.db_parts + (i - n);
-        const uint64_t pitch = weight ? n : a.outs;
-        float v = 0.0f;
-        for (uint32_t k = 0; k < a.parts; ++k) v += p[k * pitch];
-        if (!weight) {
-            put_bias(a, (uint32_t)(i - n), v);
-        } else if (a.bf16) {
-            uint16_t* g = (uint16_t*)a.dw + i;
-            narrow(a.dw_first ? v : widen(*g) + v, g);
+        if (i < quads) {
+            const float* p = a.dw_parts + 4 * i;
+            float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+            for (uint32_t k = 0; k < a.parts; ++k) {
+                float w[4];
+                unpack(load16_once(p + k * n), w, p);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] += w[j];
+            }
+            O* g = dw + 4 * i;  // (tensors start on 64 elements)
+            if (!a.dw_first)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = widen(g[j]) + v[j];
+            if constexpr (sizeof(O) == 2) {
+                u32x2 w;
+                w.x = bf16_pack(v[0], v[1]);
+                w.y = bf16_pack(v[2], v[3]);
+                *reinterpret_cast<u32x2*>(g) = w;
+            } else {
+                *reinterpret_cast<f32x4*>(g) = f32x4{v[0], v[1], v[2], v[3]};
+            }
+        } else if (i < quads + rest) {
+            const uint64_t at = 4 * quads + (i - quads);
+            float v = 0.0f;
+            for (uint32_t k = 0; k < a.parts; ++k) v += a.dw_parts[k * n + at];
+            narrow(a.dw_first ? v : widen(dw[at]) + v, dw + at);
         } else {
-            float* g = (float*)a.dw + i;
-            *g = a.dw_first ? v : *g + v;
+            const uint32_t o = (uint32_t)(i - quads - rest);
+            float v = 0.0f;
+            for (uint32_t k = 0; k < a.parts; ++k) v += a.db_parts[(uint64_t)k * a.outs + o];
+            put_bias(a, o, v);
         }
     }
 }
 
 // ---- launches -----------------------------------------------------------------------------------
-using Wide = Tile<128, 128, 32, 2, 2>;
+using Wide = Tile<256, 256, 32, 2, 4, 1, 2>;    // one block per CU
+using Narrow = Tile<128, 128, 32, 2, 2, 1, 1>;  // two
+using Planes = Narrow;                          // an fp32 dy: three products each
+
+// What a tile costs, measured: ns per row of a block that has its CU to itself, and of two that
+// share one; and ns before its first and behind its last step.  The wide tile moves half the bytes
+// per operation, the narrow one wastes less of a small gradient and needs fewer parts.
+// (8192 x 1280 x 5120 bf16: 150 us with wide tiles, 200 with narrow ones; 4096 x 384 x 1536: 35 and
+// 27.)
+struct Cost {
+    double one, two, ends;
+};
+constexpr Cost kWideCost{30.0, 60.0, 8000.0}, kNarrowCost{15.0, 22.0, 4000.0},
+    kPlanesCost{30.0, 56.0, 4000.0};
 
 template <class G, int kFormat, class T>
 int launch_tiles(const ttpi::Op& op, const LinearArgs& a) {
@@ -438,16 +588,31 @@ int launch_tiles(const ttpi::Op& op, const LinearArgs& a) {
     return TTP_OK;
 }
 
-// Tiles below the launch's room (two blocks per CU) split the rows, at least 256 to a part.
+// Cuts the work into tiles and the rows into parts of 128 or more: the number of parts that should
+// take the least time, which is returned (ns).  Parts cost their fp32 tiles' way to memory and
+// back, about 5 TB/s, a launch, and the join's loads one after the other.
 template <class T>
-void set_tiles(LinearArgs& a, int cus) {
+double set_tiles(LinearArgs& a, uint64_t cus, const Cost& c) {
     a.tiles_a = (a.cols + T::kA - 1) / T::kA;
     a.tiles_b = (a.outs + T::kB - 1) / T::kB;
-    const uint64_t tiles = (uint64_t)a.tiles_a * a.tiles_b, room = 2 * (uint64_t)cus;
-    const uint64_t parts =
-        std::max<uint64_t>(std::min<uint64_t>(room / std::min(tiles, room), a.rows / 256), 1);
-    a.per = ((a.rows + parts - 1) / parts + T::kN - 1) / T::kN * T::kN;
-    a.parts = a.per ? (uint32_t)std::max<uint64_t>((a.rows + a.per - 1) / a.per, 1) : 1;
+    const uint64_t tiles = (uint64_t)a.tiles_a * a.tiles_b;
+    const uint64_t most = std::max<uint64_t>(std::min<uint64_t>(a.rows / 128, 64), 1);
+    double best = 0.0;
+    for (uint64_t n = 1; n <= most; ++n) {
+        const uint64_t per = ((a.rows + n - 1) / n + T::kN - 1) / T::kN * T::kN;
+        const uint64_t parts = per ? std::max<uint64_t>((a.rows + per - 1) / per, 1) : 1;
+        const uint64_t blocks = tiles * parts, left = blocks % (2 * cus);
+        double ns = (double)(blocks / (2 * cus)) * (c.two * (double)per + c.ends);
+        if (left) ns += (left > cus ? c.two : c.one) * (double)per + c.ends;
+        if (parts > 1)
+            ns += 3000.0 + 150.0 * (double)parts + 8.0 * (double)parts * a.cols * a.outs / 5e3;
+        if (n == 1 || ns < best) {
+            best = ns;
+            a.per = per;
+            a.parts = (uint32_t)parts;
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -507,7 +672,17 @@ extern "C" int ttp_accumulate_linear_grad8(ttp_ctx* ctx, uint32_t weight, uint32
         a.bf16 = w.bf16;
         a.dw_first = w.first;
         a.db_first = b.first;
-        set_tiles<Wide>(a, op.num_cus);
+        const bool bf16 = dy->dtype == TTP_DTYPE_BF16;
+        const uint64_t cus = (uint64_t)op.num_cus;
+        bool wide = false;
+        if (bf16) {
+            LinearArgs b = a;
+            const double narrow_ns = set_tiles<Narrow>(a, cus, kNarrowCost);
+            wide = set_tiles<Wide>(b, cus, kWideCost) < narrow_ns;
+            if (wide) a = b;
+        } else {
+            set_tiles<Planes>(a, cus, kPlanesCost);
+        }
         if (a.parts > 1) {
             void* ws;
             const uint64_t n = (uint64_t)a.parts * cols * outs;
@@ -516,19 +691,25 @@ extern "C" int ttp_accumulate_linear_grad8(ttp_ctx* ctx, uint32_t weight, uint32
             a.db_parts = a.dw_parts + n;
         }
         const bool int8 = kept->format == TTP_CHECKPOINT_INT8;
-        if (dy->dtype == TTP_DTYPE_BF16)
+        if (bf16 && wide)
             rc = int8 ? launch_tiles<uint16_t, TTP_CHECKPOINT_INT8, Wide>(op, a)
                       : launch_tiles<uint16_t, TTP_CHECKPOINT_E4M3, Wide>(op, a);
+        else if (bf16)
+            rc = int8 ? launch_tiles<uint16_t, TTP_CHECKPOINT_INT8, Narrow>(op, a)
+                      : launch_tiles<uint16_t, TTP_CHECKPOINT_E4M3, Narrow>(op, a);
         else
-            rc = int8 ? launch_tiles<float, TTP_CHECKPOINT_INT8, Wide>(op, a)
-                      : launch_tiles<float, TTP_CHECKPOINT_E4M3, Wide>(op, a);
+            rc = int8 ? launch_tiles<float, TTP_CHECKPOINT_INT8, Planes>(op, a)
+                      : launch_tiles<float, TTP_CHECKPOINT_E4M3, Planes>(op, a);
         if (rc) return rc;
         if (a.parts > 1) {
-            const uint64_t n = cols * outs + outs;
-            const uint32_t grid = (uint32_t)std::min<uint64_t>((n + kJoinBlock - 1) / kJoinBlock,
-                                                               (uint64_t)op.num_cus * 16);
+            const uint64_t n = cols * outs / 4 + 3 + outs;
+            const dim3 block(kJoinBlock),
+                grid((uint32_t)std::min<uint64_t>((n + kJoinBlock - 1) / kJoinBlock, cus * 16));
             (void)hipGetLastError();
-            hipLaunchKernelGGL(join_parts_kernel, dim3(grid), dim3(kJoinBlock), 0, op.stream, a);
+            if (a.bf16)
+                hipLaunchKernelGGL(join_parts_kernel<uint16_t>, grid, block, 0, op.stream, a);
+            else
+                hipLaunchKernelGGL(join_parts_kernel<float>, grid, block, 0, op.stream, a);
             TTPI_HIP(hipGetLastError());
         }
         ttpi::grad_written(ctx, weight);

