@@ -310,6 +310,33 @@ public:
     }
     void set_step_count(uint64_t t) { check(ttp_set_step(ctx_, t)); }
     void sync() { check(ttp_sync(ctx_)); }
+
+    // Fine-tuning operators over the caller's device memory (ttperf.h, "fine-tuning operators").
+    void token_logprobs(const ttp_matrix& logits, const int64_t* targets, float* logps) {
+        check(ttp_token_logprobs(ctx_, &logits, targets, logps));
+    }
+    void preference_loss(const ttp_preference_args& a) { check(ttp_preference_loss(ctx_, &a)); }
+    void policy_loss(const ttp_policy_args& a) { check(ttp_policy_loss(ctx_, &a)); }
+    void checkpoint8(const ttp_matrix& x, const ttp_checkpoint8& kept) {
+        check(ttp_checkpoint8_pack(ctx_, &x, &kept));
+    }
+    void restore8(const ttp_checkpoint8& kept, const ttp_matrix& x) {
+        check(ttp_checkpoint8_restore(ctx_, &kept, &x));
+    }
+    void gelu_checkpoint8(const ttp_matrix& x, int approximate, const ttp_matrix& y,
+                          const ttp_checkpoint8& kept) {
+        check(ttp_gelu_checkpoint8(ctx_, &x, approximate, &y, &kept));
+    }
+    void gelu_backward8(const ttp_checkpoint8& kept, int approximate, const ttp_matrix& dy,
+                        const ttp_matrix& dx) {
+        check(ttp_gelu_backward8(ctx_, &kept, approximate, &dy, &dx));
+    }
+    void accumulate_linear_grad8(uint32_t weight, const ttp_checkpoint8& kept,
+                                 const ttp_matrix& dy, uint32_t bias = TTP_NO_TENSOR,
+                                 bool transposed = false) {
+        check(ttp_accumulate_linear_grad8(ctx_, weight, bias, &kept, &dy, transposed ? 1 : 0));
+    }
+
     void save_state(const std::string& path) { check(ttp_save_state(ctx_, path.c_str())); }
     void load_state(const std::string& path) { check(ttp_load_state(ctx_, path.c_str())); }
     void begin_capture() {

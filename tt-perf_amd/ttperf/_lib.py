@@ -72,18 +72,19 @@ class Matrix(C.Structure):
                 ("stride", C.c_uint64), ("dtype", C.c_int32), ("reserved", C.c_int32)]
 
 
+# (pointers to matrices as addresses, C.addressof: a fifth of the time of C.pointer)
 class PreferenceArgs(C.Structure):
-    _fields_ = [("logits", C.POINTER(Matrix)), ("targets", _P), ("starts", _P),
+    _fields_ = [("logits", _P), ("targets", _P), ("starts", _P),
                 ("ref_logps", _P), ("pairs", C.c_uint64), ("beta", C.c_double),
-                ("label_smoothing", C.c_double), ("grad", C.POINTER(Matrix)), ("logps", _P),
+                ("label_smoothing", C.c_double), ("grad", _P), ("logps", _P),
                 ("margins", _P), ("loss", _P)]
 
 
 class PolicyArgs(C.Structure):
-    _fields_ = [("logits", C.POINTER(Matrix)), ("targets", _P), ("old_logps", _P),
+    _fields_ = [("logits", _P), ("targets", _P), ("old_logps", _P),
                 ("advantages", _P), ("ref_logps", _P), ("clip_low", C.c_double),
                 ("clip_high", C.c_double), ("kl_coef", C.c_double),
-                ("denominator", C.c_double), ("grad", C.POINTER(Matrix)), ("logps", _P),
+                ("denominator", C.c_double), ("grad", _P), ("logps", _P),
                 ("loss", _P), ("kl", _P)]
 
 

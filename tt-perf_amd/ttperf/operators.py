@@ -202,10 +202,9 @@ class Operators:
         given, g = self._gradient(grad, logits, out and out.grad)
         m, gm = _matrix(z), None if g is None else _matrix(g)
         args = L.PreferenceArgs(
-            logits=C.pointer(m), targets=y.data_ptr(), starts=at.data_ptr(), ref_logps=_ptr(ref),
-            pairs=pairs, beta=beta, label_smoothing=label_smoothing,
-            grad=None if gm is None else C.pointer(gm), logps=logps.data_ptr(),
-            margins=margins.data_ptr(), loss=loss.data_ptr())
+            C.addressof(m), y.data_ptr(), at.data_ptr(), _ptr(ref), pairs, beta, label_smoothing,
+            None if gm is None else C.addressof(gm), logps.data_ptr(), margins.data_ptr(),
+            loss.data_ptr())
         used = [t for t in (z, y, at, ref) if t is not None]
         if given is not None and grad is not True:
             used.append(g)
@@ -242,11 +241,9 @@ class Operators:
         given, g = self._gradient(grad, logits, out and out.grad)
         m, gm = _matrix(z), None if g is None else _matrix(g)
         args = L.PolicyArgs(
-            logits=C.pointer(m), targets=y.data_ptr(), old_logps=old.data_ptr(),
-            advantages=adv.data_ptr(), ref_logps=_ptr(ref), clip_low=low, clip_high=high,
-            kl_coef=kl_coef, denominator=denominator or 0.0,
-            grad=None if gm is None else C.pointer(gm), logps=logps.data_ptr(),
-            loss=loss.data_ptr(), kl=kl.data_ptr())
+            C.addressof(m), y.data_ptr(), old.data_ptr(), adv.data_ptr(), _ptr(ref), low, high,
+            kl_coef, denominator or 0.0, None if gm is None else C.addressof(gm),
+            logps.data_ptr(), loss.data_ptr(), kl.data_ptr())
         used = [t for t in (z, y, old, adv, ref) if t is not None]
         if given is not None and grad is not True:
             used.append(g)
