@@ -326,7 +326,7 @@ struct PairArgs {
     uint64_t rows, pairs;
     const double* part;
     double* pair_loss;
-    float beta, smoothing;
+    double beta, smoothing;
     const float* loss_scale;
     float *coef, *margins, *loss;
 };
@@ -357,13 +357,13 @@ __global__ __launch_bounds__(kBlock) void pair_losses_kernel(PairArgs a, uint32_
         d[k] = block_sum(x, lds);
     }
     if (threadIdx.x == 0) {
-        const double eps = (double)a.smoothing, h = (double)a.beta * (d[0] - d[1]);
+        const double eps = a.smoothing, h = a.beta * (d[0] - d[1]);
         a.margins[p] = (float)h;
         st_device(a.pair_loss + p, (1.0 - eps) * softplus(-h) + eps * softplus(h));
         // (each sigmoid by itself: their difference would lose the small one)
         const double dh = eps / (1.0 + exp(-h)) - (1.0 - eps) / (1.0 + exp(h));
         const double scale = a.loss_scale ? (double)*a.loss_scale : 1.0;
-        c = (float)(dh * (double)a.beta / (double)a.pairs * scale);
+        c = (float)(dh * a.beta / (double)a.pairs * scale);
     }
     __syncthreads();
 #pragma unroll
@@ -831,8 +831,8 @@ int ttp_preference_loss(ttp_ctx* ctx, const ttp_preference_args* p) {
         pa.pairs = p->pairs;
         pa.part = a.part;
         pa.pair_loss = (double*)(w + pair_loss);
-        pa.beta = (float)p->beta;
-        pa.smoothing = (float)p->label_smoothing;
+        pa.beta = p->beta;
+        pa.smoothing = p->label_smoothing;
         pa.loss_scale = op.loss_scale;
         pa.coef = a.coef;
         pa.margins = p->margins;
