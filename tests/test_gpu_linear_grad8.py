@@ -165,6 +165,19 @@ def test_what_is_not_finite_reaches_the_gradient():
             assert (~db.isfinite()).nonzero().flatten().tolist() == [9]
 
 
+def test_the_largest_numbers():
+    """dy up to the type's largest: its parts stay finite (the gradients too, under a small x)."""
+    torch = torch_mod()
+    for dtype in (torch.bfloat16, torch.float32):
+        x = torch.full((40, 32), 2.0 ** -20, device="cuda")
+        dy = torch.full((40, 24), torch.finfo(dtype).max, device="cuda", dtype=dtype)
+        dy[::2] = -dy[::2] / 2
+        with _store(32, 24, "fp32") as store:
+            kept = store.checkpoint8(x)
+            store.accumulate_linear_grad8(1, kept, dy)
+            _check(store, kept, dy, False, bias=False)
+
+
 def test_against_differences():
     """The gradient of sum(dy * (x W + b)) in W and b by differences: it is linear, so a difference
     over a step of 1 is exact but for the rounding of the loss."""

@@ -89,12 +89,12 @@ __device__ __forceinline__ void widen16(u32x4 w, uint32_t scale, u32x4 (&out)[2]
     }
 }
 
-// x as the sum of three bf16 (pairs packed)
+// x as the sum of three bf16 (pairs packed), exactly: each takes the leading 8 bits of what is
+// left.  (Cut off, not rounded: the largest numbers would round to infinity.)
 __device__ __forceinline__ void split3(float a, float b, uint32_t (&p)[3]) {
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
-        const f32x2 two = {a, b};
-        p[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(two, bf16x2));
+        p[k] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
         a -= bf16_lo(p[k]);
         b -= bf16_hi(p[k]);
     }
