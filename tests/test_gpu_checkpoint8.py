@@ -329,6 +329,12 @@ def test_refusals():
         refused(lambda: store.gelu_backward8(kept, x, out=torch.empty(6, 63, device="cuda")))
         wide = torch.randn(7, 64, device="cuda")
         refused(lambda: store.gelu_checkpoint8(wide[:6], out=wide[1:]))  # shifted by a row
+        # kept memory of other sizes or types
+        refused(lambda: ttperf.Checkpoint8(kept.values[:5], kept.scales, (6, 64), x.dtype, "int8"))
+        refused(lambda: ttperf.Checkpoint8(kept.values, kept.scales[:, :1], (6, 64), x.dtype,
+                                           "int8"))
+        refused(lambda: ttperf.Checkpoint8(kept.values.int(), kept.scales, (6, 64), x.dtype,
+                                           "int8"))
         # kept memory that overlaps, or is not aligned
         flat = torch.zeros(6 * 64 + 64, dtype=torch.uint8, device="cuda")
         off = ttperf.Checkpoint8(flat[8:8 + 384].view(6, 64), kept.scales, (6, 64), x.dtype,

@@ -10,6 +10,7 @@ the graph reads and writes the tensors in place at every launch.
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import Any, NamedTuple, Optional
 
 from . import _lib as L
@@ -50,7 +51,13 @@ class Checkpoint8:
         self.values, self.scales = values, scales
         self.shape, self.dtype, self.format = tuple(shape), dtype, fmt
         self.cols = self.shape[-1]
-        self.rows = values.shape[0]
+        self.rows = math.prod(self.shape[:-1])
+        blocks = -(-self.cols // L.CHECKPOINT_BLOCK)
+        for t, width in ((values, blocks * L.CHECKPOINT_BLOCK), (scales, blocks)):
+            if t.dtype != torch.uint8 or t.shape != (self.rows, width) or not t.is_contiguous():
+                raise ValueError(f"a checkpoint of shape {self.shape} has contiguous uint8 values "
+                                 f"and scales of {(self.rows, blocks * L.CHECKPOINT_BLOCK)} and "
+                                 f"{(self.rows, blocks)} elements")
 
     def _c(self):
         return L.Checkpoint8(self.values.data_ptr(), self.scales.data_ptr(), self.rows, self.cols,
