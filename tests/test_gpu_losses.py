@@ -261,6 +261,34 @@ def test_policy_loss(rows, vocab, dtype, kl, scale, denom):
     assert (r.grad[y < 0] == 0).all()
 
 
+@pytest.mark.parametrize("rows", [2047, 2048, 2049])
+@pytest.mark.parametrize("vocab", [65, 2500])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_policy_loss_where_its_launches_change(rows, vocab, dtype):
+    """Few rows are counted and summed by the launch that makes the gradient, more by their own:
+    the same numbers from either (the last rows masked: their logits are not the difference)."""
+    torch = torch_mod()
+    z, y = _logits(rows, vocab, getattr(torch, dtype), rows, 0, 0)
+    y[::5] = -1
+    y[2040:] = -1
+    g = torch.Generator().manual_seed(rows)
+    base = _logp64(z, y)
+    old = (base + 0.3 * torch.randn(rows, generator=g)).float().cuda()
+    adv = torch.randn(rows, generator=g).cuda()
+    with _store(scale=256.0) as store:
+        r = store.policy_loss(z, y, old, adv, old, kl_coef=0.1)
+        more = [torch.cat([t, t[-1:].expand(3, *t.shape[1:])]) for t in (z, y, old, adv)]
+        m = store.policy_loss(*more, more[2], kl_coef=0.1)
+    loss, mean_kl, logp = _policy64(z, y, old, adv, old, 0.2, 0.2, 0.1, None)
+    e = float(_logp_tol(z, y).max()) + 8 * U
+    assert abs(float(r.loss) - loss.item()) <= 4 * e * (abs(loss.item()) + 4)
+    assert abs(float(r.kl) - mean_kl.item()) <= 4 * e * (abs(mean_kl.item()) + 1)
+    assert torch.equal(m.grad[:rows], r.grad) and torch.equal(m.logps[:rows], r.logps)
+    # the sums are in 64 bits, in another order
+    assert abs(float(m.loss) - float(r.loss)) <= 2 * U * abs(float(r.loss))
+    assert abs(float(m.kl) - float(r.kl)) <= 2 * U * abs(float(r.kl))
+
+
 def test_policy_loss_without_a_row_that_counts():
     """All rows masked, their logits NaN: loss 0, gradient 0."""
     torch = torch_mod()

@@ -388,6 +388,12 @@ struct SumArgs {
     float *loss, *kl;
     float* norm;  // what the rows' c is multiplied with: the loss scale / D
 };
+__device__ __forceinline__ double denominator_of(const SumArgs& a, double unmasked) {
+    return a.denominator > 0.0 ? a.denominator : fmax(unmasked, 1.0);
+}
+__device__ __forceinline__ float norm_of(const SumArgs& a, double d) {
+    return (float)((a.loss_scale ? (double)*a.loss_scale : 1.0) / d);
+}
 __global__ __launch_bounds__(kBlock) void row_sums_kernel(SumArgs a, uint32_t* tickets) {
     __shared__ double lds[kBlock / 64];
     __shared__ uint32_t last;
@@ -412,12 +418,12 @@ __global__ __launch_bounds__(kBlock) void row_sums_kernel(SumArgs a, uint32_t* t
         x[k] = block_sum(v, lds);
     }
     if (threadIdx.x == 0) {
-        const double d = a.denominator > 0.0 ? a.denominator : fmax(x[0], 1.0);
+        const double d = denominator_of(a, x[0]);
         if (a.part) {
             *a.loss = (float)(x[1] / d);
             *a.kl = (float)(x[2] / d);
         }
-        *a.norm = (float)((a.loss_scale ? (double)*a.loss_scale : 1.0) / d);
+        *a.norm = norm_of(a, d);
     }
 }
 
@@ -501,13 +507,18 @@ __global__ __launch_bounds__(kGradBlock) void row_grads_kernel(GradArgs a, uint3
 // ---- policy_rows_kernel -------------------------------------------------------------------------
 // The policy loss and its gradient in one pass: a row's logits stay in kThreads lanes' registers
 // (kChunks 16-byte chunks each) from the statistics to the gradient, which needs nothing of other
-// rows but their number (a.norm, known before).  One row per kThreads lanes; without a gradient
+// rows but their number (its loss scale / D, known before).  One row per kThreads lanes; without a gradient
 // (o.g null) the losses alone.  The statistics are taken and joined part by part as
 // row_scores_kernel and its joins do, so that a token's log-probability has the same bits here as
 // there: the first step on a rollout finds ratios of exactly 1.
+// Up to this many rows the launch does everything (`tickets` given): each block counts the rows by
+// itself, and the last one adds up the losses.  (One launch for three: 1021 rows of 50257 fp32 85.8
+// to 78.3 us, a call over few rows 26 to 20 us of the host.  Above, every block's count of all rows
+// and one block's sum take longer than launches of their own.)
+constexpr uint32_t kAlone = 2048;
 template <class T, int kThreads, int kChunks>
-__global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void policy_rows_kernel(RowArgs a,
-                                                                                     GradArgs o) {
+__global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void policy_rows_kernel(
+    RowArgs a, GradArgs o, SumArgs sums, uint32_t* tickets) {
     constexpr int P = kPer<T>;
     constexpr bool kWaves = kThreads == 64;  // a row is a wave, and one part
     constexpr int kRows = kWaves ? 4 : 1;
@@ -516,105 +527,157 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void policy_rows_k
     static_assert(kChunks % kLoads == 0 || kParts == 1);
     __shared__ Stat lds[kWaves ? 1 : kGroups * kParts];
     __shared__ float token;  // (a row per block) the token's logit, read before its place is written
+    __shared__ uint32_t counted[kGroups];
+    const bool alone = tickets != nullptr;
     const uint32_t t = threadIdx.x % kThreads, lane = t & 63, chunks = a.cols / P;
     // (the same in a wave: its addresses are one scalar and 32 bits per lane)
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint64_t row = (uint64_t)blockIdx.x * kRows + (kWaves ? wave : 0);
-    if (row >= a.rows) return;  // (whole waves, and only where a row is a wave)
-    const T* z = (const T*)a.z + row * a.stride;
-    T* g = (T*)o.g + row * o.g_stride;
-    const int64_t y = a.targets[row];
-    const uint32_t splits = kWaves ? 1 : (chunks + kPart - 1) / kPart;
-    // chunk k of this lane; and for the lanes of the last part's wave the row's last elements
-    const auto chunk = [&](int k) {
-        return kWaves ? lane + k * 64
-                      : (wave + k / kLoads * kGroups) * kPart + k % kLoads * 64 + lane;
-    };
-    const uint32_t e = kWaves || (splits - 1) % kGroups == wave ? chunks * P + lane : a.cols;
-    // f(k, its bytes from the row's start) for this lane's chunks in the row
-    const auto each = [&](auto&& f) {
+    const auto do_row = [&]() {
+        const T* z = (const T*)a.z + row * a.stride;
+        T* g = (T*)o.g + row * o.g_stride;
+        const int64_t y = a.targets[row];
+        const uint32_t splits = kWaves ? 1 : (chunks + kPart - 1) / kPart;
+        // chunk k of this lane; and for the lanes of the last part's wave the row's last elements
+        const auto chunk = [&](int k) {
+            return kWaves ? lane + k * 64
+                          : (wave + k / kLoads * kGroups) * kPart + k % kLoads * 64 + lane;
+        };
+        const uint32_t e = kWaves || (splits - 1) % kGroups == wave ? chunks * P + lane : a.cols;
+        // f(k, its bytes from the row's start) for this lane's chunks in the row
+        const auto each = [&](auto&& f) {
 #pragma unroll
-        for (int k = 0; k < kChunks; ++k)
-            if (chunk(k) < chunks) f(k, chunk(k) * 16);
-    };
-    const auto zeros = [&]() {
-        each([&](int, uint32_t b) { store16_once((T*)((char*)g + b), u32x4{0, 0, 0, 0}); });
-        if (e < a.cols) narrow(0.0f, g + e);
-    };
-    if (y < 0) {
-        if (t == 0) {
-            a.logps[row] = 0.0f;
-            a.part[row] = a.part_kl[row] = 0.0;
-        }
-        if (o.g) zeros();
-        return;
-    }
-    u32x4 w[kChunks];
-#pragma unroll
-    for (int k = 0; k < kChunks; ++k) w[k] = no_logits<T>();
-    each([&](int k, uint32_t b) { w[k] = load16_once((const T*)((const char*)z + b)); });
-    const float ze = e < a.cols ? widen(z[e]) : -INFINITY;
-    float zy = 0.0f;
-    if (kWaves || t == 0) zy = token_logit<T>(a, row, y);
-    Stat st;
-    if constexpr (kWaves) {
-        st = wave_stat<T, kChunks, true>(w, ze);
-    } else {
-        if (t == 0) token = zy;
-#pragma unroll
-        for (int j = 0; j < kParts; ++j) {
-            const uint32_t part = wave + j * kGroups;
-            if (part < splits) {
-                st = wave_stat<T, kLoads, true>(w + kLoads * j,
-                                                part + 1 == splits ? ze : -INFINITY);
-                if (lane == 0) lds[part] = st;
+            for (int k = 0; k < kChunks; ++k)
+                if (chunk(k) < chunks) f(k, chunk(k) * 16);
+        };
+        const auto zeros = [&]() {
+            each([&](int, uint32_t b) { store16_once((T*)((char*)g + b), u32x4{0, 0, 0, 0}); });
+            if (e < a.cols) narrow(0.0f, g + e);
+        };
+        if (y < 0) {
+            if (t == 0) {
+                a.logps[row] = 0.0f;
+                st_device(a.part + row, 0.0);
+                st_device(a.part_kl + row, 0.0);
             }
+            if (o.g) zeros();
+            return;
         }
-        __syncthreads();
-        zy = token;
-        uint32_t lanes = 1;
-        while (lanes < splits && lanes < 64) lanes *= 2;
-        st = join_parts(splits, lanes, [&](uint32_t k) { return lds[k]; });
-    }
-    // every lane for itself: a second wait for one lane's result costs more
-    const float logp = row_logp(zy, st);
-    const PolicyRow p = policy_row(a, row, logp);
-    if (t == 0) {
-        a.logps[row] = logp;
-        a.part[row] = (double)p.loss;
-        a.part_kl[row] = (double)p.kl;
-    }
-    if (!o.g) return;
-    const float c = p.coef * *o.norm;
-    if (c == 0.0f) {
-        zeros();
-        return;
-    }
-    const float f = -c / st.s;
-    // the packed registers are unpacked once more: kept from before, the values would take two
-    // to four times the registers
+        uint32_t n = 0;  // the rows that count, of those that this wave looks at
+        if (alone && o.g && !(sums.denominator > 0.0)) {
 #pragma unroll
-    for (int k = 0; k < kChunks; ++k) asm volatile("" : "+v"(w[k]));
-    // a row off the 16-byte grid: its stores share cache lines, which L2 puts together
-    if ((uintptr_t)g % 16 == 0)
-        each([&](int k, uint32_t b) {
-            store16_once((T*)((char*)g + b), grad16(w[k], z, f, st.m));
-        });
-    else
-        each([&](int k, uint32_t b) {
-            store16((T*)((char*)g + b), grad16(w[k], z, f, st.m));
-        });
-    if (e < a.cols) {
-        const float v = f * power(ze, st.m);
-        narrow((int64_t)e == y ? v + c : v, g + e);
+            for (uint32_t i = 0; i < kAlone; i += kThreads) {
+                const bool one = i + t < a.rows && a.targets[i + t] >= 0;
+                n += __popcll(__ballot(one));
+            }
+            if (!kWaves && lane == 0) counted[wave] = n;
+        }
+        u32x4 w[kChunks];
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) w[k] = no_logits<T>();
+        each([&](int k, uint32_t b) { w[k] = load16_once((const T*)((const char*)z + b)); });
+        const float ze = e < a.cols ? widen(z[e]) : -INFINITY;
+        float zy = 0.0f;
+        if (kWaves || t == 0) zy = token_logit<T>(a, row, y);
+        Stat st;
+        if constexpr (kWaves) {
+            st = wave_stat<T, kChunks, true>(w, ze);
+        } else {
+            if (t == 0) token = zy;
+#pragma unroll
+            for (int j = 0; j < kParts; ++j) {
+                const uint32_t part = wave + j * kGroups;
+                if (part < splits) {
+                    st = wave_stat<T, kLoads, true>(w + kLoads * j,
+                                                    part + 1 == splits ? ze : -INFINITY);
+                    if (lane == 0) lds[part] = st;
+                }
+            }
+            __syncthreads();
+            zy = token;
+            uint32_t lanes = 1;
+            while (lanes < splits && lanes < 64) lanes *= 2;
+            st = join_parts(splits, lanes, [&](uint32_t k) { return lds[k]; });
+        }
+        // every lane for itself: a second wait for one lane's result costs more
+        const float logp = row_logp(zy, st);
+        const PolicyRow p = policy_row(a, row, logp);
+        if (t == 0) {
+            a.logps[row] = logp;
+            st_device(a.part + row, (double)p.loss);
+            st_device(a.part_kl + row, (double)p.kl);
+        }
+        if (!o.g) return;
+        if (alone && !kWaves) {
+            n = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kGroups; ++i) n += counted[i];
+        }
+        const float norm = alone ? norm_of(sums, denominator_of(sums, (double)n)) : *o.norm;
+        const float c = p.coef * norm;
+        if (c == 0.0f) {
+            zeros();
+            return;
+        }
+        const float f = -c / st.s;
+        // the packed registers are unpacked once more: kept from before, the values would take two
+        // to four times the registers
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k) asm volatile("" : "+v"(w[k]));
+        // a row off the 16-byte grid: its stores share cache lines, which L2 puts together
+        if ((uintptr_t)g % 16 == 0)
+            each([&](int k, uint32_t b) {
+                store16_once((T*)((char*)g + b), grad16(w[k], z, f, st.m));
+            });
+        else
+            each([&](int k, uint32_t b) {
+                store16((T*)((char*)g + b), grad16(w[k], z, f, st.m));
+            });
+        if (e < a.cols) {
+            const float v = f * power(ze, st.m);
+            narrow((int64_t)e == y ? v + c : v, g + e);
+        }
+        // the token's own: c more, in fp32, by the lane that has written its chunk
+        const uint64_t cy = (uint64_t)y / P;
+        if (cy < chunks) {
+            const uint32_t x = (uint32_t)cy;
+            const uint32_t owner = kWaves ? x % 64 : x / kPart % kGroups * 64 + x % 64;
+            if (owner == t) narrow(f * power(zy, st.m) + c, g + y);
+        }
+    };
+    if (row < a.rows) do_row();  // (whole waves are past the end, and only where a row is a wave)
+    if (!alone) return;
+    // the sums, by the launch's last block
+    __shared__ uint32_t last;
+    if constexpr (kWaves) {  // each wave has stored a row's part
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
     }
-    // the token's own: c more, in fp32, by the lane that has written its chunk
-    const uint64_t cy = (uint64_t)y / P;
-    if (cy < chunks) {
-        const uint32_t x = (uint32_t)cy;
-        const uint32_t owner = kWaves ? x % 64 : x / kPart % kGroups * 64 + x % 64;
-        if (owner == t) narrow(f * power(zy, st.m) + c, g + y);
+    if (!is_last_block(tickets, &last)) return;
+    constexpr uint32_t kBlockWaves = kWaves ? 4 : kGroups;
+    __shared__ double parts[3][kBlockWaves];
+    double x[3] = {0.0, 0.0, 0.0};
+    for (uint64_t i = threadIdx.x; i < a.rows; i += kBlockWaves * 64) {
+        x[0] += a.targets[i] >= 0 ? 1.0 : 0.0;
+        x[1] += ld_device(a.part + i);
+        x[2] += ld_device(a.part_kl + i);
     }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        x[k] = wave_sum(x[k]);
+        if (lane == 0) parts[k][threadIdx.x / 64] = x[k];
+    }
+    __syncthreads();
+    if (threadIdx.x) return;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        x[k] = 0.0;
+        for (uint32_t i = 0; i < kBlockWaves; ++i) x[k] += parts[k][i];
+    }
+    const double d = denominator_of(sums, x[0]);
+    *sums.loss = (float)(x[1] / d);
+    *sums.kl = (float)(x[2] / d);
 }
 
 // ---- launches -----------------------------------------------------------------------------------
@@ -714,14 +777,15 @@ bool policy_shape(uint32_t chunks, bool on_grid, F&& f) {
     return false;
 }
 template <class T>
-int launch_policy(const ttpi::Op& op, const RowArgs& a, const GradArgs& g) {
+int launch_policy(const ttpi::Op& op, const RowArgs& a, const GradArgs& g, const SumArgs& sums) {
     (void)hipGetLastError();
     const bool on_grid = ((uintptr_t)a.z | a.stride * sizeof(T)) % 16 == 0;
     policy_shape(a.cols / kPer<T>, on_grid, [&](auto lanes, auto chunks) {
         constexpr int kLanes = lanes, kChunks = chunks, kRows = kLanes < 256 ? 256 / kLanes : 1;
         hipLaunchKernelGGL((policy_rows_kernel<T, kLanes, kChunks>),
                            dim3((uint32_t)((a.rows + kRows - 1) / kRows)),
-                           dim3(kLanes < 256 ? 256 : kLanes), 0, op.stream, a, g);
+                           dim3(kLanes < 256 ? 256 : kLanes), 0, op.stream, a, g, sums,
+                           a.rows <= kAlone ? op.tickets : nullptr);
     });
     TTPI_HIP(hipGetLastError());
     return TTP_OK;
@@ -937,10 +1001,11 @@ int ttp_policy_loss(ttp_ctx* ctx, const ttp_policy_args* p) {
             rows && rows <= (1u << 21) &&
             policy_shape(row_chunks((uint32_t)cols, p->logits->dtype), true, [](auto, auto) {});
         if (one_pass) {
-            if (p->grad && (rc = launch_sums())) return rc;
-            rc = p->logits->dtype == TTP_DTYPE_BF16 ? launch_policy<uint16_t>(op, a, g)
-                                                    : launch_policy<float>(op, a, g);
-            if (rc) return rc;
+            const bool alone = rows <= kAlone;
+            if (!alone && p->grad && (rc = launch_sums())) return rc;
+            rc = p->logits->dtype == TTP_DTYPE_BF16 ? launch_policy<uint16_t>(op, a, g, sa)
+                                                    : launch_policy<float>(op, a, g, sa);
+            if (rc || alone) return rc;
             sa.part = a.part;
             sa.part_kl = a.part_kl;
             return launch_sums();
