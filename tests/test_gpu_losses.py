@@ -196,6 +196,15 @@ def test_preference_loss(rows, vocab, pairs, dtype, eps, with_ref, scale):
     assert (r.grad.cpu()[outside | (y < 0).cpu()] == 0).all()
 
 
+@pytest.mark.parametrize("rows,vocab,pairs", [(4096, 65, 2), (4096, 65, 16), (4096, 65, 17),
+                                              (4097, 65, 16), (300, 9000, 16), (300, 9000, 17)])
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_preference_loss_where_its_launches_change(rows, vocab, pairs, dtype):
+    """Few pairs over few rows are finished by the last block of the launch that scores the rows,
+    or of the one that joins their parts; more by a launch of their own."""
+    test_preference_loss(rows, vocab, pairs, dtype, 0.1, True, 512.0)
+
+
 def _policy64(z, y, old, adv, ref, low, high, k_coef, denom):
     torch = torch_mod()
     logp = _logp64(z, y)

@@ -131,7 +131,7 @@ struct RowArgs {
     const int64_t* targets;
     float* logps;
     // preference: the row's part of its sequence's sum, its statistics and its c (set to 0 here,
-    // by pair_losses_kernel where a sequence covers the row)
+    // by pair_losses_kernel or few_pairs where a sequence covers the row)
     const float* ref;
     double* part;
     Stat* stats;
@@ -184,9 +184,10 @@ __device__ __forceinline__ void finish_row(const RowArgs& a, uint64_t row, Stat 
     const float logp = y < 0 ? 0.0f : row_logp(token_logit<T>(a, row, y), st);
     a.logps[row] = logp;
     if constexpr (kLoss == kPreference) {
-        a.part[row] = y < 0 ? 0.0 : (double)logp - (a.ref ? (double)a.ref[row] : 0.0);
+        st_device(a.part + row, y < 0 ? 0.0 : (double)logp - (a.ref ? (double)a.ref[row] : 0.0));
         a.stats[row] = st;
-        a.coef[row] = 0.0f;
+        // (at memory before another block of this launch writes the sequence's c)
+        __hip_atomic_store(a.coef + row, 0.0f, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     } else if constexpr (kLoss == kPolicy) {
         PolicyRow p = {0.0f, 0.0f, 0.0f};
         if (y >= 0) p = policy_row(a, row, logp);
@@ -194,6 +195,80 @@ __device__ __forceinline__ void finish_row(const RowArgs& a, uint64_t row, Stat 
         a.part_kl[row] = (double)p.kl;
         a.stats[row] = st;
         a.coef[row] = p.coef;
+    }
+}
+
+// ---- a sequence's part of the loss ------------------------------------------------------------
+__device__ __forceinline__ uint64_t bounded(int64_t x, uint64_t lo, uint64_t hi) {
+    return x < (int64_t)lo ? lo : (uint64_t)x > hi ? hi : (uint64_t)x;
+}
+// log(1 + exp(x))
+__device__ __forceinline__ double softplus(double x) {
+    return fmax(x, 0.0) + log1p(exp(-fabs(x)));
+}
+
+struct PairArgs {
+    const int64_t* starts;
+    uint64_t rows, pairs;
+    const double* part;
+    double* pair_loss;
+    double beta, smoothing;
+    const float* loss_scale;
+    float *coef, *margins, *loss;
+};
+// One pair's loss from its margin h, and its c = scale dloss/dmargin beta / pairs.
+__device__ __forceinline__ double pair_loss(const PairArgs& a, double h) {
+    const double eps = a.smoothing;
+    return (1.0 - eps) * softplus(-h) + eps * softplus(h);
+}
+__device__ __forceinline__ float pair_coef(const PairArgs& a, double h) {
+    // (each sigmoid by itself: their difference would lose the small one)
+    const double eps = a.smoothing, dh = eps / (1.0 + exp(-h)) - (1.0 - eps) / (1.0 + exp(h));
+    const double scale = a.loss_scale ? (double)*a.loss_scale : 1.0;
+    return (float)(dh * a.beta / (double)a.pairs * scale);
+}
+
+// The pairs of few rows, by the block that sees them all finished: 16 lanes to a sequence.  Up to
+// kFewPairs and kFewRows: a launch less is 3 us of the host (250 to 4000 rows, 4 or 16 pairs: 26 to
+// 23.5 us a call, the GPU's time the same; 64 pairs take it 6 us more).
+constexpr uint32_t kFewPairs = 16, kFewRows = 4096;
+static_assert(kBlock == 256);
+__device__ __forceinline__ void few_pairs(const PairArgs& a) {
+    constexpr uint32_t kLanes = 16, kLoads = 16;
+    __shared__ double d[2 * kFewPairs], lds[kBlock / 64];
+    __shared__ float c[kFewPairs];
+    const uint32_t t = threadIdx.x, lane = t % kLanes, sequences = 2 * (uint32_t)a.pairs;
+    for (uint32_t s = t / kLanes; s < sequences; s += kBlock / kLanes) {
+        const uint32_t lo = (uint32_t)bounded(a.starts[s], 0, a.rows);
+        const uint32_t hi = (uint32_t)bounded(a.starts[s + 1], lo, a.rows);
+        double x = 0.0;
+        // (the loads of 256 rows together: each comes from memory)
+        for (uint32_t r = lo + lane; r < hi; r += kLanes * kLoads) {
+            double v[kLoads];
+#pragma unroll
+            for (uint32_t k = 0; k < kLoads; ++k)
+                v[k] = ld_device(a.part + min(r + k * kLanes, hi - 1));
+#pragma unroll
+            for (uint32_t k = 0; k < kLoads; ++k) x += r + k * kLanes < hi ? v[k] : 0.0;
+        }
+        for (uint32_t off = kLanes / 2; off; off >>= 1) x += __shfl_xor(x, (int)off);
+        if (lane == 0) d[s] = x;
+    }
+    __syncthreads();
+    double x = 0.0;
+    if (t < a.pairs) {
+        const double h = a.beta * (d[t] - d[t + a.pairs]);
+        a.margins[t] = (float)h;
+        x = pair_loss(a, h);
+        c[t] = pair_coef(a, h);
+    }
+    x = block_sum(x, lds);
+    if (t == 0) *a.loss = (float)(x / (double)a.pairs);
+    for (uint32_t s = t / kLanes; s < sequences; s += kBlock / kLanes) {
+        const uint32_t lo = (uint32_t)bounded(a.starts[s], 0, a.rows);
+        const uint32_t hi = (uint32_t)bounded(a.starts[s + 1], lo, a.rows);
+        const float v = s < a.pairs ? c[s] : -c[s - a.pairs];
+        for (uint32_t r = lo + lane; r < hi; r += kLanes) a.coef[r] = v;
     }
 }
 
@@ -248,7 +323,7 @@ template <class T, Loss kLoss>
 __global__ __launch_bounds__(kRowBlock) void row_scores_kernel(RowArgs a, uint32_t splits,
                                                                uint32_t lanes, double* parts,
                                                                uint32_t last_joins,
-                                                               uint32_t* tickets) {
+                                                               PairArgs pairs, uint32_t* tickets) {
     constexpr uint32_t kWaves = kRowBlock / 64;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     // a step of all the launch's waves, as rows and parts: no division per part
@@ -287,7 +362,8 @@ __global__ __launch_bounds__(kRowBlock) void row_scores_kernel(RowArgs a, uint32
         now = next;
         advance(next);
     }
-    if (!last_joins) return;
+    const bool here = kLoss == kPreference && pairs.starts && (splits == 1 || last_joins);
+    if (!last_joins && !here) return;
     __shared__ uint32_t last;
     // every wave's parts are at memory before the block takes its ticket
     asm volatile("" ::: "memory");
@@ -295,19 +371,28 @@ __global__ __launch_bounds__(kRowBlock) void row_scores_kernel(RowArgs a, uint32
     __syncthreads();
     if (!is_last_block(tickets, &last)) return;
     const uint32_t rows = kRowBlock / lanes;
-    for (uint64_t base = 0; base < a.rows; base += rows) {
-        const uint64_t row = min(base + threadIdx.x / lanes, a.rows - 1);
-        const Stat st = join_parts(splits, lanes, [&](uint32_t k) {
-            return __builtin_bit_cast(Stat, ld_device(parts + row * splits + k));
-        });
-        if (base + threadIdx.x / lanes < a.rows && threadIdx.x % lanes == 0)
-            finish_row<T, kLoss>(a, row, st);
-    }
+    if (last_joins)
+        for (uint64_t base = 0; base < a.rows; base += rows) {
+            const uint64_t row = min(base + threadIdx.x / lanes, a.rows - 1);
+            const Stat st = join_parts(splits, lanes, [&](uint32_t k) {
+                return __builtin_bit_cast(Stat, ld_device(parts + row * splits + k));
+            });
+            if (base + threadIdx.x / lanes < a.rows && threadIdx.x % lanes == 0)
+                finish_row<T, kLoss>(a, row, st);
+        }
+    if constexpr (kLoss == kPreference)
+        if (here) {
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0);
+            __syncthreads();
+            few_pairs(pairs);
+        }
 }
 template <class T, Loss kLoss>
 __global__ __launch_bounds__(kRowBlock) void finish_rows_kernel(RowArgs a, uint32_t splits,
                                                                 uint32_t lanes,
-                                                                const double* parts) {
+                                                                const double* parts, PairArgs pairs,
+                                                                uint32_t* tickets) {
     const uint32_t rows = kRowBlock / lanes;
     for (uint64_t base = (uint64_t)blockIdx.x * rows; base < a.rows;
          base += (uint64_t)gridDim.x * rows) {
@@ -318,26 +403,17 @@ __global__ __launch_bounds__(kRowBlock) void finish_rows_kernel(RowArgs a, uint3
         if (base + threadIdx.x / lanes < a.rows && threadIdx.x % lanes == 0)
             finish_row<T, kLoss>(a, row, st);
     }
+    if constexpr (kLoss == kPreference) {
+        if (!pairs.starts) return;
+        __shared__ uint32_t last;
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0);
+        __syncthreads();
+        if (is_last_block(tickets, &last)) few_pairs(pairs);
+    }
 }
 
 // ---- pair_losses_kernel -----------------------------------------------------------------------
-struct PairArgs {
-    const int64_t* starts;
-    uint64_t rows, pairs;
-    const double* part;
-    double* pair_loss;
-    double beta, smoothing;
-    const float* loss_scale;
-    float *coef, *margins, *loss;
-};
-__device__ __forceinline__ uint64_t bounded(int64_t x, uint64_t lo, uint64_t hi) {
-    return x < (int64_t)lo ? lo : (uint64_t)x > hi ? hi : (uint64_t)x;
-}
-// log(1 + exp(x))
-__device__ __forceinline__ double softplus(double x) {
-    return fmax(x, 0.0) + log1p(exp(-fabs(x)));
-}
-
 // Block p: pair p.  Sums in fp64 (a margin is the small difference of sums over hundreds of
 // tokens), each lane's share in row order, then the block's lanes in a fixed order.
 __global__ __launch_bounds__(kBlock) void pair_losses_kernel(PairArgs a, uint32_t* tickets) {
@@ -357,13 +433,10 @@ __global__ __launch_bounds__(kBlock) void pair_losses_kernel(PairArgs a, uint32_
         d[k] = block_sum(x, lds);
     }
     if (threadIdx.x == 0) {
-        const double eps = a.smoothing, h = a.beta * (d[0] - d[1]);
+        const double h = a.beta * (d[0] - d[1]);
         a.margins[p] = (float)h;
-        st_device(a.pair_loss + p, (1.0 - eps) * softplus(-h) + eps * softplus(h));
-        // (each sigmoid by itself: their difference would lose the small one)
-        const double dh = eps / (1.0 + exp(-h)) - (1.0 - eps) / (1.0 + exp(h));
-        const double scale = a.loss_scale ? (double)*a.loss_scale : 1.0;
-        c = (float)(dh * a.beta / (double)a.pairs * scale);
+        st_device(a.pair_loss + p, pair_loss(a, h));
+        c = pair_coef(a, h);
     }
     __syncthreads();
 #pragma unroll
@@ -513,8 +586,9 @@ __global__ __launch_bounds__(kGradBlock) void row_grads_kernel(GradArgs a, uint3
 // there: the first step on a rollout finds ratios of exactly 1.
 // Up to this many rows the launch does everything (`tickets` given): each block counts the rows by
 // itself, and the last one adds up the losses.  (One launch for three: 1021 rows of 50257 fp32 85.8
-// to 78.3 us, a call over few rows 26 to 20 us of the host.  Above, every block's count of all rows
-// and one block's sum take longer than launches of their own.)
+// to 78.3 us, a call over few rows 26 to 20 us of the host, 2000 rows of 50257 bf16 94.8 to 93.6 us.
+// Above, every block's count of all rows and one block's sum take longer than launches of their
+// own: 4000 rows 204 us against 187.)
 constexpr uint32_t kAlone = 2048;
 template <class T, int kThreads, int kChunks>
 __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void policy_rows_kernel(
@@ -704,7 +778,8 @@ Split split_rows(uint64_t rows, uint32_t cols, int dtype) {
 }
 
 template <Loss kLoss, class T>
-int launch_scores_of(const ttpi::Op& op, const RowArgs& a, Split sp, double* parts) {
+int launch_scores_of(const ttpi::Op& op, const RowArgs& a, Split sp, double* parts,
+                     const PairArgs& pairs) {
     if (!a.rows) return TTP_OK;
     // (four rounds of blocks that fit the GPU at once: each wave starts its next part while it
     // sums one, and the rounds even out what masked rows leave)
@@ -712,20 +787,22 @@ int launch_scores_of(const ttpi::Op& op, const RowArgs& a, Split sp, double* par
                                                                    (uint64_t)op.num_cus * 32));
     (void)hipGetLastError();
     hipLaunchKernelGGL((row_scores_kernel<T, kLoss>), grid, block, 0, op.stream, a, sp.splits,
-                       sp.lanes, parts, sp.last_joins ? 1u : 0u, op.tickets);
+                       sp.lanes, parts, sp.last_joins ? 1u : 0u, pairs, op.tickets);
     TTPI_HIP(hipGetLastError());
     if (sp.splits == 1 || sp.last_joins) return TTP_OK;
     const uint64_t per_block = kRowBlock / sp.lanes;
     hipLaunchKernelGGL((finish_rows_kernel<T, kLoss>),
                        dim3(grid_of((a.rows + per_block - 1) / per_block)), block, 0, op.stream, a,
-                       sp.splits, sp.lanes, (const double*)parts);
+                       sp.splits, sp.lanes, (const double*)parts, pairs, op.tickets);
     TTPI_HIP(hipGetLastError());
     return TTP_OK;
 }
+// `pairs` (preference): finished in the same launches, where its starts are given.
 template <Loss kLoss>
-int launch_scores(const ttpi::Op& op, const RowArgs& a, int dtype, Split sp, double* parts) {
-    return dtype == TTP_DTYPE_BF16 ? launch_scores_of<kLoss, uint16_t>(op, a, sp, parts)
-                                   : launch_scores_of<kLoss, float>(op, a, sp, parts);
+int launch_scores(const ttpi::Op& op, const RowArgs& a, int dtype, Split sp, double* parts,
+                  const PairArgs& pairs = {}) {
+    return dtype == TTP_DTYPE_BF16 ? launch_scores_of<kLoss, uint16_t>(op, a, sp, parts, pairs)
+                                   : launch_scores_of<kLoss, float>(op, a, sp, parts, pairs);
 }
 
 template <class T>
@@ -886,9 +963,6 @@ int ttp_preference_loss(ttp_ctx* ctx, const ttp_preference_args* p) {
         a.part = (double*)(w + part);
         a.stats = (Stat*)(w + stats);
         a.coef = (float*)(w + coef);
-        if ((rc = launch_scores<kPreference>(op, a, p->logits->dtype, sp, (double*)(w + parts))))
-            return rc;
-
         PairArgs pa{};
         pa.starts = p->starts;
         pa.rows = rows;
@@ -901,10 +975,16 @@ int ttp_preference_loss(ttp_ctx* ctx, const ttp_preference_args* p) {
         pa.coef = a.coef;
         pa.margins = p->margins;
         pa.loss = p->loss;
-        (void)hipGetLastError();
-        hipLaunchKernelGGL(pair_losses_kernel, dim3((uint32_t)p->pairs), dim3(kBlock), 0,
-                           op.stream, pa, op.tickets);
-        TTPI_HIP(hipGetLastError());
+        const bool few = rows && rows <= kFewRows && p->pairs <= kFewPairs;
+        if ((rc = launch_scores<kPreference>(op, a, p->logits->dtype, sp, (double*)(w + parts),
+                                             few ? pa : PairArgs{})))
+            return rc;
+        if (!few) {
+            (void)hipGetLastError();
+            hipLaunchKernelGGL(pair_losses_kernel, dim3((uint32_t)p->pairs), dim3(kBlock), 0,
+                               op.stream, pa, op.tickets);
+            TTPI_HIP(hipGetLastError());
+        }
         if (!p->grad) return TTP_OK;
         GradArgs g{a.z,    p->grad->data, rows,    a.stride, p->grad->stride,
                    a.cols, p->targets,    a.stats, a.coef,   nullptr};
