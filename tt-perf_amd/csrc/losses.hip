@@ -597,8 +597,8 @@ __global__ __launch_bounds__(kGradBlock) void row_grads_kernel(GradArgs a, uint3
 // row_scores_kernel and its joins do, so that a token's log-probability has the same bits here as
 // there: the first step on a rollout finds ratios of exactly 1.
 // Bound by HBM, and by how few rows a CU holds: one row's loads have to cover another's
-// exponentials and stores.  16384 rows of 50257 bf16 every 50304 575 us, 5.7 TB/s; every 50257, so
-// off the 16-byte grid, 709 us (the loads' share of the difference 60 us, the stores' 20) where two
+// exponentials and stores.  16384 rows of 50257 bf16 every 50304 565 us, 5.8 TB/s; every 50257, so
+// off the 16-byte grid, 720 us (the loads' share of the difference 60 us, the stores' 20) where two
 // passes take 854 (816 over batches of rows that the 256 MB cache holds); 1021 rows of 50257 fp32
 // 78 us, 5.2 TB/s.
 
@@ -625,6 +625,17 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void policy_rows_k
     // (the same in a wave: its addresses are one scalar and 32 bits per lane)
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint64_t row = (uint64_t)blockIdx.x * kRows + (kWaves ? wave : 0);
+    // The rows that count, of those that this wave looks at.  (Out here: behind the masked row's
+    // return, the 1024-lane shapes took 680 us for 565, alone or not.)
+    uint32_t n = 0;
+    if (alone && o.g && !(sums.denominator > 0.0)) {
+#pragma unroll
+        for (uint32_t i = 0; i < kAlone; i += kThreads) {
+            const bool one = i + t < a.rows && a.targets[i + t] >= 0;
+            n += __popcll(__ballot(one));
+        }
+        if (!kWaves && lane == 0) counted[wave] = n;
+    }
     const auto do_row = [&]() {
         const T* z = (const T*)a.z + row * a.stride;
         T* g = (T*)o.g + row * o.g_stride;
@@ -655,15 +666,8 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void policy_rows_k
             if (o.g) zeros();
             return;
         }
-        uint32_t n = 0;  // the rows that count, of those that this wave looks at
-        if (alone && o.g && !(sums.denominator > 0.0)) {
-#pragma unroll
-            for (uint32_t i = 0; i < kAlone; i += kThreads) {
-                const bool one = i + t < a.rows && a.targets[i + t] >= 0;
-                n += __popcll(__ballot(one));
-            }
-            if (!kWaves && lane == 0) counted[wave] = n;
-        }
+        // (read now: behind the statistics every row would wait for it)
+        float norm = !alone && o.g ? *o.norm : 0.0f;
         u32x4 w[kChunks];
 #pragma unroll
         for (int k = 0; k < kChunks; ++k) w[k] = no_logits<T>();
@@ -700,12 +704,14 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void policy_rows_k
             st_device(a.part_kl + row, (double)p.kl);
         }
         if (!o.g) return;
-        if (alone && !kWaves) {
-            n = 0;
+        if (alone) {
+            if (!kWaves) {
+                n = 0;
 #pragma unroll
-            for (uint32_t i = 0; i < kGroups; ++i) n += counted[i];
+                for (uint32_t i = 0; i < kGroups; ++i) n += counted[i];
+            }
+            norm = norm_of(sums, denominator_of(sums, (double)n));
         }
-        const float norm = alone ? norm_of(sums, denominator_of(sums, (double)n)) : *o.norm;
         const float c = p.coef * norm;
         if (c == 0.0f) {
             zeros();
