@@ -618,7 +618,6 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void policy_rows_k
     constexpr int kParts = (kChunks + kLoads - 1) / kLoads;  // of a wave
     static_assert(kChunks % kLoads == 0 || kParts == 1);
     __shared__ Stat lds[kWaves ? 1 : kGroups * kParts];
-    __shared__ float token;  // (a row per block) the token's logit, read before its place is written
     __shared__ uint32_t counted[kGroups];
     const bool alone = tickets != nullptr;
     const uint32_t t = threadIdx.x % kThreads, lane = t & 63, chunks = a.cols / P;
@@ -668,18 +667,20 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void policy_rows_k
         }
         // (read now: behind the statistics every row would wait for it)
         float norm = !alone && o.g ? *o.norm : 0.0f;
+        // (first, and without a branch to wait in: their values are there once the chunks are)
+        const T last_z = z[min(e, a.cols - 1)];
+        const T token_z = z[min((uint64_t)y, (uint64_t)a.cols - 1)];
         u32x4 w[kChunks];
 #pragma unroll
         for (int k = 0; k < kChunks; ++k) w[k] = no_logits<T>();
         each([&](int k, uint32_t b) { w[k] = load16_once((const T*)((const char*)z + b)); });
-        const float ze = e < a.cols ? widen(z[e]) : -INFINITY;
-        float zy = 0.0f;
-        if (kWaves || t == 0) zy = token_logit<T>(a, row, y);
+        const float ze = e < a.cols ? widen(last_z) : -INFINITY;
+        float zy = y < (int64_t)a.cols ? widen(token_z) : NAN;
+        asm volatile("" : "+v"(zy));  // read before any lane writes a gradient in its place
         Stat st;
         if constexpr (kWaves) {
             st = wave_stat<T, kChunks, true>(w, ze);
         } else {
-            if (t == 0) token = zy;
 #pragma unroll
             for (int j = 0; j < kParts; ++j) {
                 const uint32_t part = wave + j * kGroups;
@@ -690,7 +691,6 @@ __global__ __launch_bounds__(kThreads < 256 ? 256 : kThreads) void policy_rows_k
                 }
             }
             __syncthreads();
-            zy = token;
             uint32_t lanes = 1;
             while (lanes < splits && lanes < 64) lanes *= 2;
             st = join_parts(splits, lanes, [&](uint32_t k) { return lds[k]; });
