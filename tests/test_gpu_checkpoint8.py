@@ -329,6 +329,9 @@ def test_refusals():
         refused(lambda: store.gelu_backward8(kept, x, out=torch.empty(6, 63, device="cuda")))
         wide = torch.randn(7, 64, device="cuda")
         refused(lambda: store.gelu_checkpoint8(wide[:6], out=wide[1:]))  # shifted by a row
+        # another activation's type: what is restored would have it
+        refused(lambda: store.checkpoint8(x.bfloat16(), out=kept))
+        refused(lambda: store.gelu_checkpoint8(x.bfloat16(), kept=kept))
         # kept memory of other sizes or types
         refused(lambda: ttperf.Checkpoint8(kept.values[:5], kept.scales, (6, 64), x.dtype, "int8"))
         refused(lambda: ttperf.Checkpoint8(kept.values, kept.scales[:, :1], (6, 64), x.dtype,

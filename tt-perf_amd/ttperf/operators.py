@@ -271,8 +271,9 @@ class Operators:
         rows, cols = x.shape
         blocks = -(-cols // L.CHECKPOINT_BLOCK)
         if out is not None and (not isinstance(out, Checkpoint8) or out.format != fmt or
-                                out.shape != tuple(shape)):
-            raise ValueError(f"out must be a checkpoint of shape {tuple(shape)} in {fmt}")
+                                out.shape != tuple(shape) or out.dtype != x.dtype):
+            raise ValueError(f"out must be a checkpoint of shape {tuple(shape)} in {fmt}, of a "
+                             f"{str(x.dtype)[6:]} activation")
         values = self._result(out and out.values, x, (rows, blocks * L.CHECKPOINT_BLOCK),
                               torch.uint8, "the checkpoint")
         scales = self._result(out and out.scales, x, (rows, blocks), torch.uint8,
