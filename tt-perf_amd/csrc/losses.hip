@@ -286,36 +286,47 @@ constexpr int kRowBlock = 256;
 constexpr int kLoads = 4;
 constexpr uint32_t kPart = kLoads * 64;
 
-// One part on its way through a wave: where it is, whether its row counts, its logits.
-template <class T>
-struct Part {
+// Where a wave is: a part of a row, and whether the row counts (a masked row's logits are not read).
+struct Place {
     uint64_t row;
     uint32_t part;
     bool live;
+};
+// A part on its way through a wave.  Its loads are issued without a branch, so that what is waited
+// for can be counted and the next part's stay in flight: lanes that have no chunk load the row's
+// last one, and a row without one, or that does not count, loads from `other`.
+template <class T>
+struct Part {
     u32x4 w[kLoads];
-    float extra;
+    T last;
 
-    __device__ __forceinline__ void look(const RowArgs& a) {
-        live = row < a.rows && a.targets[row] >= 0;  // a masked row's logits are not read
-    }
     // (kOnce: no gradient kernel reads them again soon)
     template <bool kOnce>
-    __device__ __forceinline__ void load(const RowArgs& a, uint32_t splits) {
+    __device__ __forceinline__ void load(const RowArgs& a, const Place& at, const void* other) {
         constexpr int P = kPer<T>;
         const uint32_t chunks = a.cols / P, lane = threadIdx.x & 63;
-        const T* z = (const T*)a.z + row * a.stride;
-        extra = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < kLoads; ++k) w[k] = no_logits<T>();
-        if (!live) return;
+        const T* z = at.live ? (const T*)a.z + at.row * a.stride : (const T*)other;
+        last = z[at.live ? min(chunks * P + lane, a.cols - 1) : 0u];
+        const T* first = chunks ? z : (const T*)other;
+        const uint32_t top = at.live && chunks ? chunks - 1 : 0;
 #pragma unroll
         for (int k = 0; k < kLoads; ++k) {
-            const uint32_t c = part * kPart + k * 64 + lane;
-            const T* p = z + (uint64_t)c * P;
-            if (c < chunks) w[k] = kOnce ? load16_once(p) : load16(p);
+            const uint32_t c = min(at.part * kPart + k * 64 + lane, top);
+            const T* p = first + (uint64_t)c * P;
+            w[k] = kOnce ? load16_once(p) : load16(p);
         }
-        const uint32_t e = chunks * P + lane;
-        if (part + 1 == splits && e < a.cols) extra = widen(z[e]);
+    }
+    __device__ __forceinline__ Stat stat(const RowArgs& a, const Place& at, uint32_t splits) {
+        constexpr int P = kPer<T>;
+        const uint32_t chunks = a.cols / P, lane = threadIdx.x & 63;
+        float extra = -INFINITY;
+        if (at.part + 1 == splits) {
+            if (chunks * P + lane < a.cols) extra = widen(last);
+#pragma unroll
+            for (int k = 0; k < kLoads; ++k)
+                if (at.part * kPart + k * 64 + lane >= chunks) w[k] = no_logits<T>();
+        }
+        return wave_stat<T, kLoads, false>(w, extra);
     }
 };
 
@@ -324,7 +335,7 @@ struct Part {
 // finish_rows_kernel does; rows of one part are finished at once.
 // Bound by the exponentials and reading the logits, about evenly.  Parts rather than rows per block:
 // the waves in flight then sweep a narrow window of memory.  Measured: 8192 rows of 50257 bf16 (one
-// in ten masked) 134 us, 5.5 TB/s of the logits it reads; one such row in 7 blocks 6 us, of which
+// in ten masked) 131 us, 5.65 TB/s of the logits it reads (on the 16-byte grid 5.9, fp32 6.1); one such row in 7 blocks 6 us, of which
 // three quarters are the launch, the first loads and the join.
 template <class T, Loss kLoss>
 __global__ __launch_bounds__(kRowBlock) void row_scores_kernel(RowArgs a, uint32_t splits,
@@ -336,38 +347,48 @@ __global__ __launch_bounds__(kRowBlock) void row_scores_kernel(RowArgs a, uint32
     // a step of all the launch's waves, as rows and parts: no division per part
     const uint32_t step = gridDim.x * kWaves;
     const uint32_t step_rows = step / splits, step_parts = step - step_rows * splits;
-    const auto advance = [&](Part<T>& p) {
-        p.row += step_rows;
-        p.part += step_parts;
-        if (p.part >= splits) {
-            p.part -= splits;
-            p.row += 1;
+    // (by the scalar unit: nothing writes to the targets meanwhile, and vector loads in flight are
+    // not waited for)
+    const auto* targets = (const __attribute__((address_space(4))) int64_t*)(uintptr_t)a.targets;
+    const auto look = [&](Place& p) { p.live = p.row < a.rows && targets[p.row] >= 0; };
+    const auto behind = [&](const Place& p) {
+        Place n{p.row + step_rows, p.part + step_parts, false};
+        if (n.part >= splits) {
+            n.part -= splits;
+            n.row += 1;
         }
-        p.look(a);
+        look(n);
+        return n;
     };
-    // the next part's logits and the one after's target are on their way while one is summed
-    Part<T> now, next;
-    const uint32_t first = blockIdx.x * kWaves + wave;
-    now.row = first / splits;
-    now.part = first - (uint32_t)now.row * splits;
-    now.look(a);
-    next.row = now.row;
-    next.part = now.part;
-    advance(next);
-    constexpr bool kOnce = kLoss == kScore;
-    now.template load<kOnce>(a, splits);
-    while (now.row < a.rows) {
-        next.template load<kOnce>(a, splits);
+    const auto finish = [&](Part<T>& p, const Place& at) {
         Stat st = {-INFINITY, 0.0f};
-        if (now.live) st = wave_stat<T, kLoads, false>(now.w, now.extra);
+        if (at.live) st = p.stat(a, at, splits);
         if ((threadIdx.x & 63) == 0) {
             if (splits == 1)
-                finish_row<T, kLoss>(a, now.row, st);
+                finish_row<T, kLoss>(a, at.row, st);
             else
-                st_device(parts + now.row * splits + now.part, __builtin_bit_cast(double, st));
+                st_device(parts + at.row * splits + at.part, __builtin_bit_cast(double, st));
         }
-        now = next;
-        advance(next);
+    };
+    // the next part's logits are on their way while one is summed
+    constexpr bool kOnce = kLoss == kScore;
+    const uint32_t first = blockIdx.x * kWaves + wave;
+    Part<T> one, two;
+    Place at{first / splits, 0, false}, next;
+    at.part = first - (uint32_t)at.row * splits;
+    look(at);
+    if (at.row < a.rows) {
+        one.template load<kOnce>(a, at, tickets);
+        for (;;) {
+            next = behind(at);
+            two.template load<kOnce>(a, next, tickets);
+            finish(one, at);
+            if (next.row >= a.rows) break;
+            at = behind(next);
+            one.template load<kOnce>(a, at, tickets);
+            finish(two, next);
+            if (at.row >= a.rows) break;
+        }
     }
     const bool here = kLoss == kPreference && pairs.starts && (splits == 1 || last_joins);
     if (!last_joins && !here) return;
