@@ -91,10 +91,10 @@ __device__ __forceinline__ Place place(const KeptArgs& a, uint32_t i) {
 constexpr float kSqrt2OverPi = 0.79788456080286535588f;
 constexpr float kCubic = 0.044715f;
 
-// The normal distribution function and its density at x.  With z = |x| / sqrt 2, t = 1 / (1 + 0.46 z),
-// erfc(z) = t poly(t) exp(-z^2), whose exponential is the density's.  poly is of the sixth degree,
-// fitted here by least maximum error to exp(z^2) erfc(z) / t over z = 0 to 25, weighted by
-// t max(exp(-z^2), 1e-4): 5e-9 of erfc, 6e-5 of itself out to x = -6.
+// The normal distribution function and its density at x.  With z = |x| / sqrt 2 and
+// t = 1 / (1 + 0.46 z), erfc(z) = t poly(t) exp(-z^2), whose exponential is the density's.  poly is
+// of the sixth degree, fitted here by least maximum error to exp(z^2) erfc(z) / t over z = 0 to 25,
+// weighted by t max(exp(-z^2), 1e-4): to 5e-9 of erfc, and 6e-5 of itself out to x = -6.
 struct Normal {
     float cdf, pdf;
 };

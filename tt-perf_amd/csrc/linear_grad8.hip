@@ -14,9 +14,9 @@
 // in flight while the matrix instructions run.  Few tiles split the rows: each part writes its
 // fp32 tile to scratch memory and join_parts_kernel adds them up in order.
 //
-// Measured, bf16 8192 x 1280 x 5120 (256 x 256 tiles, two parts: 200 blocks for 256 CUs): 115 to 130
-// us by the card's clock, 825 to 930 TFLOP/s, and the join 11; on a CU with a block the matrix pipe is
-// busy half of the time, the LDS 0.4 of it, and what is left are waits at the steps' barriers.
+// Measured, bf16 8192 x 1280 x 5120 (256 x 256 tiles, two parts: 200 blocks for 256 CUs) 115 to
+// 130 us by the card's clock, 825 to 930 TFLOP/s, and the join 11; on a CU with a block the matrix
+// pipe is busy half of the time, the LDS 0.4; the rest are waits at the steps' barriers.
 // fp32 3585 x 384 x 1536 (128 x 128 tiles, seven parts of 512 rows): 25 us, three products each; the
 // matrix pipe is busy a quarter of the time, 16 steps are too few to hide the first and the last.
 #include <hip/hip_runtime.h>
@@ -295,7 +295,8 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads == 512 ? 1 : 2) void linea
             for (int k = 0; k < kChunksB; ++k) {
                 const G* p = pb + (uint64_t)(k * kRowsB) * a.dy_stride;
                 const int n = tb + k * kRowsB < left ? some_b : 0;
-                const bool spill = a.outs >= 8 && row0 + step * T::kN + tb + k * kRowsB + 1 < a.rows;
+                const uint64_t row = row0 + step * T::kN + tb + k * kRowsB;
+                const bool spill = a.outs >= 8 && row + 1 < a.rows;
                 if (n == 8 || (n && spill)) {
                     r.b[k].load(p);
                     if (n < 8) r.b[k].keep(n);

@@ -286,7 +286,7 @@ constexpr int kRowBlock = 256;
 constexpr int kLoads = 4;
 constexpr uint32_t kPart = kLoads * 64;
 
-// Where a wave is: a part of a row, and whether the row counts (a masked row's logits are not read).
+// Where a wave is: a part of a row, and whether the row counts (a masked row is not read).
 struct Place {
     uint64_t row;
     uint32_t part;
@@ -333,10 +333,10 @@ struct Part {
 // Wave i: part i % splits of row i / splits, and on by the launch's waves.  With `last_joins`
 // (every wave then has one part) the launch's last block joins the rows' parts, else
 // finish_rows_kernel does; rows of one part are finished at once.
-// Bound by the exponentials and reading the logits, about evenly.  Parts rather than rows per block:
-// the waves in flight then sweep a narrow window of memory.  Measured: 8192 rows of 50257 bf16 (one
-// in ten masked) 131 us, 5.65 TB/s of the logits it reads (on the 16-byte grid 5.9, fp32 6.1); one such row in 7 blocks 6 us, of which
-// three quarters are the launch, the first loads and the join.
+// Bound by the exponentials and the reading, about evenly.  Parts rather than rows per block:
+// the waves in flight then sweep a narrow window of memory.  Measured: 8192 rows of 50257 bf16, one
+// in ten masked, 131 us, 5.65 TB/s of the logits it reads (on the 16-byte grid 5.9, fp32 6.1); one
+// such row in 7 blocks 6 us, of which three quarters are the launch, the first loads and the join.
 template <class T, Loss kLoss>
 __global__ __launch_bounds__(kRowBlock) void row_scores_kernel(RowArgs a, uint32_t splits,
                                                                uint32_t lanes, double* parts,
@@ -557,8 +557,8 @@ __device__ __forceinline__ u32x4 grad16(u32x4 w, const T* type, float f, float m
 
 // Block b: part b % splits of row b / splits (kLanes 64: four rows per block, of at most 128
 // chunks).  Each element is read before it is written by the same lane, so the gradient may take
-// the logits' place.  Bound by HBM: 9733 rows of 50257 bf16, three in ten masked, 300 us, 5.5 TB/s read
-// and written.
+// the logits' place.  Bound by HBM: 9733 rows of 50257 bf16, three in ten masked, 300 us, 5.5 TB/s
+// read and written.
 template <class T, int kLanes>
 __global__ __launch_bounds__(kGradBlock) void row_grads_kernel(GradArgs a, uint32_t splits) {
     constexpr int P = kPer<T>, kRows = kGradBlock / kLanes, kLoads = 2;
@@ -625,7 +625,7 @@ __global__ __launch_bounds__(kGradBlock) void row_grads_kernel(GradArgs a, uint3
 
 // Up to this many rows the launch does everything (`tickets` given): each block counts the rows by
 // itself, and the last one adds up the losses.  (One launch for three: 1021 rows of 50257 fp32 85.8
-// to 78.3 us, a call over few rows 26 to 20 us of the host, 2000 rows of 50257 bf16 94.8 to 93.6 us.
+// to 78.3 us, a call over few rows 26 to 20 us of the host, 2000 rows of 50257 bf16 94.8 to 93.6.
 // Above, every block's count of all rows and one block's sum take longer than launches of their
 // own: 4000 rows 204 us against 187.)
 constexpr uint32_t kAlone = 2048;
