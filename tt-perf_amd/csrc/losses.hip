@@ -873,9 +873,9 @@ int launch_grads(const ttpi::Op& op, const GradArgs& a, int dtype) {
 
 // The one-pass policy kernel's shape for rows of `chunks` chunks: f<lanes, chunks per lane>, or
 // false where no shape holds them.  1024 lanes, two rows or one on a CU (16384 rows of 50257 bf16
-// every 50304, so on the 16-byte grid: 575 us, 618 with 256 lanes; 1021 rows of 50257 fp32: 85.5
-// us, 88 with 512), but where rows lie anywhere and three of them fit a CU's registers, 256 lanes
-// (the same rows every 50257: 733 us, 765 with 1024 lanes).
+// every 50304, so on the 16-byte grid: 565 us, 618 with 256 lanes; 1021 rows of 50257 fp32 78 us, 3
+// us more with 512), but where rows lie anywhere and three of them fit a CU's registers, 256 lanes
+// (the same rows every 50257: 725 us, 769 with 1024 lanes).
 template <class F>
 bool policy_shape(uint32_t chunks, bool on_grid, F&& f) {
 #define TTP_SHAPE(T, C)                                                 \
