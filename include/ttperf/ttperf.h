@@ -516,6 +516,8 @@ int ttp_token_logprobs(ttp_ctx* ctx, const ttp_matrix* logits, const int64_t* ta
  * sequence P + p the one rejected against p.  With d_s the sum over a sequence's unmasked rows
  * of logp - ref_logps (ref_logps null: of logp), and h_p = beta (d_p - d_{P+p}):
  *   loss = mean_p [ -(1 - eps) log sigmoid(h_p) - eps log sigmoid(-h_p) ],   margins[p] = h_p
+ * (eps 0: the first term alone, so a pair whose rejected sequence has probability 0, h = +inf,
+ * adds 0 to the loss and to the gradient)
  * grad (null: none): dloss/dlogits times the context's loss scale while loss scaling is on; of
  * logits' shape and type; zeros on masked rows and on rows in no sequence.  It may be exactly
  * `logits`.  The sums over a sequence are in fp64. */

@@ -221,10 +221,11 @@ struct PairArgs {
     const float* loss_scale;
     float *coef, *margins, *loss;
 };
-// One pair's loss from its margin h, and its c = scale dloss/dmargin beta / pairs.
+// One pair's loss from its margin h, and its c = scale dloss/dmargin beta / pairs.  Without
+// smoothing the second term is left out: at a margin of +inf it would be 0 x inf.
 __device__ __forceinline__ double pair_loss(const PairArgs& a, double h) {
     const double eps = a.smoothing;
-    return (1.0 - eps) * softplus(-h) + eps * softplus(h);
+    return (1.0 - eps) * softplus(-h) + (eps > 0.0 ? eps * softplus(h) : 0.0);
 }
 __device__ __forceinline__ float pair_coef(const PairArgs& a, double h) {
     // (each sigmoid by itself: their difference would lose the small one)
