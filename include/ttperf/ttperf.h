@@ -601,7 +601,8 @@ int ttp_gelu_backward8(ttp_ctx* ctx, const ttp_checkpoint8* kept, int approximat
  * rounded once; the same rule for captured calls; a current gradient sum becomes stale):
  *   weight (+)= xhat^T dy  (cols x outs; transposed: outs x cols),   bias (+)= sum of dy's rows
  * xhat: the values `kept` stands for (rows x cols); dy: rows x outs, of either type whatever the
- * store's.  Products are exact (an fp32 dy goes in as three bf16 parts), sums in fp32.
+ * store's.  Products are exact (an fp32 dy goes in as three bf16 parts; of one below 2^-110 the
+ * bits below 2^-133 are lost), sums in fp32.
  * bias: a tensor index, or TTP_NO_TENSOR. */
 #define TTP_NO_TENSOR 0xFFFFFFFFu
 int ttp_accumulate_linear_grad8(ttp_ctx* ctx, uint32_t weight, uint32_t bias,
