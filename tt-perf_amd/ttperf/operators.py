@@ -89,6 +89,39 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+def _cuts(shape):
+    """Where rows in C order begin a new index of a leading dimension, by their counts: the
+    elements behind each dimension.  A shape that splits or merges another's dimensions has a
+    superset or a subset of its cuts."""
+    n, cuts = 1, set()
+    for d in reversed(shape):
+        cuts.add(n)
+        n *= d
+    return cuts - {1, n}
+
+
+def _check_row_order(logits, *per_row):
+    """Refuses tensors of one element per row (checked to be as many) whose shape is not the
+    others' with some dimensions split or merged (flat: all merged): (T, B) targets of (B, T)
+    rows would be paired in another order."""
+    rows, finest = None, None
+    for t in per_row:
+        if t is None or t.dim() < 2:
+            continue
+        if rows is None:
+            rows = logits.shape[:-1]
+        if t.shape == rows or not t.numel():
+            continue
+        if finest is None:
+            finest = _cuts(rows)
+        cuts = _cuts(t.shape)
+        if cuts >= finest:
+            finest = cuts
+        elif not cuts <= finest:
+            raise ValueError(f"a tensor of shape {tuple(t.shape)} has its rows in another order "
+                             f"than the others (the logits' rows: {tuple(rows)})")
+
+
 class Operators:
     """Mixed into ParamStore.  (What runs on every call asks as little as it can: a call over one
     row takes 10.5 us of host time: 4.1 the library, 2.9 the streams and sources, 1.7 each new
@@ -175,10 +208,12 @@ class Operators:
 
     def token_logprobs(self, logits, targets, *, out=None):
         """Each row's log-probability of its token under softmax(logits): float32, of targets'
-        shape.  logits: (..., V) float32 or bfloat16; targets: int64, a negative one masks its
-        row (0).  A token past the vocabulary gives NaN.  (ttp_token_logprobs)"""
+        shape.  logits: (..., V) float32 or bfloat16; targets: int64, of the logits' rows (or flat,
+        or with dimensions split or merged), a negative one masks its row (0).  A token past the
+        vocabulary gives NaN.  (ttp_token_logprobs)"""
         z = self._rows_of(logits, "the logits")
         y = self._vector_of(targets, z.shape[0], torch.int64, "the targets")
+        _check_row_order(logits, targets)
         result = self._result(out, z, targets.shape, torch.float32, "out")
         self._queue((z, y) if out is None else (z, y, out), L.lib.ttp_token_logprobs,
                     _matrix(z), y.data_ptr(), result.data_ptr())
@@ -208,6 +243,7 @@ class Operators:
         at = self._vector_of(starts, 2 * pairs + 1, torch.int64, "starts")
         ref = None if ref_logps is None else self._vector_of(
             ref_logps, rows, torch.float32, "ref_logps")
+        _check_row_order(logits, targets, ref_logps)
         loss = self._result(out and out.loss, z, (), torch.float32, "the loss")
         margins = self._result(out and out.margins, z, (pairs,), torch.float32, "the margins")
         logps = self._result(out and out.logps, z, targets.shape, torch.float32, "the logps")
@@ -247,6 +283,7 @@ class Operators:
         adv = self._vector_of(advantages, rows, torch.float32, "advantages")
         ref = None if ref_logps is None else self._vector_of(
             ref_logps, rows, torch.float32, "ref_logps")
+        _check_row_order(logits, targets, old_logps, advantages, ref_logps)
         loss = self._result(out and out.loss, z, (), torch.float32, "the loss")
         kl = self._result(out and out.kl, z, (), torch.float32, "kl")
         logps = self._result(out and out.logps, z, targets.shape, torch.float32, "the logps")
