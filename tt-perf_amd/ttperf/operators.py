@@ -6,6 +6,11 @@ work is queued on the store's stream, ordered with torch's current stream as the
 device work is (no synchronisation when both share one stream, see ParamStore.set_stream).
 While the store captures a graph, every result has to be given (an earlier call's, `out=`), and
 the graph reads and writes the tensors in place at every launch.
+
+Autograd does not follow the operators: no result requires a gradient, whatever the inputs do (a
+loss's gradient goes on by logits.backward(r.grad)).  A given result counts as changed in place:
+where torch's backward still needs its old contents (the result of a tanh, an exp or a softmax) it
+refuses.  What a captured graph writes at its launches is not seen, as with torch's own graphs.
 """
 from __future__ import annotations
 
@@ -178,15 +183,19 @@ class Operators:
                              f"{tuple(shape)} on cuda:{self.device}")
         return given
 
-    def _queue(self, tensors, call, *args):
+    def _queue(self, tensors, written, call, *args):
         """Queue the library's `call` behind torch's work on `tensors`: what it reads, and the
-        results that were given (a new one is torch's on its current stream already)."""
+        results that were given (a new one is torch's on its current stream already).  `written`:
+        those results, whose versions it raises as torch's own in-place operations do: a backward
+        that saved one of them refuses rather than use what is there now."""
         if self._in_capture:
             L.check(call(self._h, *args))
-            return
-        kept = self._before_device_sources(tensors)
-        L.check(call(self._h, *args))
-        self._after_device_sources(kept)
+        else:
+            kept = self._before_device_sources(tensors)
+            L.check(call(self._h, *args))
+            self._after_device_sources(kept)
+        if written:
+            torch.autograd.graph.increment_version(written)
 
     def _gradient(self, grad, logits, want):
         """(what the caller gets back, its matrix) of a loss's gradient: `grad` True for a new
@@ -206,6 +215,13 @@ class Operators:
             raise ValueError("the gradient must be a tensor of the logits' shape and type")
         return grad, self._rows_of(grad, "the gradient")
 
+    @staticmethod
+    def _given_results(grad, given, out):
+        """Of a loss's results, those that the caller gave (`given`: the gradient's tensor)."""
+        if out is None:
+            return [] if given is None or grad is True else [given]
+        return [*out[:3]] if given is None else [*out[:3], given]
+
     def token_logprobs(self, logits, targets, *, out=None):
         """Each row's log-probability of its token under softmax(logits): float32, of targets'
         shape.  logits: (..., V) float32 or bfloat16; targets: int64, of the logits' rows (or flat,
@@ -215,8 +231,9 @@ class Operators:
         y = self._vector_of(targets, z.shape[0], torch.int64, "the targets")
         _check_row_order(logits, targets)
         result = self._result(out, z, targets.shape, torch.float32, "out")
-        self._queue((z, y) if out is None else (z, y, out), L.lib.ttp_token_logprobs,
-                    _matrix(z), y.data_ptr(), result.data_ptr())
+        given = () if out is None else (out,)
+        self._queue((z, y) + given, given, L.lib.ttp_token_logprobs, _matrix(z), y.data_ptr(),
+                    result.data_ptr())
         return result
 
     def preference_loss(self, logits, targets, starts, ref_logps=None, *, beta=0.1,
@@ -254,11 +271,8 @@ class Operators:
             None if gm is None else C.addressof(gm), logps.data_ptr(), margins.data_ptr(),
             loss.data_ptr())
         used = [t for t in (z, y, at, ref) if t is not None]
-        if given is not None and grad is not True:
-            used.append(g)
-        if out is not None:
-            used += [t for t in out if t is not None]
-        self._queue(used, L.lib.ttp_preference_loss, args)
+        written = self._given_results(grad, given, out)
+        self._queue(used + written, written, L.lib.ttp_preference_loss, args)
         return PreferenceLoss(loss, margins, logps, given)
 
     def policy_loss(self, logits, targets, old_logps, advantages, ref_logps=None, *, clip=0.2,
@@ -294,11 +308,8 @@ class Operators:
             kl_coef, denominator or 0.0, None if gm is None else C.addressof(gm),
             logps.data_ptr(), loss.data_ptr(), kl.data_ptr())
         used = [t for t in (z, y, old, adv, ref) if t is not None]
-        if given is not None and grad is not True:
-            used.append(g)
-        if out is not None:
-            used += [t for t in out if t is not None]
-        self._queue(used, L.lib.ttp_policy_loss, args)
+        written = self._given_results(grad, given, out)
+        self._queue(used + written, written, L.lib.ttp_policy_loss, args)
         return PolicyLoss(loss, kl, logps, given)
 
     # ---- activations kept in 8 bits ------------------------------------------------------------
@@ -329,8 +340,8 @@ class Operators:
         NaN.  out: a Checkpoint8 to write again.  (ttp_checkpoint8_pack)"""
         m = self._rows_of(x, "the activation")
         kept = self._kept_of(m, fmt, out, x.shape)
-        self._queue((m,) if out is None else (m, out.values, out.scales),
-                    L.lib.ttp_checkpoint8_pack, _matrix(m), kept._c())
+        given = () if out is None else (out.values, out.scales)
+        self._queue((m,) + given, given, L.lib.ttp_checkpoint8_pack, _matrix(m), kept._c())
         return kept
 
     def restore8(self, kept, *, dtype=None, out=None):
@@ -342,8 +353,8 @@ class Operators:
             raise ValueError("dtype must be torch.float32 or torch.bfloat16")
         result = self._result(out, kept.values, kept.shape, dtype, "out")
         m = self._rows_of(result, "out")
-        used = (kept.values, kept.scales)
-        self._queue(used if out is None else used + (out,), L.lib.ttp_checkpoint8_restore,
+        given = () if out is None else (out,)
+        self._queue((kept.values, kept.scales) + given, given, L.lib.ttp_checkpoint8_restore,
                     kept._c(), _matrix(m))
         return result
 
@@ -353,17 +364,18 @@ class Operators:
         Checkpoint8 to write again.  (ttp_gelu_checkpoint8)"""
         approx = _choice(_APPROXIMATE, approximate, "approximate")
         m = self._rows_of(x, "the input")
-        used = [m]
+        given = []
         if kept is not None:
             self._check_kept(kept)
-            used += [kept.values, kept.scales]
+            given += [kept.values, kept.scales]
         if out is None:
             out = self._result(None, x, x.shape, x.dtype, "out")
         else:
-            used.append(out)
+            given.append(out)
         y = self._like(out, x, "out")
         kept = self._kept_of(m, fmt, kept, x.shape)
-        self._queue(used, L.lib.ttp_gelu_checkpoint8, _matrix(m), approx, _matrix(y), kept._c())
+        self._queue([m] + given, given, L.lib.ttp_gelu_checkpoint8, _matrix(m), approx, _matrix(y),
+                    kept._c())
         return out, kept
 
     def gelu_backward8(self, kept, dy, *, approximate="none", out=None):
@@ -374,13 +386,12 @@ class Operators:
         g = self._rows_of(dy, "dy")
         if tuple(dy.shape) != kept.shape:
             raise ValueError(f"dy has shape {tuple(dy.shape)}, the checkpoint {kept.shape}")
-        used = [kept.values, kept.scales, g]
+        given = () if out is None else (out,)
         if out is None:
             out = self._result(None, dy, dy.shape, dy.dtype, "out")
-        else:
-            used.append(out)
         d = self._like(out, dy, "out")
-        self._queue(used, L.lib.ttp_gelu_backward8, kept._c(), approx, _matrix(g), _matrix(d))
+        self._queue((kept.values, kept.scales, g) + given, given, L.lib.ttp_gelu_backward8,
+                    kept._c(), approx, _matrix(g), _matrix(d))
         return out
 
     def accumulate_linear_grad8(self, index, kept, dy, *, bias=None, transposed=False):
@@ -394,7 +405,7 @@ class Operators:
         g = self._rows_of(dy, "dy")
         if tuple(dy.shape[:-1]) != kept.shape[:-1]:
             raise ValueError(f"dy has shape {tuple(dy.shape)}, the checkpoint {kept.shape}")
-        self._queue((kept.values, kept.scales, g), L.lib.ttp_accumulate_linear_grad8, index,
+        self._queue((kept.values, kept.scales, g), (), L.lib.ttp_accumulate_linear_grad8, index,
                     L.NO_TENSOR if bias is None else bias, kept._c(), _matrix(g),
                     1 if transposed else 0)
 
