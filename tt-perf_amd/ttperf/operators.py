@@ -405,9 +405,15 @@ class Operators:
         g = self._rows_of(dy, "dy")
         if tuple(dy.shape[:-1]) != kept.shape[:-1]:
             raise ValueError(f"dy has shape {tuple(dy.shape)}, the checkpoint {kept.shape}")
+        if bias is None:
+            bias = L.NO_TENSOR
+        # (here: the library has 32 bits of an index, and -1 would be no bias)
+        for i in (index,) if bias == L.NO_TENSOR else (index, bias):
+            if not 0 <= i < len(self.tensors):
+                raise ValueError(f"tensor index {i} out of range (the store has "
+                                 f"{len(self.tensors)} tensors)")
         self._queue((kept.values, kept.scales, g), (), L.lib.ttp_accumulate_linear_grad8, index,
-                    L.NO_TENSOR if bias is None else bias, kept._c(), _matrix(g),
-                    1 if transposed else 0)
+                    bias, kept._c(), _matrix(g), 1 if transposed else 0)
 
     def _like(self, out, x, what):
         """The matrix of a result that has x's shape and type."""
