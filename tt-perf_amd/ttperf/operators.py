@@ -53,6 +53,7 @@ class Checkpoint8:
     __slots__ = ("values", "scales", "shape", "dtype", "format", "rows", "cols")
 
     def __init__(self, values, scales, shape, dtype, fmt):
+        _choice(_FORMATS, fmt, "fmt")
         self._set(values, scales, shape, dtype, fmt)
         blocks = -(-self.cols // L.CHECKPOINT_BLOCK)
         for t, width in ((values, blocks * L.CHECKPOINT_BLOCK), (scales, blocks)):
