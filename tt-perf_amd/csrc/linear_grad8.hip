@@ -36,12 +36,12 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) s16x4* lds_s16x4;
 
-// kA x kB of the gradient per block, kN rows per step; kWA x kWB waves over the tile, and kWN over
-// the rows of a step: each of the kWN sums its share, and they are added up at the end.
-template <int A, int B, int N, int WA, int WB, int WN, int D>
+// kA x kB of the gradient per block, kN rows per step, kWA x kWB waves over the tile, kDepth steps'
+// loads from memory in flight.
+template <int A, int B, int N, int WA, int WB, int D>
 struct Tile {
-    static constexpr int kA = A, kB = B, kN = N, kWA = WA, kWB = WB, kWN = WN, kDepth = D;
-    static constexpr int kThreads = 64 * WA * WB * WN;
+    static constexpr int kA = A, kB = B, kN = N, kWA = WA, kWB = WB, kDepth = D;
+    static constexpr int kThreads = 64 * WA * WB;
     static constexpr int kFA = A / WA / 32, kFB = B / WB / 32;  // 32 x 32 fragments of a wave
     // LDS rows are 64 bytes longer than the tile: the four rows that a transposing load takes at
     // once lie in different banks
@@ -242,14 +242,11 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads == 512 ? 1 : 2) void linea
     constexpr int kChunksA = T::kN * T::kA / 16 / T::kThreads;  // per lane and step
     constexpr int kChunksB = T::kN * T::kB / 8 / T::kThreads;
     static_assert(kChunksA >= 1 && kChunksB >= 1 && T::kThreads % (T::kB / 8) == 0 &&
-                  T::kThreads % (T::kA / 16) == 0 && T::kN % (16 * T::kWN) == 0);
+                  T::kThreads % (T::kA / 16) == 0);
     constexpr int kRowsA = T::kThreads / (T::kA / 16), kRowsB = T::kThreads / (T::kB / 8);
-    constexpr int kPairs = T::kWA * T::kWB;  // waves over the tile
     constexpr int kOutPitch = 36;  // floats; a wave's 32 x 32 of the gradient on its way out
-    constexpr int kOut = kPairs * 32 * kOutPitch * 2;
-    constexpr int kAdd = T::kWN > 1 ? kPairs * T::kFB * 64 * 16 * 2 : 0;  // see below
-    constexpr int kMost = 2 * kBuffer > kOut ? 2 * kBuffer : kOut;
-    __shared__ __align__(16) short lds[kMost > kAdd ? kMost : kAdd];
+    constexpr int kOut = T::kThreads / 64 * 32 * kOutPitch * 2;
+    __shared__ __align__(16) short lds[2 * kBuffer > kOut ? 2 * kBuffer : kOut];
 
     const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
     const uint32_t part = id / (a.tiles_a * a.tiles_b), tile = id % (a.tiles_a * a.tiles_b);
@@ -260,8 +257,7 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads == 512 ? 1 : 2) void linea
 
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int pair = wave % kPairs, share = wave / kPairs;
-    const int wa = pair / T::kWB * (T::kA / T::kWA), wb = pair % T::kWB * (T::kB / T::kWB);
+    const int wa = wave / T::kWB * (T::kA / T::kWA), wb = wave % T::kWB * (T::kB / T::kWB);
 
     // this lane's chunks: columns ca of xhat (of the tile), rows ta + k kRowsA; and of dy
     const uint32_t ca = t % (T::kA / 16) * 16, ta = t / (T::kA / 16);
@@ -373,12 +369,12 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads == 512 ? 1 : 2) void linea
     // A step is two rounds of 16 rows, whose operands are in registers before the step begins: step
     // s + 1 goes to the other LDS buffer behind round 0's instructions, its rounds' operands come
     // back behind round 1's, and step s + 2's loads from memory are in flight meanwhile.
-    static_assert(T::kN / T::kWN == 32);
+    static_assert(T::kN == 32);
     struct Round {
         bf16x8 a[T::kFA], b[kPlanes][T::kFB];
     } round[2];
     const auto fetch = [&](const short* buffer, int r) {
-        const int n = share * 32 + r * 16;
+        const int n = r * 16;
 #pragma unroll
         for (int i = 0; i < T::kFA; ++i)
             round[r].a[i] = fragment(buffer, T::kPitchA, n, wa + 32 * i);
@@ -457,90 +453,56 @@ __global__ __launch_bounds__(T::kThreads, T::kThreads == 512 ? 1 : 2) void linea
     }
     __syncthreads();
 
-    if constexpr (T::kWN > 1) {
-        // the shares' sums, one row of fragments at a time: the others' go through LDS, in order
-        f32x4* parts = reinterpret_cast<f32x4*>(lds) + pair * T::kFB * 64 * 4;
-#pragma unroll
-        for (int i = 0; i < T::kFA; ++i)
-#pragma unroll
-            for (int h = 1; h < T::kWN; ++h) {
-                if (share == h) {
-#pragma unroll
-                    for (int j = 0; j < T::kFB; ++j)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            parts[(j * 4 + k) * 64 + lane] =
-                                f32x4{acc[i][j][4 * k], acc[i][j][4 * k + 1],
-                                      acc[i][j][4 * k + 2], acc[i][j][4 * k + 3]};
-                }
-                __syncthreads();
-                if (share == 0) {
-#pragma unroll
-                    for (int j = 0; j < T::kFB; ++j)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const f32x4 v = parts[(j * 4 + k) * 64 + lane];
-#pragma unroll
-                            for (int m = 0; m < 4; ++m) acc[i][j][4 * k + m] += v[m];
-                        }
-                }
-                __syncthreads();
-            }
-    }
-
     // out, 32 x 32 at a time through this wave's LDS: the gradient's rows are columns of xhat,
     // or of dy where the weight is transposed
-    if (share == 0) {
-        float* out = reinterpret_cast<float*>(lds) + pair * 32 * kOutPitch;
-        const uint32_t rows_out = a.transposed ? a.outs : a.cols;
-        const uint32_t cols_out = a.transposed ? a.cols : a.outs;
+    float* out = reinterpret_cast<float*>(lds) + wave * 32 * kOutPitch;
+    const uint32_t rows_out = a.transposed ? a.outs : a.cols;
+    const uint32_t cols_out = a.transposed ? a.cols : a.outs;
 #pragma unroll
-        for (int i = 0; i < T::kFA; ++i)
+    for (int i = 0; i < T::kFA; ++i)
 #pragma unroll
-            for (int j = 0; j < T::kFB; ++j) {
-                // lane: column lane % 32 of dy, rows 8 (k / 4) + 4 (lane / 32) + k % 4 of xhat
+        for (int j = 0; j < T::kFB; ++j) {
+            // lane: column lane % 32 of dy, rows 8 (k / 4) + 4 (lane / 32) + k % 4 of xhat
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                    const int x = 8 * (k / 4) + 4 * (lane >> 5) + k % 4, y = lane & 31;
-                    out[(a.transposed ? y : x) * kOutPitch + (a.transposed ? x : y)] =
-                        acc[i][j][k];
-                }
-                __builtin_amdgcn_wave_barrier();
-                const uint32_t xa = a0 + wa + 32 * i, yb = b0 + wb + 32 * j;
-                const uint32_t r = (a.transposed ? yb : xa) + lane / 2;
-                const uint32_t c = (a.transposed ? xa : yb) + lane % 2 * 16;
-                float v[16];
+            for (int k = 0; k < 16; ++k) {
+                const int x = 8 * (k / 4) + 4 * (lane >> 5) + k % 4, y = lane & 31;
+                out[(a.transposed ? y : x) * kOutPitch + (a.transposed ? x : y)] = acc[i][j][k];
+            }
+            __builtin_amdgcn_wave_barrier();
+            const uint32_t xa = a0 + wa + 32 * i, yb = b0 + wb + 32 * j;
+            const uint32_t r = (a.transposed ? yb : xa) + lane / 2;
+            const uint32_t c = (a.transposed ? xa : yb) + lane % 2 * 16;
+            float v[16];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const f32x4 q = *reinterpret_cast<const f32x4*>(out + lane / 2 * kOutPitch +
-                                                                    lane % 2 * 16 + 4 * k);
+            for (int k = 0; k < 4; ++k) {
+                const f32x4 q = *reinterpret_cast<const f32x4*>(out + lane / 2 * kOutPitch +
+                                                                lane % 2 * 16 + 4 * k);
 #pragma unroll
-                    for (int m = 0; m < 4; ++m) v[4 * k + m] = q[m];
-                }
-                __builtin_amdgcn_wave_barrier();
-                if (r < rows_out && c < cols_out) {
-                    const uint64_t at = (uint64_t)r * cols_out + c;
-                    const uint32_t n = min(16u, cols_out - c);
-                    if (a.parts == 1) {
-                        put(a, at, n, v);
-                    } else {
-                        float* p = a.dw_parts + (uint64_t)part * rows_out * cols_out + at;
-                        if (n == 16) {
+                for (int m = 0; m < 4; ++m) v[4 * k + m] = q[m];
+            }
+            __builtin_amdgcn_wave_barrier();
+            if (r < rows_out && c < cols_out) {
+                const uint64_t at = (uint64_t)r * cols_out + c;
+                const uint32_t n = min(16u, cols_out - c);
+                if (a.parts == 1) {
+                    put(a, at, n, v);
+                } else {
+                    float* p = a.dw_parts + (uint64_t)part * rows_out * cols_out + at;
+                    if (n == 16) {
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const float w[4] = {v[4 * k], v[4 * k + 1], v[4 * k + 2],
-                                                    v[4 * k + 3]};
-                                store16(p + 4 * k, pack(w, p));
-                            }
-                        } else {
-#pragma unroll
-                            for (int k = 0; k < 16; ++k)
-                                if (k < (int)n) p[k] = v[k];
+                        for (int k = 0; k < 4; ++k) {
+                            const float w[4] = {v[4 * k], v[4 * k + 1], v[4 * k + 2],
+                                                v[4 * k + 3]};
+                            store16(p + 4 * k, pack(w, p));
                         }
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 16; ++k)
+                            if (k < (int)n) p[k] = v[k];
                     }
                 }
             }
-    }
+        }
     if (!bias) return;
     __syncthreads();
     // the lanes that share columns, in order
@@ -607,9 +569,9 @@ __global__ __launch_bounds__(kJoinBlock) void join_parts_kernel(LinearArgs a) {
 }
 
 // ---- launches -----------------------------------------------------------------------------------
-using Wide = Tile<256, 256, 32, 2, 4, 1, 2>;    // one block per CU
-using Narrow = Tile<128, 128, 32, 2, 2, 1, 1>;  // two
-using Planes = Narrow;                          // an fp32 dy: three products each
+using Wide = Tile<256, 256, 32, 2, 4, 2>;    // one block per CU
+using Narrow = Tile<128, 128, 32, 2, 2, 1>;  // two
+using Planes = Narrow;                       // an fp32 dy: three products each
 
 // What a tile costs, measured: ns per row of a block that has its CU to itself, and of two that
 // share one; and ns before its first and behind its last step.  The wide tile moves half the bytes
