@@ -25,6 +25,7 @@
 
 #include "checkpoint8.hpp"
 #include "context.hpp"
+#include "linear_tiles.hpp"
 #include "matrix.hpp"
 #include "vector16.hpp"
 
@@ -569,20 +570,9 @@ __global__ __launch_bounds__(kJoinBlock) void join_parts_kernel(LinearArgs a) {
 }
 
 // ---- launches -----------------------------------------------------------------------------------
-using Wide = Tile<256, 256, 32, 2, 4, 2>;    // one block per CU
-using Narrow = Tile<128, 128, 32, 2, 2, 1>;  // two
-using Planes = Narrow;                       // an fp32 dy: three products each
-
-// What a tile costs, measured: ns per row of a block that has its CU to itself, and of two that
-// share one; and ns before its first and behind its last step.  The wide tile moves half the bytes
-// per operation, the narrow one wastes less of a small gradient and needs fewer parts.
-// (8192 x 1280 x 5120 bf16: 150 us with wide tiles, 200 with narrow ones; 4096 x 384 x 1536: 35 and
-// 27.)
-struct Cost {
-    double one, two, ends;
-};
-constexpr Cost kWideCost{30.0, 60.0, 8000.0}, kNarrowCost{15.0, 22.0, 4000.0},
-    kPlanesCost{30.0, 56.0, 4000.0};
+using Wide = Tile<kWideTile, kWideTile, kStepRows, 2, 4, 2>;        // one block per CU
+using Narrow = Tile<kNarrowTile, kNarrowTile, kStepRows, 2, 2, 1>;  // two
+using Planes = Narrow;  // an fp32 dy: three products each
 
 template <class G, int kFormat, class T>
 int launch_tiles(const ttpi::Op& op, const LinearArgs& a) {
@@ -594,33 +584,6 @@ int launch_tiles(const ttpi::Op& op, const LinearArgs& a) {
                        dim3(T::kThreads), 0, op.stream, a);
     TTPI_HIP(hipGetLastError());
     return TTP_OK;
-}
-
-// Cuts the work into tiles and the rows into parts of 128 or more: the number of parts that should
-// take the least time, which is returned (ns).  Parts cost their fp32 tiles' way to memory and
-// back, about 5 TB/s, a launch, and the join's loads one after the other.
-template <class T>
-double set_tiles(LinearArgs& a, uint64_t cus, const Cost& c) {
-    a.tiles_a = (a.cols + T::kA - 1) / T::kA;
-    a.tiles_b = (a.outs + T::kB - 1) / T::kB;
-    const uint64_t tiles = (uint64_t)a.tiles_a * a.tiles_b;
-    const uint64_t most = std::max<uint64_t>(std::min<uint64_t>(a.rows / 128, 64), 1);
-    double best = 0.0;
-    for (uint64_t n = 1; n <= most; ++n) {
-        const uint64_t per = ((a.rows + n - 1) / n + T::kN - 1) / T::kN * T::kN;
-        const uint64_t parts = per ? std::max<uint64_t>((a.rows + per - 1) / per, 1) : 1;
-        const uint64_t blocks = tiles * parts, left = blocks % (2 * cus);
-        double ns = (double)(blocks / (2 * cus)) * (c.two * (double)per + c.ends);
-        if (left) ns += (left > cus ? c.two : c.one) * (double)per + c.ends;
-        if (parts > 1)
-            ns += 3000.0 + 150.0 * (double)parts + 8.0 * (double)parts * a.cols * a.outs / 5e3;
-        if (n == 1 || ns < best) {
-            best = ns;
-            a.per = per;
-            a.parts = (uint32_t)parts;
-        }
-    }
-    return best;
 }
 
 }  // namespace
@@ -682,15 +645,11 @@ extern "C" int ttp_accumulate_linear_grad8(ttp_ctx* ctx, uint32_t weight, uint32
         a.db_first = b.first;
         const bool bf16 = dy->dtype == TTP_DTYPE_BF16;
         const uint64_t cus = (uint64_t)op.num_cus;
-        bool wide = false;
-        if (bf16) {
-            LinearArgs b = a;
-            const double narrow_ns = set_tiles<Narrow>(a, cus, kNarrowCost);
-            wide = set_tiles<Wide>(b, cus, kWideCost) < narrow_ns;
-            if (wide) a = b;
-        } else {
-            set_tiles<Planes>(a, cus, kPlanesCost);
-        }
+        const Cut cut = choose_cut(rows, a.cols, a.outs, bf16, cus);
+        a.tiles_a = cut.tiles_a;
+        a.tiles_b = cut.tiles_b;
+        a.parts = cut.parts;
+        a.per = cut.per;
         if (a.parts > 1) {
             void* ws;
             const uint64_t n = (uint64_t)a.parts * cols * outs;
@@ -699,7 +658,7 @@ extern "C" int ttp_accumulate_linear_grad8(ttp_ctx* ctx, uint32_t weight, uint32
             a.db_parts = a.dw_parts + n;
         }
         const bool int8 = kept->format == TTP_CHECKPOINT_INT8;
-        if (bf16 && wide)
+        if (bf16 && cut.wide)
             rc = int8 ? launch_tiles<uint16_t, TTP_CHECKPOINT_INT8, Wide>(op, a)
                       : launch_tiles<uint16_t, TTP_CHECKPOINT_E4M3, Wide>(op, a);
         else if (bf16)
