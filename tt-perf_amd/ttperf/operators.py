@@ -110,16 +110,11 @@ def _check_row_order(logits, *per_row):
     """Refuses tensors of one element per row (checked to be as many) whose shape is not the
     others' with some dimensions split or merged (flat: all merged): (T, B) targets of (B, T)
     rows would be paired in another order."""
-    rows, finest = None, None
+    rows = logits.shape[:-1]
+    finest = _cuts(rows)
     for t in per_row:
-        if t is None or t.dim() < 2:
+        if t is None or t.shape == rows or not t.numel():
             continue
-        if rows is None:
-            rows = logits.shape[:-1]
-        if t.shape == rows or not t.numel():
-            continue
-        if finest is None:
-            finest = _cuts(rows)
         cuts = _cuts(t.shape)
         if cuts >= finest:
             finest = cuts
@@ -230,7 +225,8 @@ class Operators:
         vocabulary gives NaN.  (ttp_token_logprobs)"""
         z = self._rows_of(logits, "the logits")
         y = self._vector_of(targets, z.shape[0], torch.int64, "the targets")
-        _check_row_order(logits, targets)
+        if targets.dim() > 1:
+            _check_row_order(logits, targets)
         result = self._result(out, z, targets.shape, torch.float32, "out")
         given = () if out is None else (out,)
         self._queue((z, y) + given, given, L.lib.ttp_token_logprobs, _matrix(z), y.data_ptr(),
@@ -261,7 +257,8 @@ class Operators:
         at = self._vector_of(starts, 2 * pairs + 1, torch.int64, "starts")
         ref = None if ref_logps is None else self._vector_of(
             ref_logps, rows, torch.float32, "ref_logps")
-        _check_row_order(logits, targets, ref_logps)
+        if targets.dim() > 1 or (ref is not None and ref_logps.dim() > 1):
+            _check_row_order(logits, targets, ref_logps)
         loss = self._result(out and out.loss, z, (), torch.float32, "the loss")
         margins = self._result(out and out.margins, z, (pairs,), torch.float32, "the margins")
         logps = self._result(out and out.logps, z, targets.shape, torch.float32, "the logps")
@@ -272,8 +269,8 @@ class Operators:
             None if gm is None else C.addressof(gm), logps.data_ptr(), margins.data_ptr(),
             loss.data_ptr())
         used = [t for t in (z, y, at, ref) if t is not None]
-        written = self._given_results(grad, given, out)
-        self._queue(used + written, written, L.lib.ttp_preference_loss, args)
+        written = () if out is None and grad is True else self._given_results(grad, given, out)
+        self._queue([*used, *written], written, L.lib.ttp_preference_loss, args)
         return PreferenceLoss(loss, margins, logps, given)
 
     def policy_loss(self, logits, targets, old_logps, advantages, ref_logps=None, *, clip=0.2,
@@ -298,7 +295,9 @@ class Operators:
         adv = self._vector_of(advantages, rows, torch.float32, "advantages")
         ref = None if ref_logps is None else self._vector_of(
             ref_logps, rows, torch.float32, "ref_logps")
-        _check_row_order(logits, targets, old_logps, advantages, ref_logps)
+        if targets.dim() > 1 or old_logps.dim() > 1 or advantages.dim() > 1 or \
+                (ref is not None and ref_logps.dim() > 1):
+            _check_row_order(logits, targets, old_logps, advantages, ref_logps)
         loss = self._result(out and out.loss, z, (), torch.float32, "the loss")
         kl = self._result(out and out.kl, z, (), torch.float32, "kl")
         logps = self._result(out and out.logps, z, targets.shape, torch.float32, "the logps")
@@ -309,8 +308,8 @@ class Operators:
             kl_coef, denominator or 0.0, None if gm is None else C.addressof(gm),
             logps.data_ptr(), loss.data_ptr(), kl.data_ptr())
         used = [t for t in (z, y, old, adv, ref) if t is not None]
-        written = self._given_results(grad, given, out)
-        self._queue(used + written, written, L.lib.ttp_policy_loss, args)
+        written = () if out is None and grad is True else self._given_results(grad, given, out)
+        self._queue([*used, *written], written, L.lib.ttp_policy_loss, args)
         return PolicyLoss(loss, kl, logps, given)
 
     # ---- activations kept in 8 bits ------------------------------------------------------------
