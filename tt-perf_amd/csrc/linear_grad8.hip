@@ -14,11 +14,12 @@
 // in flight while the matrix instructions run.  Few tiles split the rows: each part writes its
 // fp32 tile to scratch memory and join_parts_kernel adds them up in order.
 //
-// Measured, bf16 8192 x 1280 x 5120 (256 x 256 tiles, two parts: 200 blocks for 256 CUs) 115 to
-// 130 us by the card's clock, 825 to 930 TFLOP/s, and the join 11; on a CU with a block the matrix
+// Measured, bf16 8192 x 1280 x 5120 (256 x 256 tiles, two parts: 200 blocks for 256 CUs) 116 to
+// 131 us by the card's clock, 820 to 925 TFLOP/s, and the join 11; on a CU with a block the matrix
 // pipe is busy half of the time, the LDS 0.4; the rest are waits at the steps' barriers.
-// fp32 3585 x 384 x 1536 (128 x 128 tiles, seven parts of 512 rows): 25 us, three products each; the
-// matrix pipe is busy a quarter of the time, 16 steps are too few to hide the first and the last.
+// fp32 3585 x 384 x 1536 (128 x 128 tiles, seven parts of 512 rows): 28 us, three products each;
+// the matrix pipe is busy a quarter of the time, 16 steps are too few to hide the first and the
+// last.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -3,7 +3,9 @@ kept in 8 bits and the gradients made from them.
 
 They take and give torch tensors on the store's device.  Results are new tensors unless given;
 work is queued on the store's stream, ordered with torch's current stream as the store's other
-device work is (no synchronisation when both share one stream, see ParamStore.set_stream).
+device work is.  Where both share one stream (ParamStore.set_stream) nothing waits; a store on a
+stream of its own, the default, waits for torch's stream before a call's work and for that work
+after it.
 While the store captures a graph, every result has to be given (an earlier call's, `out=`), and
 the graph reads and writes the tensors in place at every launch.
 
