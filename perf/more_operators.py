@@ -204,7 +204,7 @@ def _run_own(s):
         store.zero_grad(set_to_none=True, fill=False)
         for tokens, dy in zip(s["tokens"], s["dy"]):
             store.accumulate_embedding_grad(0, tokens, dy, scale=_scale(c))
-        return _gradients(s, 1)[0]
+        return _gradients(s, 1)[0].reshape(-1)
     if op == "layer_norm":
         store.zero_grad(set_to_none=True, fill=False)
         r = store.layer_norm(0, s["x"], bias=1, eps=EPS)
