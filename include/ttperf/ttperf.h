@@ -609,6 +609,86 @@ int ttp_accumulate_linear_grad8(ttp_ctx* ctx, uint32_t weight, uint32_t bias,
                                 const ttp_checkpoint8* kept, const ttp_matrix* dy,
                                 int transposed);
 
+/* ---- a block's operators --------------------------------------------------------------------
+ * What a transformer block has around its attention: embeddings, layer norm, dropout and linear
+ * products, on the store's own weights (its parameter buffer: bf16, or fp32 in an FP32 store),
+ * which a call names by tensor index, and with gradients into the store.  The rules of the
+ * fine-tuning operators hold here too: queued on the context's stream, checked device memory,
+ * no overlap but for results in an input's place, scratch memory, 32-bit sums rounded once, the
+ * same bits for the same inputs. */
+
+/* Dropout without a stored mask: whether an element is kept follows from its place and these
+ * numbers alone, so a backward pass that gives the same ones drops the same elements (and the
+ * gradient's dropout is this same operation).  Columns c of row r belong to the group
+ * g = r * ceil(cols / 8) + c / 8; Philox 4x32 of ten rounds (Salmon, Moraes, Dror and Shaw,
+ * "Parallel random numbers: as easy as 1, 2, 3", 2011) with the key `seed` and the counter
+ * (g, stream), low words first, gives the group four words, whose eight 16-bit halves, the low one
+ * of a word first, are its elements'.  With T = p 2^16 rounded to a whole number (at most 65535),
+ * an element whose half is below T is dropped (0, whatever it was), others are multiplied by
+ * 2^16 / (2^16 - T). */
+typedef struct ttp_dropout {
+    double p;                    /* in [0, 1) */
+    uint64_t seed;
+    uint64_t stream;             /* which of a program's dropouts */
+    const uint64_t* device_seed; /* null, or where the device holds the seed (`seed` is not used):
+                                    a graph's launches then read it anew */
+} ttp_dropout;
+/* y = dropout(x), or residual + dropout(x) (a dropped element: the residual as it is).  All of one
+ * type and shape; y may be exactly x or exactly the residual. */
+int ttp_dropout_forward(ttp_ctx* ctx, const ttp_dropout* dropout, const ttp_matrix* x,
+                        const ttp_matrix* residual, const ttp_matrix* y);
+
+/* y[t] = scale table[tokens[t]] (+ positions' rows of a second table).  table: a tensor index, a
+ * matrix of y->cols columns; tokens: y->rows int64.  A negative token stands for zeros, one past
+ * the table gives NaN; the same holds for a position.  position_table TTP_NO_TENSOR (positions
+ * null): none.  y of either type. */
+int ttp_embedding(ttp_ctx* ctx, uint32_t table, const int64_t* tokens, double scale,
+                  uint32_t position_table, const int64_t* positions, const ttp_matrix* y);
+/* The table's gradient: row v (+)= scale times the sum of dy's rows whose token is v, in the order
+ * of the rows, into the store's gradient as ttp_accumulate_grad puts it (no gradient yet: the
+ * other rows become 0; else they are left as they are).  Tokens outside the table are passed
+ * over.  dy of either type. */
+int ttp_accumulate_embedding_grad(ttp_ctx* ctx, uint32_t table, const int64_t* tokens, double scale,
+                                  const ttp_matrix* dy);
+
+/* Layer norm over each row: m the mean, r = 1 / sqrt(mean((x - m)^2) + eps),
+ *   y = (x - m) r weight + bias     (weight, bias: tensor indices or TTP_NO_TENSOR: 1 and 0)
+ * mean and rstd (rows each): m and r, for the backward.  y of either type; of x's type it may be
+ * exactly x.  At most 2^24 columns; eps 0 or more. */
+int ttp_layer_norm(ttp_ctx* ctx, uint32_t weight, uint32_t bias, const ttp_matrix* x, double eps,
+                   const ttp_matrix* y, float* mean, float* rstd);
+/* With h = (x - m) r and g = dy weight:
+ *   dx = add + r (g - mean(g) - h mean(g h))    weight (+)= sum dy h,   bias (+)= sum dy
+ * over the rows, into the store's gradients as ttp_accumulate_grad puts them.  add (null: none)
+ * and dx have x's type; dy either.  dx may be exactly dy, add or x. */
+int ttp_layer_norm_backward(ttp_ctx* ctx, uint32_t weight, uint32_t bias, const ttp_matrix* x,
+                            const ttp_matrix* dy, const float* mean, const float* rstd,
+                            const ttp_matrix* add, const ttp_matrix* dx);
+
+/* y = residual + dropout(activation(x W + bias)), x: rows x cols, y: rows x outs, in one launch (a
+ * second one joins parts where few rows split the sum).
+ * weight: cols x outs (py/nn.py:36), or transposed outs x cols; x has the store's parameter type,
+ * y either, the residual y's.  The input's gradient of y = x W is this call on dy with
+ * `transposed` the other way round.  Products of bf16 are exact, sums in fp32.  fp32 operands go
+ * in as three bf16 parts each, of whose products the six largest are taken: what is left out is
+ * below 2^-22 of a product (of an operand below 2^-110 the bits below 2^-133 are lost).
+ * y may be exactly the residual. */
+#define TTP_ACTIVATION_NONE 0
+#define TTP_ACTIVATION_RELU 1
+#define TTP_ACTIVATION_GELU_ERF 2
+#define TTP_ACTIVATION_GELU_TANH 3
+typedef struct ttp_linear_args {
+    const ttp_matrix* x;
+    const ttp_matrix* residual;  /* or null */
+    const ttp_matrix* y;         /* out */
+    const ttp_dropout* dropout;  /* or null */
+    uint32_t weight;
+    uint32_t bias;               /* or TTP_NO_TENSOR */
+    int32_t transposed;
+    int32_t activation;          /* TTP_ACTIVATION_* */
+} ttp_linear_args;
+int ttp_linear(ttp_ctx* ctx, const ttp_linear_args* args);
+
 /* ---- per-kernel timing (HIP events on the context's stream) ------------------------------ */
 #define TTP_KERNEL_NORM 0   /* grad-norm / inf-check pass and the step's decisions */
 #define TTP_KERNEL_UPDATE 1 /* fused multi-tensor update pass               */

@@ -337,6 +337,30 @@ public:
         check(ttp_accumulate_linear_grad8(ctx_, weight, bias, &kept, &dy, transposed ? 1 : 0));
     }
 
+    // A block's operators on this store's weights (ttperf.h, "a block's operators").
+    void dropout(const ttp_dropout& d, const ttp_matrix& x, const ttp_matrix& y,
+                 const ttp_matrix* residual = nullptr) {
+        check(ttp_dropout_forward(ctx_, &d, &x, residual, &y));
+    }
+    void embedding(uint32_t table, const int64_t* tokens, const ttp_matrix& y, double scale = 1.0,
+                   uint32_t position_table = TTP_NO_TENSOR, const int64_t* positions = nullptr) {
+        check(ttp_embedding(ctx_, table, tokens, scale, position_table, positions, &y));
+    }
+    void accumulate_embedding_grad(uint32_t table, const int64_t* tokens, const ttp_matrix& dy,
+                                   double scale = 1.0) {
+        check(ttp_accumulate_embedding_grad(ctx_, table, tokens, scale, &dy));
+    }
+    void layer_norm(uint32_t weight, uint32_t bias, const ttp_matrix& x, const ttp_matrix& y,
+                    float* mean, float* rstd, double eps = 1e-5) {
+        check(ttp_layer_norm(ctx_, weight, bias, &x, eps, &y, mean, rstd));
+    }
+    void layer_norm_backward(uint32_t weight, uint32_t bias, const ttp_matrix& x,
+                             const ttp_matrix& dy, const float* mean, const float* rstd,
+                             const ttp_matrix& dx, const ttp_matrix* add = nullptr) {
+        check(ttp_layer_norm_backward(ctx_, weight, bias, &x, &dy, mean, rstd, add, &dx));
+    }
+    void linear(const ttp_linear_args& a) { check(ttp_linear(ctx_, &a)); }
+
     void save_state(const std::string& path) { check(ttp_save_state(ctx_, path.c_str())); }
     void load_state(const std::string& path) { check(ttp_load_state(ctx_, path.c_str())); }
     void begin_capture() {

@@ -1,5 +1,5 @@
-// context.hpp — what the operators' files (losses.hip, checkpoint8.hip, linear_grad8.hip) use of
-// a context, whose state and checks are ttperf.hip's.
+// context.hpp — what the operators' files (losses.hip, checkpoint8.hip, linear.hip and the others)
+// use of a context, whose state and checks are ttperf.hip's.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -55,6 +55,14 @@ struct GradTarget {
 __attribute__((visibility("hidden"))) int grad_target(ttp_ctx* c, uint32_t index, GradTarget* out);
 // The kernel that writes them is queued: the tensor has a gradient, its sum is not current.
 __attribute__((visibility("hidden"))) void grad_written(ttp_ctx* c, uint32_t index);
+
+// Tensor `index`'s parameters, to be read.
+struct Param {
+    const void* data;
+    uint64_t numel;
+    bool bf16;  // or fp32
+};
+__attribute__((visibility("hidden"))) int param(ttp_ctx* c, uint32_t index, Param* out);
 
 // Runs an entry point's body: no exception crosses the C ABI.
 template <class F>

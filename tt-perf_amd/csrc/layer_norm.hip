@@ -1,0 +1,635 @@
+// layer_norm.hip — layer norm and its gradients.
+//
+//   m = mean x,  r = 1 / sqrt(mean (x - m)^2 + eps),  y = (x - m) r w + b
+//   h = (x - m) r,  g = dy w,  dx = add + r (g - mean g - h mean(g h)),  dw = sum dy h,  db = sum dy
+//
+// Bound by memory.  A row of up to 2048 columns is a wave's, one of up to 8192 a block's of four:
+// it is read once, into registers, and its sums are taken there (the variance from the differences,
+// not from the squares, whose difference would lose what a mean far from 0 shares).  Longer rows are
+// read again for each sum.  The backward keeps the weight's and the bias's sums of its rows in
+// registers too: a block has a range of rows, writes one partial sum per column, and
+// join_columns_kernel adds those up in order.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "columns8.hpp"
+#include "context.hpp"
+#include "matrix.hpp"
+#include "vector16.hpp"
+
+namespace ttp {
+namespace {
+
+constexpr uint32_t kWaveCols = 512;  // columns of a wave's step: 8 a lane
+
+// a vector of the store's parameters, or a constant
+struct Vector {
+    const void* data;  // null: every element is `otherwise`
+    bool bf16;
+    float otherwise;
+};
+__device__ __forceinline__ void load_vector(const Vector& p, uint32_t c, uint32_t cols,
+                                            float (&v)[8]) {
+    if (!p.data) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] = p.otherwise;
+    } else if (p.bf16) {
+        load_cols((const uint16_t*)p.data, c, cols, v);
+    } else {
+        load_cols((const float*)p.data, c, cols, v);
+    }
+}
+
+// the wave's sum in every lane, by a butterfly without LDS permutes (see wave_sum)
+__device__ __forceinline__ double wave_total(double x) { return wave_sum(x); }
+__device__ __forceinline__ float wave_total(float x) {
+    {
+        const uint32_t u = __float_as_uint(x);
+        const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        x = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+    {
+        const uint32_t u = __float_as_uint(x);
+        const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        x = __uint_as_float(s[0]) + __uint_as_float(s[1]);
+    }
+    const auto add = [&](uint32_t u) { x += __uint_as_float(u); };
+    add(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0x128, 0xF, 0xF, true));
+    add(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0x124, 0xF, 0xF, true));
+    add(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0x4E, 0xF, 0xF, true));
+    add(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0xB1, 0xF, 0xF, true));
+    return x;
+}
+
+// The sums of N numbers over the kWaves waves of a row, in every lane.
+template <int kWaves, int N, class F>
+__device__ __forceinline__ void row_sums(F (&x)[N], F* lds) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) x[n] = wave_total(x[n]);
+    if constexpr (kWaves > 1) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        __syncthreads();  // the last sums have been read
+        if (lane == 0)
+#pragma unroll
+            for (int n = 0; n < N; ++n) lds[wave * N + n] = x[n];
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            F s = lds[n];
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) s += lds[w * N + n];
+            x[n] = s;
+        }
+    }
+}
+
+struct NormArgs {
+    uint64_t rows;
+    uint32_t cols;
+    double eps;
+    Vector weight, bias;
+    const void *x, *in;  // in: dy of the backward
+    const void* add;
+    void* out;           // y or dx
+    uint64_t x_stride, in_stride, add_stride, out_stride;
+    float *mean, *rstd;
+    float* parts;        // backward: per block the columns' sums of dy h, then those of dy
+};
+
+// ---- rows in registers ------------------------------------------------------------------------
+// kWaves waves have a row of up to kC steps of 512 kWaves columns.
+template <class T, class Y, int kWaves, int kC>
+__global__ __launch_bounds__(256) void norm_kernel(NormArgs a) {
+    __shared__ float lds[4];
+    const uint32_t lane = kWaves == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const uint64_t row =
+        kWaves == 1 ? (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (uint64_t)blockIdx.x;
+    if (row >= a.rows) return;  // (a wave, or the block, together)
+    const T* x = (const T*)a.x + row * a.x_stride;
+    float v[kC][8];
+    float s[1] = {0.0f};
+#pragma unroll
+    for (int k = 0; k < kC; ++k) {
+        load_cols(x, (k * 64 * kWaves + lane) * 8, a.cols, v[k]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[0] += v[k][j];
+    }
+    row_sums<kWaves>(s, lds);
+    const float n = (float)a.cols, m = s[0] / n;
+    s[0] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kC; ++k)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[k][j] = (k * 64 * kWaves + lane) * 8 + j < a.cols ? v[k][j] - m : 0.0f;
+            s[0] += v[k][j] * v[k][j];
+        }
+    row_sums<kWaves>(s, lds);
+    const float r = 1.0f / sqrtf(s[0] / n + (float)a.eps);
+    if (lane == 0) {
+        a.mean[row] = m;
+        a.rstd[row] = r;
+    }
+    Y* y = (Y*)a.out + row * a.out_stride;
+#pragma unroll
+    for (int k = 0; k < kC; ++k) {
+        const uint32_t c = (k * 64 * kWaves + lane) * 8;
+        if (c >= a.cols) break;
+        float w[8], b[8];
+        load_vector(a.weight, c, a.cols, w);
+        load_vector(a.bias, c, a.cols, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = v[k][j] * r * w[j] + b[j];
+        store_cols(y, c, a.cols, w);
+    }
+}
+
+// Rows of this block: a wave each (kWaves 1: eight waves), or the four waves' together.
+template <class T, class G, int kWaves, int kC>
+__global__ __launch_bounds__(kWaves == 1 ? 512 : 256) void norm_backward_kernel(NormArgs a,
+                                                                                uint64_t per) {
+    constexpr uint32_t kRows = kWaves == 1 ? 8 : 1;  // at a time
+    __shared__ float lds[kWaves == 1 ? 2 * kC * kWaveCols : 8];
+    const uint32_t lane = kWaves == 1 ? threadIdx.x & 63 : threadIdx.x;
+    const uint32_t wave = kWaves == 1 ? threadIdx.x >> 6 : 0;
+    const uint64_t first = blockIdx.x * per, end = min(first + per, a.rows);
+    const float n = (float)a.cols;
+    float w[kC][8], sum_w[kC][8], sum_b[kC][8];
+#pragma unroll
+    for (int k = 0; k < kC; ++k) {
+        load_vector(a.weight, (k * 64 * kWaves + lane) * 8, a.cols, w[k]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum_w[k][j] = sum_b[k][j] = 0.0f;
+    }
+    for (uint64_t row = first + wave; row < end; row += kRows) {
+        const T* x = (const T*)a.x + row * a.x_stride;
+        const G* dy = (const G*)a.in + row * a.in_stride;
+        const float m = a.mean[row], r = a.rstd[row];
+        float h[kC][8], g[kC][8], s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < kC; ++k) {
+            const uint32_t c = (k * 64 * kWaves + lane) * 8;
+            load_cols(x, c, a.cols, h[k]);
+            load_cols(dy, c, a.cols, g[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < kC; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {  // (past the row's end dy is 0)
+                const bool in = (k * 64 * kWaves + lane) * 8 + j < a.cols;
+                h[k][j] = in ? (h[k][j] - m) * r : 0.0f;
+                sum_w[k][j] += g[k][j] * h[k][j];
+                sum_b[k][j] += g[k][j];
+                g[k][j] = in ? g[k][j] * w[k][j] : 0.0f;
+                s[0] += g[k][j];
+                s[1] += g[k][j] * h[k][j];
+            }
+        row_sums<kWaves>(s, lds);
+        const float mean_g = s[0] / n, mean_gh = s[1] / n;
+        T* dx = (T*)a.out + row * a.out_stride;
+#pragma unroll
+        for (int k = 0; k < kC; ++k) {
+            const uint32_t c = (k * 64 * kWaves + lane) * 8;
+            if (c >= a.cols) break;
+            float o[8];
+            if (a.add) {
+                load_cols((const T*)a.add + row * a.add_stride, c, a.cols, o);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) o[j] = 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[j] += r * (g[k][j] - mean_g - h[k][j] * mean_gh);
+            store_cols(dx, c, a.cols, o);
+        }
+    }
+    float* part = a.parts + (uint64_t)blockIdx.x * 2 * a.cols;
+    if constexpr (kWaves == 1) {  // the waves' sums, in order
+        float* of_b = lds + kC * kWaveCols;
+        for (uint32_t t = 0; t < kRows; ++t) {
+            if (wave == t)
+#pragma unroll
+                for (int k = 0; k < kC; ++k)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t at = k * kWaveCols + j * 64 + lane;  // a column's place
+                        lds[at] = t ? lds[at] + sum_w[k][j] : sum_w[k][j];
+                        of_b[at] = t ? of_b[at] + sum_b[k][j] : sum_b[k][j];
+                    }
+            __syncthreads();
+        }
+        for (uint32_t c = threadIdx.x; c < a.cols; c += 512) {
+            const uint32_t at = c / kWaveCols * kWaveCols + c % 8 * 64 + c % kWaveCols / 8;
+            part[c] = lds[at];
+            part[a.cols + c] = of_b[at];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < kC; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t c = (k * 64 * kWaves + lane) * 8 + j;
+                if (c < a.cols) {
+                    part[c] = sum_w[k][j];
+                    part[a.cols + c] = sum_b[k][j];
+                }
+            }
+    }
+}
+
+// ---- rows that registers do not hold -----------------------------------------------------------
+// A block per row, which reads it once for each sum and once more; the sums in 64 bits.
+template <class T, class Y>
+__global__ __launch_bounds__(256) void norm_long_kernel(NormArgs a) {
+    __shared__ double lds[8];
+    const uint64_t row = blockIdx.x;
+    const T* x = (const T*)a.x + row * a.x_stride;
+    double s[1] = {0.0};
+    for (uint64_t c = threadIdx.x * 8; c < a.cols; c += 2048) {
+        float v[8];
+        load_cols(x, (uint32_t)c, a.cols, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[0] += v[j];
+    }
+    row_sums<4>(s, lds);
+    const float m = (float)(s[0] / a.cols);
+    s[0] = 0.0;
+    for (uint64_t c = threadIdx.x * 8; c < a.cols; c += 2048) {
+        float v[8];
+        load_cols(x, (uint32_t)c, a.cols, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float d = c + j < a.cols ? v[j] - m : 0.0f;
+            s[0] += (double)d * d;
+        }
+    }
+    row_sums<4>(s, lds);
+    const float r = (float)(1.0 / sqrt(s[0] / a.cols + a.eps));
+    if (threadIdx.x == 0) {
+        a.mean[row] = m;
+        a.rstd[row] = r;
+    }
+    Y* y = (Y*)a.out + row * a.out_stride;
+    for (uint64_t c = threadIdx.x * 8; c < a.cols; c += 2048) {
+        float v[8], w[8], b[8];
+        load_cols(x, (uint32_t)c, a.cols, v);
+        load_vector(a.weight, (uint32_t)c, a.cols, w);
+        load_vector(a.bias, (uint32_t)c, a.cols, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (v[j] - m) * r * w[j] + b[j];
+        store_cols(y, (uint32_t)c, a.cols, v);
+    }
+}
+
+// dx alone, behind the columns' sums: it may be written over what they read.
+template <class T, class G>
+__global__ __launch_bounds__(256) void norm_backward_long_kernel(NormArgs a) {
+    __shared__ double lds[8];
+    const uint64_t row = blockIdx.x;
+    const T* x = (const T*)a.x + row * a.x_stride;
+    const G* dy = (const G*)a.in + row * a.in_stride;
+    const float m = a.mean[row], r = a.rstd[row];
+    double s[2] = {0.0, 0.0};
+    for (uint64_t c = threadIdx.x * 8; c < a.cols; c += 2048) {
+        float h[8], g[8], w[8];
+        load_cols(x, (uint32_t)c, a.cols, h);
+        load_cols(dy, (uint32_t)c, a.cols, g);
+        load_vector(a.weight, (uint32_t)c, a.cols, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float gw = c + j < a.cols ? g[j] * w[j] : 0.0f;
+            s[0] += gw;
+            s[1] += (double)gw * (c + j < a.cols ? (h[j] - m) * r : 0.0f);
+        }
+    }
+    row_sums<4>(s, lds);
+    const float mean_g = (float)(s[0] / a.cols), mean_gh = (float)(s[1] / a.cols);
+    T* dx = (T*)a.out + row * a.out_stride;
+    for (uint64_t c = threadIdx.x * 8; c < a.cols; c += 2048) {
+        float h[8], g[8], w[8], o[8] = {};
+        load_cols(x, (uint32_t)c, a.cols, h);
+        load_cols(dy, (uint32_t)c, a.cols, g);
+        load_vector(a.weight, (uint32_t)c, a.cols, w);
+        if (a.add) load_cols((const T*)a.add + row * a.add_stride, (uint32_t)c, a.cols, o);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            o[j] += r * (g[j] * w[j] - mean_g - (h[j] - m) * r * mean_gh);
+        store_cols(dx, (uint32_t)c, a.cols, o);
+    }
+}
+
+// The columns' sums over a range of rows: 8 columns a lane.
+template <class T, class G>
+__global__ __launch_bounds__(256) void norm_columns_kernel(NormArgs a, uint64_t per) {
+    const uint32_t tiles = (a.cols + 2047) / 2048, part = blockIdx.x / tiles;
+    const uint64_t at = (uint64_t)(blockIdx.x % tiles) * 2048 + threadIdx.x * 8;
+    if (at >= a.cols) return;
+    const uint32_t c = (uint32_t)at;
+    const uint64_t end = min((part + 1) * per, a.rows);
+    float sum_w[8] = {}, sum_b[8] = {};
+    for (uint64_t row = part * per; row < end; ++row) {
+        float h[8], g[8];
+        load_cols((const T*)a.x + row * a.x_stride, c, a.cols, h);
+        load_cols((const G*)a.in + row * a.in_stride, c, a.cols, g);
+        const float m = a.mean[row], r = a.rstd[row];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            sum_w[j] += g[j] * ((h[j] - m) * r);
+            sum_b[j] += g[j];
+        }
+    }
+    float* p = a.parts + (uint64_t)part * 2 * a.cols + c;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (c + j < a.cols) {
+            p[j] = sum_w[j];
+            p[a.cols + j] = sum_b[j];
+        }
+}
+
+// ---- the parts' sums into the gradients -------------------------------------------------------
+struct JoinArgs {
+    const float* parts;
+    uint32_t n, cols;      // parts; columns
+    void *dw, *db;         // null: no such tensor
+    bool bf16, dw_first, db_first;
+};
+__device__ __forceinline__ void put(void* p, bool bf16, bool first, uint32_t c, float v) {
+    if (bf16) {
+        uint16_t* q = (uint16_t*)p + c;
+        narrow(first ? v : widen(*q) + v, q);
+    } else {
+        float* q = (float*)p + c;
+        *q = first ? v : *q + v;
+    }
+}
+// 64 columns of a block (the bias's behind the weight's), whose 16 waves have the parts in turn.
+__global__ __launch_bounds__(1024) void join_columns_kernel(JoinArgs a) {
+    __shared__ float lds[16][64];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint64_t c = (uint64_t)blockIdx.x * 64 + lane, all = 2ull * a.cols;
+    const uint32_t per = (a.n + 15) / 16, end = min((wave + 1) * per, a.n);
+    float v = 0.0f;
+    if (c < all)
+        for (uint32_t k = wave * per; k < end; ++k) v += a.parts[k * all + c];
+    lds[wave][lane] = v;
+    __syncthreads();
+    if (wave || c >= all) return;
+#pragma unroll
+    for (int w = 1; w < 16; ++w) v += lds[w][lane];
+    if (c < a.cols) {
+        if (a.dw) put(a.dw, a.bf16, a.dw_first, (uint32_t)c, v);
+    } else if (a.db) {
+        put(a.db, a.bf16, a.db_first, (uint32_t)(c - a.cols), v);
+    }
+}
+
+// ---- launches ---------------------------------------------------------------------------------
+constexpr uint32_t kLongCols = 8192;  // rows longer than that are not kept in registers
+constexpr uint64_t kMostCols = 1u << 24;
+
+// f(waves of a row, steps): the shape that holds a row of `cols` <= kLongCols
+template <class F>
+void with_shape(uint32_t cols, F&& f) {
+    using std::integral_constant;
+    if (cols <= kWaveCols)
+        f(integral_constant<int, 1>(), integral_constant<int, 1>());
+    else if (cols <= 2 * kWaveCols)
+        f(integral_constant<int, 1>(), integral_constant<int, 2>());
+    else if (cols <= 3 * kWaveCols)
+        f(integral_constant<int, 1>(), integral_constant<int, 3>());
+    else if (cols <= 4 * kWaveCols)
+        f(integral_constant<int, 1>(), integral_constant<int, 4>());
+    else if (cols <= 8 * kWaveCols)
+        f(integral_constant<int, 4>(), integral_constant<int, 2>());
+    else
+        f(integral_constant<int, 4>(), integral_constant<int, 4>());
+}
+
+// A launch has fewer than 2^32 work-items: f(first row, rows) over ranges of rows.
+template <class F>
+int for_row_ranges(uint64_t rows, F&& f) {
+    constexpr uint64_t kMost = (1u << 24) - 4;  // of 256 lanes each
+    for (uint64_t r = 0; r < rows; r += kMost) {
+        (void)hipGetLastError();
+        f(r, std::min(kMost, rows - r));
+        TTPI_HIP(hipGetLastError());
+    }
+    return TTP_OK;
+}
+// The arguments of the rows from r on.
+template <class T, class In, class Out>
+NormArgs from_row(NormArgs a, uint64_t r, uint64_t rows) {
+    a.rows = rows;
+    a.x = (const T*)a.x + r * a.x_stride;
+    if (a.in) a.in = (const In*)a.in + r * a.in_stride;
+    if (a.add) a.add = (const T*)a.add + r * a.add_stride;
+    a.out = (Out*)a.out + r * a.out_stride;
+    a.mean += r;
+    a.rstd += r;
+    return a;
+}
+
+template <class T, class Y>
+int norm_rows(const ttpi::Op& op, const NormArgs& all) {
+    return for_row_ranges(all.rows, [&](uint64_t r, uint64_t rows) {
+        const NormArgs a = from_row<T, T, Y>(all, r, rows);
+        if (a.cols > kLongCols) {
+            hipLaunchKernelGGL((norm_long_kernel<T, Y>), dim3((uint32_t)rows), dim3(256), 0,
+                               op.stream, a);
+            return;
+        }
+        with_shape(a.cols, [&](auto waves, auto steps) {
+            const uint64_t blocks = waves == 1 ? (rows + 3) / 4 : rows;
+            hipLaunchKernelGGL((norm_kernel<T, Y, waves(), steps()>), dim3((uint32_t)blocks),
+                               dim3(256), 0, op.stream, a);
+        });
+    });
+}
+
+// The parts that the columns' sums are taken in, and the rows of each.
+struct Parts {
+    uint32_t n;
+    uint64_t per;
+};
+Parts parts_of(const ttpi::Op& op, uint64_t rows, uint32_t cols) {
+    uint64_t n, step = 1;
+    if (cols > kLongCols) {
+        const uint64_t tiles = ((uint64_t)cols + 2047) / 2048;
+        n = std::max<uint64_t>(4 * (uint64_t)op.num_cus / tiles, 1);
+    } else if (cols > 4 * kWaveCols) {
+        n = 2 * (uint64_t)op.num_cus;
+    } else {
+        n = (uint64_t)op.num_cus;
+        step = 8;  // a row for each of the block's waves
+    }
+    const uint64_t per = std::max<uint64_t>((rows + n - 1) / n, 1);
+    const uint64_t whole = (per + step - 1) / step * step;
+    return {(uint32_t)((rows + whole - 1) / whole), whole};
+}
+
+template <class T, class G>
+int norm_backward_rows(const ttpi::Op& op, const NormArgs& a, const Parts& p) {
+    (void)hipGetLastError();
+    if (a.cols > kLongCols) {
+        const uint32_t tiles = (a.cols + 2047) / 2048;
+        hipLaunchKernelGGL((norm_columns_kernel<T, G>), dim3(p.n * tiles), dim3(256), 0, op.stream,
+                           a, p.per);
+        TTPI_HIP(hipGetLastError());
+        const int rc = for_row_ranges(a.rows, [&](uint64_t r, uint64_t rows) {
+            hipLaunchKernelGGL((norm_backward_long_kernel<T, G>), dim3((uint32_t)rows), dim3(256),
+                               0, op.stream, (from_row<T, G, T>(a, r, rows)));
+        });
+        if (rc) return rc;
+    } else {
+        with_shape(a.cols, [&](auto waves, auto steps) {
+            hipLaunchKernelGGL((norm_backward_kernel<T, G, waves(), steps()>), dim3(p.n),
+                               dim3(waves == 1 ? 512 : 256), 0, op.stream, a, p.per);
+        });
+    }
+    TTPI_HIP(hipGetLastError());
+    return TTP_OK;
+}
+
+int check_cols(uint64_t cols) {
+    if (cols <= kMostCols) return TTP_OK;
+    return ttpi::fail(TTP_ERR_RANGE, "layer norm takes rows of at most 2^24 columns");
+}
+
+// A weight or bias of `cols` elements (or none), to be read.
+int vector_param(ttp_ctx* ctx, ttpi::Buffers& b, uint32_t index, uint64_t cols, float otherwise,
+                 const char* what, Vector* out) {
+    *out = {nullptr, false, otherwise};
+    if (index == TTP_NO_TENSOR) return TTP_OK;
+    ttpi::Param p{};
+    int rc = ttpi::param(ctx, index, &p);
+    if (rc) return rc;
+    if (p.numel != cols)
+        return ttpi::fail(TTP_ERR_RANGE, "tensor " + std::to_string(index) + " has " +
+                                             std::to_string(p.numel) + " elements, not " +
+                                             std::to_string(cols));
+    *out = {p.data, p.bf16, otherwise};
+    return b.array(p.data, cols, p.bf16 ? 2 : 4, what, false);
+}
+
+}  // namespace
+}  // namespace ttp
+
+using namespace ttp;
+using ttpi::fail;
+
+extern "C" {
+
+int ttp_layer_norm(ttp_ctx* ctx, uint32_t weight, uint32_t bias, const ttp_matrix* x, double eps,
+                   const ttp_matrix* y, float* mean, float* rstd) {
+    return ttpi::guarded([&]() -> int {
+        ttpi::Op op;
+        int rc = ttpi::begin(ctx, &op);
+        if (rc) return rc;
+        if (!(eps >= 0.0 && eps <= 1e30)) return fail(TTP_ERR_INVALID, "eps must be 0 or more");
+        if ((rc = ttpi::check_matrix(x, "the input"))) return rc;
+        const uint64_t rows = x->rows, cols = x->cols;
+        if ((rc = check_cols(cols))) return rc;
+        NormArgs a{};
+        ttpi::Buffers b(ctx);
+        if ((rc = b.matrix(x, rows, cols, "the input", false))) return rc;
+        if ((rc = vector_param(ctx, b, weight, cols, 1.0f, "the weight", &a.weight))) return rc;
+        if ((rc = vector_param(ctx, b, bias, cols, 0.0f, "the bias", &a.bias))) return rc;
+        if ((rc = b.matrix(y, rows, cols, "the output", true, x))) return rc;
+        if ((rc = b.array(mean, rows, 4, "the means", true))) return rc;
+        if ((rc = b.array(rstd, rows, 4, "the reciprocal deviations", true))) return rc;
+        if (!rows) return TTP_OK;
+        a.rows = rows;
+        a.cols = (uint32_t)cols;
+        a.eps = eps;
+        a.x = x->data;
+        a.x_stride = x->stride;
+        a.out = y->data;
+        a.out_stride = y->stride;
+        a.mean = mean;
+        a.rstd = rstd;
+        const bool bf16 = y->dtype == TTP_DTYPE_BF16;
+        if (x->dtype == TTP_DTYPE_BF16)
+            return bf16 ? norm_rows<uint16_t, uint16_t>(op, a) : norm_rows<uint16_t, float>(op, a);
+        return bf16 ? norm_rows<float, uint16_t>(op, a) : norm_rows<float, float>(op, a);
+    });
+}
+
+int ttp_layer_norm_backward(ttp_ctx* ctx, uint32_t weight, uint32_t bias, const ttp_matrix* x,
+                            const ttp_matrix* dy, const float* mean, const float* rstd,
+                            const ttp_matrix* add, const ttp_matrix* dx) {
+    return ttpi::guarded([&]() -> int {
+        ttpi::Op op;
+        int rc = ttpi::begin(ctx, &op);
+        if (rc) return rc;
+        if ((rc = ttpi::check_matrix(x, "the input"))) return rc;
+        const uint64_t rows = x->rows, cols = x->cols;
+        if ((rc = check_cols(cols))) return rc;
+        const bool has_weight = weight != TTP_NO_TENSOR, has_bias = bias != TTP_NO_TENSOR;
+        if (has_weight && weight == bias)
+            return fail(TTP_ERR_INVALID, "the weight and the bias are the same tensor");
+        ttpi::GradTarget w{}, s{};
+        if (has_weight && (rc = ttpi::grad_target(ctx, weight, &w))) return rc;
+        if (has_bias && (rc = ttpi::grad_target(ctx, bias, &s))) return rc;
+        NormArgs a{};
+        ttpi::Buffers b(ctx);
+        if ((rc = b.matrix(x, rows, cols, "the input", false))) return rc;
+        if ((rc = b.matrix(dy, rows, cols, "the output's gradient", false))) return rc;
+        if (add && (rc = b.matrix(add, rows, cols, "the gradient to add", false))) return rc;
+        if ((rc = b.array(mean, rows, 4, "the means", false))) return rc;
+        if ((rc = b.array(rstd, rows, 4, "the reciprocal deviations", false))) return rc;
+        Vector ignored;
+        if ((rc = vector_param(ctx, b, weight, cols, 1.0f, "the weight", &a.weight))) return rc;
+        if ((rc = vector_param(ctx, b, bias, cols, 0.0f, "the bias", &ignored))) return rc;
+        const uint64_t size = w.bf16 || s.bf16 ? 2 : 4;
+        if (has_weight && (rc = b.array(w.data, cols, size, "the weight's gradient", true)))
+            return rc;
+        if (has_bias && (rc = b.array(s.data, cols, size, "the bias's gradient", true))) return rc;
+        const ttp_matrix* place = !dx                            ? x
+                                  : add && dx->data == add->data ? add
+                                  : dy->data == dx->data         ? dy
+                                                                 : x;
+        if ((rc = b.matrix(dx, rows, cols, "the input's gradient", true, place))) return rc;
+        if (dx->dtype != x->dtype || (add && add->dtype != x->dtype))
+            return fail(TTP_ERR_INVALID,
+                        "the input, its gradient and the gradient to add have different types");
+        a.rows = rows;
+        a.cols = (uint32_t)cols;
+        a.x = x->data;
+        a.x_stride = x->stride;
+        a.in = dy->data;
+        a.in_stride = dy->stride;
+        a.add = add ? add->data : nullptr;
+        a.add_stride = add ? add->stride : 0;
+        a.out = dx->data;
+        a.out_stride = dx->stride;
+        a.mean = const_cast<float*>(mean);
+        a.rstd = const_cast<float*>(rstd);
+        const Parts p = parts_of(op, rows, a.cols);
+        void* ws = nullptr;
+        if (p.n && (rc = ttpi::workspace(ctx, (uint64_t)p.n * 2 * cols * 4, &ws))) return rc;
+        a.parts = (float*)ws;
+        if (p.n) {
+            const bool bf16 = dy->dtype == TTP_DTYPE_BF16;
+            if (x->dtype == TTP_DTYPE_BF16)
+                rc = bf16 ? norm_backward_rows<uint16_t, uint16_t>(op, a, p)
+                          : norm_backward_rows<uint16_t, float>(op, a, p);
+            else
+                rc = bf16 ? norm_backward_rows<float, uint16_t>(op, a, p)
+                          : norm_backward_rows<float, float>(op, a, p);
+            if (rc) return rc;
+        }
+        if (has_weight || has_bias) {
+            const JoinArgs j{a.parts, p.n, a.cols, w.data, s.data, size == 2, w.first, s.first};
+            const uint32_t blocks = (uint32_t)((2 * cols + 63) / 64);
+            hipLaunchKernelGGL(join_columns_kernel, dim3(blocks), dim3(1024), 0, op.stream, j);
+            TTPI_HIP(hipGetLastError());
+        }
+        if (has_weight) ttpi::grad_written(ctx, weight);
+        if (has_bias) ttpi::grad_written(ctx, bias);
+        return TTP_OK;
+    });
+}
+
+}  // extern "C"

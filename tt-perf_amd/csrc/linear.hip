@@ -1,0 +1,374 @@
+// linear.hip — y = residual + dropout(activation(x W + bias)).
+//
+// Bound by the matrix instructions at 2 rows cols outs operations.  bf16 products are exact, sums are
+// fp32.  An fp32 operand is the sum of three bf16 parts (8 bits each), and of the nine products of
+// two operands the six largest are taken.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "columns8.hpp"
+#include "context.hpp"
+#include "dropout.hpp"
+#include "gelu.hpp"
+#include "matrix.hpp"
+#include "operand.hpp"
+#include "vector16.hpp"
+
+namespace ttp {
+namespace {
+
+struct LinearArgs {
+    const void *x, *w;
+    uint64_t x_stride, w_stride;
+    uint32_t rows, cols, outs;
+    uint32_t tiles_m, tiles_n;
+    // what follows the product
+    const void* bias;  // or null, of x's type
+    int activation;
+    bool has_dropout;
+    Dropout dropout;
+    const void* residual;  // or null, of y's type
+    void* y;
+    uint64_t residual_stride, y_stride;
+};
+
+// ---- what follows the product -----------------------------------------------------------------
+// 8 neighbouring sums of a row (column c a multiple of 8), on to y.
+template <class G, class Y>
+__device__ __forceinline__ void finish8(const LinearArgs& a, uint64_t seed, uint32_t row, uint32_t c,
+                                        float (&v)[8]) {
+    if (a.bias) {
+        float b[8];
+        load_cols((const G*)a.bias, c, a.outs, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += b[j];
+    }
+    if (a.activation == TTP_ACTIVATION_RELU) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];  // (NaN stays NaN)
+    } else if (a.activation == TTP_ACTIVATION_GELU_ERF) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = gelu<false>(v[j]);
+    } else if (a.activation == TTP_ACTIVATION_GELU_TANH) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = gelu<true>(v[j]);
+    }
+    float r[8];
+    if (a.residual) load_cols((const Y*)a.residual + row * a.residual_stride, c, a.outs, r);
+    if (a.has_dropout) {
+        const uint32_t groups = (a.outs + 7) / 8;
+        const u32x4 w = philox(seed, a.dropout.stream, (uint64_t)row * groups + c / 8);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const bool keep = keeps(w, j, a.dropout.threshold);
+            const float kept = v[j] * a.dropout.factor;
+            if (a.residual)
+                v[j] = keep ? r[j] + kept : r[j];
+            else
+                v[j] = keep ? kept : 0.0f;
+        }
+    } else if (a.residual) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = r[j] + v[j];
+    }
+    store_cols((Y*)a.y + row * a.y_stride, c, a.outs, v);
+}
+
+// ---- operands ---------------------------------------------------------------------------------
+// a and b as sums of three bf16 each (pairs packed): the first cut off, so that infinities and the
+// largest numbers stay what they are, the others to nearest.  What is left of an infinity is taken
+// from the largest number.  (See split3 for numbers below 2^-110 and NaN.)
+__device__ __forceinline__ void split3_nearest(float a, float b, uint32_t (&p)[3]) {
+    constexpr float kMost = 3.4028234663852886e38f;
+    p[0] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+    a = __builtin_amdgcn_fmed3f(a, -kMost, kMost);
+    b = __builtin_amdgcn_fmed3f(b, -kMost, kMost);
+    a -= __uint_as_float(__float_as_uint(a) & 0xFFFF0000u);
+    b -= __uint_as_float(__float_as_uint(b) & 0xFFFF0000u);
+#pragma unroll
+    for (int k = 1; k < 3; ++k) {
+        const f32x2 two = {a, b};
+        p[k] = __builtin_bit_cast(uint32_t, __builtin_convertvector(two, bf16x2));
+        a -= bf16_lo(p[k]);
+        b -= bf16_hi(p[k]);
+    }
+}
+template <class G>
+__device__ __forceinline__ void planes_of(const Chunk8<G>& c, u32x4 (&p)[sizeof(G) == 2 ? 1 : 3]) {
+    if constexpr (sizeof(G) == 2) {
+        c.planes(p);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            uint32_t three[3];
+            split3_nearest(c.value(2 * k), c.value(2 * k + 1), three);
+#pragma unroll
+            for (int j = 0; j < 3; ++j) p[j][k] = three[j];
+        }
+    }
+}
+
+// The first parts with infinities as the largest number, for the products with another operand's
+// second and third part, which may be 0 where the operand is not.
+__device__ __forceinline__ bf16x8 finite(bf16x8 v) {
+    typedef short i16x8 __attribute__((ext_vector_type(8)));
+    typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+    const i16x8 most = (i16x8)(short)0x7F7F;
+    const u16x8 least = (u16x8)(unsigned short)0xFF7F;
+    const u16x8 u = __builtin_elementwise_min(__builtin_bit_cast(u16x8, v), least);
+    return __builtin_bit_cast(bf16x8,
+                              __builtin_elementwise_min(__builtin_bit_cast(i16x8, u), most));
+}
+
+// ---- operands of any alignment, through registers ---------------------------------------------
+// 128 x 128 of y per block, 32 of the summed index per step, through two LDS buffers.
+constexpr uint32_t kTile = 128, kStep = 32;
+constexpr int kPitchK = kStep + 8;  // LDS rows along the summed index, padded against conflicts
+constexpr int kPitchN = kTile + 32;
+
+// 8 consecutive elements of the summed index of row f + lane % 32, from n + 8 (lane / 32) on
+__device__ __forceinline__ bf16x8 row_fragment(const short* lds, int n, int f) {
+    const int lane = threadIdx.x & 63;
+    return *reinterpret_cast<const bf16x8*>(lds + (f + (lane & 31)) * kPitchK + n + (lane >> 5) * 8);
+}
+
+template <class G, class Y, bool kTransposed>
+__global__ __launch_bounds__(256) void linear_kernel(LinearArgs a) {
+    constexpr int kPlanes = sizeof(G) == 2 ? 1 : 3;
+    constexpr int kSizeA = kTile * kPitchK;
+    constexpr int kSizeB = kTransposed ? kTile * kPitchK : kStep * kPitchN;
+    constexpr int kBuffer = kPlanes * (kSizeA + kSizeB);
+    constexpr int kOutPitch = 36;  // floats; a wave's 32 x 32 of y on its way out
+    static_assert(2 * kBuffer * 2 >= 4 * 32 * kOutPitch * 4);
+    __shared__ __align__(16) short lds[2 * kBuffer];
+
+    const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
+    const uint32_t m0 = id % a.tiles_m * kTile, n0 = id / a.tiles_m * kTile;
+    const int t = threadIdx.x, lane = t & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int wm = wave / 2 * 64, wn = wave % 2 * 64;
+
+    // this lane's chunks of a step: two of x (rows along the summed index), two of W
+    const uint32_t rk = t % 4 * 8, rr = t / 4;            // of 32 columns x 128 rows
+    const uint32_t nn = t % 16 * 8, nk = t / 16;          // of 128 columns x 32 rows
+    struct Loads {
+        Chunk8<G> a[2], b[2];
+    };
+    const auto some = [](Chunk8<G>& c, const G* p, int n) {
+        if (n >= 8)
+            c.load(p);
+        else if (n > 0)
+            c.load_some(p, n);
+        else
+            c.clear();
+    };
+    const auto load = [&](Loads& l, uint32_t k0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t m = m0 + rr + 64 * h, k = k0 + rk;
+            some(l.a[h], (const G*)a.x + m * a.x_stride + k,
+                 m < a.rows && k < a.cols ? (int)min(a.cols - k, 8u) : 0);
+            if constexpr (kTransposed) {
+                const uint32_t n = n0 + rr + 64 * h;
+                some(l.b[h], (const G*)a.w + n * a.w_stride + k,
+                     n < a.outs && k < a.cols ? (int)min(a.cols - k, 8u) : 0);
+            } else {
+                const uint32_t n = n0 + nn, kb = k0 + nk + 16 * h;
+                some(l.b[h], (const G*)a.w + kb * a.w_stride + n,
+                     kb < a.cols && n < a.outs ? (int)min(a.outs - n, 8u) : 0);
+            }
+        }
+    };
+    const auto store = [&](const Loads& l, short* buffer) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            u32x4 w[kPlanes];
+            planes_of(l.a[h], w);
+#pragma unroll
+            for (int p = 0; p < kPlanes; ++p)
+                *reinterpret_cast<u32x4*>(buffer + p * kSizeA + (rr + 64 * h) * kPitchK + rk) =
+                    w[p];
+            planes_of(l.b[h], w);
+            short* b = buffer + kPlanes * kSizeA;
+#pragma unroll
+            for (int p = 0; p < kPlanes; ++p)
+                *reinterpret_cast<u32x4*>(
+                    b + p * kSizeB +
+                    (kTransposed ? (rr + 64 * h) * kPitchK + rk : (nk + 16 * h) * kPitchN + nn)) =
+                    w[p];
+        }
+    };
+
+    f32x16 acc[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
+    const auto multiply = [&](const short* buffer) {
+#pragma unroll
+        for (int k = 0; k < (int)kStep; k += 16) {
+            bf16x8 fa[kPlanes][2], fb[kPlanes][2];
+#pragma unroll
+            for (int p = 0; p < kPlanes; ++p)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    fa[p][i] = row_fragment(buffer + p * kSizeA, k, wm + 32 * i);
+                    const short* b = buffer + kPlanes * kSizeA + p * kSizeB;
+                    fb[p][i] = kTransposed ? row_fragment(b, k, wn + 32 * i)
+                                           : fragment(b, kPitchN, k, wn + 32 * i);
+                }
+            const auto products = [&](const bf16x8(&u)[2], const bf16x8(&v)[2]) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[i], v[j], acc[i][j],
+                                                                            0, 0, 0);
+            };
+            products(fa[0], fb[0]);
+            if constexpr (kPlanes == 3) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    fa[0][i] = finite(fa[0][i]);
+                    fb[0][i] = finite(fb[0][i]);
+                }
+                products(fa[0], fb[1]);
+                products(fa[1], fb[0]);
+                products(fa[0], fb[2]);
+                products(fa[1], fb[1]);
+                products(fa[2], fb[0]);
+            }
+        }
+    };
+    const uint32_t steps = (a.cols + kStep - 1) / kStep;
+    Loads l;
+    load(l, 0);
+    store(l, lds);
+    __syncthreads();
+    for (uint32_t s = 0; s < steps; ++s) {
+        if (s + 1 < steps) load(l, (s + 1) * kStep);
+        multiply(lds + (s & 1) * kBuffer);
+        if (s + 1 < steps) store(l, lds + ((s + 1) & 1) * kBuffer);
+        __syncthreads();
+    }
+
+    // out, 32 x 32 at a time through this wave's LDS
+    const uint64_t seed = a.has_dropout ? seed_of(a.dropout) : 0;
+    float* out = reinterpret_cast<float*>(lds) + wave * 32 * kOutPitch;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                out[(8 * (k / 4) + 4 * (lane >> 5) + k % 4) * kOutPitch + (lane & 31)] =
+                    acc[i][j][k];
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t r = lane / 4 + 16 * h, c = lane % 4 * 8;
+                float v[8];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const f32x4 w = *reinterpret_cast<const f32x4*>(out + r * kOutPitch + c + 4 * q);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) v[4 * q + k] = w[k];
+                }
+                const uint32_t row = m0 + wm + 32 * i + r, col = n0 + wn + 32 * j + c;
+                if (row < a.rows && col < a.outs) finish8<G, Y>(a, seed, row, col, v);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+}
+
+template <class G, class Y>
+int multiply(const ttpi::Op& op, LinearArgs a, bool transposed) {
+    a.tiles_m = (a.rows + kTile - 1) / kTile;
+    a.tiles_n = (a.outs + kTile - 1) / kTile;
+    const uint64_t blocks = (uint64_t)a.tiles_m * a.tiles_n;
+    if (blocks >= (1ull << 24))
+        return ttpi::fail(TTP_ERR_RANGE, "the product has too many tiles for one launch");
+    (void)hipGetLastError();
+    const dim3 grid((uint32_t)blocks), block(256);
+    if (transposed)
+        hipLaunchKernelGGL((linear_kernel<G, Y, true>), grid, block, 0, op.stream, a);
+    else
+        hipLaunchKernelGGL((linear_kernel<G, Y, false>), grid, block, 0, op.stream, a);
+    TTPI_HIP(hipGetLastError());
+    return TTP_OK;
+}
+
+}  // namespace
+}  // namespace ttp
+
+using namespace ttp;
+using ttpi::fail;
+
+extern "C" int ttp_linear(ttp_ctx* ctx, const ttp_linear_args* args) {
+    return ttpi::guarded([&]() -> int {
+        ttpi::Op op;
+        int rc = ttpi::begin(ctx, &op);
+        if (rc) return rc;
+        if (!args) return fail(TTP_ERR_INVALID, "null arguments");
+        const ttp_matrix *x = args->x, *y = args->y, *res = args->residual;
+        if (args->transposed != 0 && args->transposed != 1)
+            return fail(TTP_ERR_INVALID, "transposed must be 0 or 1");
+        if (args->activation < TTP_ACTIVATION_NONE || args->activation > TTP_ACTIVATION_GELU_TANH)
+            return fail(TTP_ERR_INVALID, "activation must be a TTP_ACTIVATION_*");
+        if (args->dropout && (rc = check_dropout(args->dropout))) return rc;
+        if ((rc = ttpi::check_matrix(x, "the input"))) return rc;
+        if ((rc = ttpi::check_matrix(y, "the output"))) return rc;
+        const uint64_t rows = x->rows, cols = x->cols, outs = y->cols;
+        const bool has_bias = args->bias != TTP_NO_TENSOR;
+        ttpi::Param w{}, bias{};
+        if ((rc = ttpi::param(ctx, args->weight, &w))) return rc;
+        if (has_bias && (rc = ttpi::param(ctx, args->bias, &bias))) return rc;
+        if (w.numel != cols * outs)
+            return fail(TTP_ERR_RANGE, "tensor " + std::to_string(args->weight) + " has " +
+                                           std::to_string(w.numel) + " elements, not " +
+                                           std::to_string(cols) + " x " + std::to_string(outs));
+        if (has_bias && bias.numel != outs)
+            return fail(TTP_ERR_RANGE, "tensor " + std::to_string(args->bias) + " has " +
+                                           std::to_string(bias.numel) + " elements, not " +
+                                           std::to_string(outs));
+        const bool bf16 = x->dtype == TTP_DTYPE_BF16;
+        if (bf16 != w.bf16)
+            return fail(TTP_ERR_INVALID, std::string("the input has another type than the weight (") +
+                                             (w.bf16 ? "bfloat16" : "float32") + ")");
+        ttpi::Buffers b(ctx);
+        if ((rc = b.matrix(x, rows, cols, "the input", false))) return rc;
+        if ((rc = b.array(w.data, w.numel, bf16 ? 2 : 4, "the weight", false))) return rc;
+        if (has_bias && (rc = b.array(bias.data, outs, bf16 ? 2 : 4, "the bias", false))) return rc;
+        if (res && (rc = b.matrix(res, rows, outs, "the residual", false))) return rc;
+        if (args->dropout && args->dropout->device_seed &&
+            (rc = b.array(args->dropout->device_seed, 1, 8, "the seed", false)))
+            return rc;
+        if ((rc = b.matrix(y, rows, outs, "the output", true, res))) return rc;
+        if (res && res->dtype != y->dtype)
+            return fail(TTP_ERR_INVALID, "the residual and the output have different types");
+        if (!rows) return TTP_OK;
+        LinearArgs a{};
+        a.x = x->data;
+        a.w = w.data;
+        a.x_stride = x->stride;
+        a.w_stride = args->transposed ? cols : outs;
+        a.rows = (uint32_t)rows;
+        a.cols = (uint32_t)cols;
+        a.outs = (uint32_t)outs;
+        a.bias = bias.data;
+        a.activation = args->activation;
+        a.has_dropout = args->dropout != nullptr;
+        if (a.has_dropout) a.dropout = dropout_of(*args->dropout);
+        a.residual = res ? res->data : nullptr;
+        a.residual_stride = res ? res->stride : 0;
+        a.y = y->data;
+        a.y_stride = y->stride;
+        const bool y16 = y->dtype == TTP_DTYPE_BF16;
+        if (bf16)
+            return y16 ? multiply<uint16_t, uint16_t>(op, a, args->transposed)
+                       : multiply<uint16_t, float>(op, a, args->transposed);
+        return y16 ? multiply<float, uint16_t>(op, a, args->transposed)
+                   : multiply<float, float>(op, a, args->transposed);
+    });
+}

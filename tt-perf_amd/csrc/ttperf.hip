@@ -1300,6 +1300,14 @@ void grad_written(ttp_ctx* c, uint32_t index) {
     set_fresh(c, index, false);
 }
 
+int param(ttp_ctx* c, uint32_t index, Param* out) {
+    int rc = check_index(c, index);
+    if (rc) return rc;
+    const TensorRec& t = c->tensors[index];
+    *out = {(const char*)c->param + t.offset * param_esize(c), t.numel, bf16_grads(c)};
+    return TTP_OK;
+}
+
 }  // namespace ttpi
 
 // =====================================================================================

@@ -8,13 +8,13 @@ from . import _lib
 from ._lib import (ALL_TENSORS, BUF_EXP_AVG, BUF_EXP_AVG_SQ, BUF_GRAD, BUF_MASTER,
                    BUF_MOMENTUM, BUF_PARAM, TTPError, TTPMemoryError, TTPValueError,
                    device_count)
-from .operators import Checkpoint8, PolicyLoss, PreferenceLoss
+from .operators import Checkpoint8, LayerNorm, PolicyLoss, PreferenceLoss
 from .optim import SGD, Adam, AdamW
 from .store import GradView, Parameter, ParamStore, StepGraph, Tensor, TraceContext
 
 __all__ = ["SGD", "Adam", "AdamW", "ParamStore", "Tensor", "Parameter", "GradView",
            "StepGraph", "TraceContext", "PreferenceLoss", "PolicyLoss",
-           "Checkpoint8",
+           "Checkpoint8", "LayerNorm",
            "TTPError", "TTPValueError", "TTPMemoryError", "device_count", "_lib",
            "BUF_PARAM", "BUF_GRAD", "BUF_MASTER", "BUF_EXP_AVG", "BUF_EXP_AVG_SQ",
            "BUF_MOMENTUM", "ALL_TENSORS"]

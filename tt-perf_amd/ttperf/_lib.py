@@ -28,6 +28,7 @@ CHECKPOINT_INT8, CHECKPOINT_E4M3 = 0, 1
 CHECKPOINT_BLOCK = 32  # columns that share a scale
 GELU_ERF, GELU_TANH = 0, 1
 NO_TENSOR = 0xFFFFFFFF
+ACTIVATION_NONE, ACTIVATION_RELU, ACTIVATION_GELU_ERF, ACTIVATION_GELU_TANH = range(4)
 STEP_TENSOR_SUMS = 1
 STEP_DEFER_SCALE = 2
 KERNEL_NORM, KERNEL_UPDATE = 0, 1
@@ -93,6 +94,16 @@ class Checkpoint8(C.Structure):
                 ("format", C.c_int32), ("reserved", C.c_int32)]
 
 
+class Dropout(C.Structure):
+    _fields_ = [("p", C.c_double), ("seed", C.c_uint64), ("stream", C.c_uint64),
+                ("device_seed", _P)]
+
+
+class LinearArgs(C.Structure):
+    _fields_ = [("x", _P), ("residual", _P), ("y", _P), ("dropout", _P), ("weight", C.c_uint32),
+                ("bias", C.c_uint32), ("transposed", C.c_int32), ("activation", C.c_int32)]
+
+
 # name -> (restype, argtypes); the ABI surface the header declares
 SIGNATURES = {
     "ttp_device_count": (C.c_int, [C.POINTER(C.c_int)]),
@@ -153,6 +164,18 @@ SIGNATURES = {
                                      C.POINTER(Matrix)]),
     "ttp_accumulate_linear_grad8": (C.c_int, [_P, C.c_uint32, C.c_uint32, C.POINTER(Checkpoint8),
                                               C.POINTER(Matrix), C.c_int]),
+    "ttp_dropout_forward": (C.c_int, [_P, C.POINTER(Dropout), C.POINTER(Matrix), C.POINTER(Matrix),
+                                      C.POINTER(Matrix)]),
+    "ttp_embedding": (C.c_int, [_P, C.c_uint32, _P, C.c_double, C.c_uint32, _P,
+                                C.POINTER(Matrix)]),
+    "ttp_accumulate_embedding_grad": (C.c_int, [_P, C.c_uint32, _P, C.c_double,
+                                                C.POINTER(Matrix)]),
+    "ttp_layer_norm": (C.c_int, [_P, C.c_uint32, C.c_uint32, C.POINTER(Matrix), C.c_double,
+                                 C.POINTER(Matrix), _P, _P]),
+    "ttp_layer_norm_backward": (C.c_int, [_P, C.c_uint32, C.c_uint32, C.POINTER(Matrix),
+                                          C.POINTER(Matrix), _P, _P, C.POINTER(Matrix),
+                                          C.POINTER(Matrix)]),
+    "ttp_linear": (C.c_int, [_P, C.POINTER(LinearArgs)]),
     "ttp_timing_enable": (C.c_int, [_P, C.c_int]),
     "ttp_timing_collect": (C.c_int, [_P, C.c_int, C.POINTER(C.c_double), C.POINTER(C.c_uint64)]),
     "ttp_last_error": (C.c_char_p, []),

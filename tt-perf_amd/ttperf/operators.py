@@ -1,5 +1,6 @@
-"""The fine-tuning operators of a ParamStore: losses over logits with their gradient, activations
-kept in 8 bits and the gradients made from them.
+"""The operators of a ParamStore: a fine-tuning step's (losses over logits with their gradient,
+activations kept in 8 bits and the gradients made from them) and a transformer block's (embeddings,
+layer norm, dropout and linear products on the store's weights, with their gradients).
 
 They take and give torch tensors on the store's device.  Results are new tensors unless given;
 work is queued on the store's stream, ordered with torch's current stream as the store's other
@@ -47,6 +48,14 @@ class PolicyLoss(NamedTuple):
     grad: Optional[Any]
 
 
+class LayerNorm(NamedTuple):
+    """y like the input, and each row's mean and reciprocal standard deviation in float32, which
+    the backward takes."""
+    y: Any
+    mean: Any
+    rstd: Any
+
+
 class Checkpoint8:
     """An activation kept in 8 bits (ttp_checkpoint8): `values` (rows, cols rounded up to 32) and
     `scales` (rows, that / 32), both uint8; element i of a row is values[i] (int8, or fp8 e4m3)
@@ -78,6 +87,8 @@ class Checkpoint8:
 
 _FORMATS = {"int8": L.CHECKPOINT_INT8, "e4m3": L.CHECKPOINT_E4M3}
 _APPROXIMATE = {"none": L.GELU_ERF, "tanh": L.GELU_TANH}
+_ACTIVATIONS = {None: L.ACTIVATION_NONE, "relu": L.ACTIVATION_RELU, "gelu": L.ACTIVATION_GELU_ERF,
+                "gelu_tanh": L.ACTIVATION_GELU_TANH}
 
 
 def _choice(table, key, what):
@@ -416,6 +427,203 @@ class Operators:
                                  f"{len(self.tensors)} tensors)")
         self._queue((kept.values, kept.scales, g), (), L.lib.ttp_accumulate_linear_grad8, index,
                     bias, kept._c(), _matrix(g), 1 if transposed else 0)
+
+    # ---- a transformer block's operators ---------------------------------------------------------
+    def _index(self, index, what):
+        """A tensor index for the library, which has 32 bits of it (None: no tensor)."""
+        if index is None:
+            return L.NO_TENSOR
+        if not 0 <= index < len(self.tensors):
+            raise ValueError(f"{what}: tensor index {index} out of range (the store has "
+                             f"{len(self.tensors)} tensors)")
+        return index
+
+    def _table(self, index, what):
+        """(index, columns) of a table: a tensor of two dimensions."""
+        if index is None:
+            raise ValueError(f"{what} must be a tensor index")
+        index, shape = self._index(index, what), self.tensors[index].shape
+        if len(shape) != 2 or not shape[0] or not shape[1]:
+            raise ValueError(f"{what} has shape {shape}; rows and columns are needed")
+        return index, shape[1]
+
+    def _param_dtype(self):
+        return torch.float32 if self.mode == L.MODE_FP32 else torch.bfloat16
+
+    def _output(self, out, like, shape, dtype, what):
+        """(the result, its matrix): `out`, checked, or a new tensor; rows may be apart."""
+        if dtype not in _ROW_TYPES:
+            raise ValueError("dtype must be torch.float32 or torch.bfloat16")
+        if out is None:
+            out = self._result(None, like, shape, dtype, what)
+        elif not isinstance(out, torch.Tensor) or out.dtype != dtype or \
+                out.shape != torch.Size(shape):
+            raise ValueError(f"{what} must be a {str(dtype)[6:]} tensor of shape {tuple(shape)}")
+        return out, self._rows_of(out, what)
+
+    def _tokens(self, t, what):
+        if not isinstance(t, torch.Tensor):
+            raise ValueError(f"{what} must be a int64 tensor on the GPU")
+        return self._vector_of(t, t.numel(), torch.int64, what)
+
+    def embedding(self, index, tokens, *, scale=1.0, position=None, positions=None, dtype=None,
+                  out=None):
+        """The rows of tensor `index` (vocabulary, cols) that `tokens` (int64, any shape) name,
+        times `scale`: (*tokens.shape, cols), of the store's parameter type or `dtype`.
+        position, positions: a second table and its row for each token, added (GPT-2's learned
+        positions).  A negative token or position stands for zeros, one past its table gives NaN.
+        (ttp_embedding)"""
+        if (position is None) != (positions is None):
+            raise ValueError("a table of positions and the positions go together")
+        index, cols = self._table(index, "the table")
+        t, p = self._tokens(tokens, "the tokens"), None
+        if position is not None:
+            position, width = self._table(position, "the table of positions")
+            if width != cols:
+                raise ValueError(f"the tables have {cols} and {width} columns")
+            p = self._vector_of(positions, t.numel(), torch.int64, "the positions")
+            if positions.dim() > 1 and positions.shape != tokens.shape:
+                raise ValueError("the positions must have the tokens' shape (or be flat)")
+        given = () if out is None else (out,)
+        dtype = dtype or (self._param_dtype() if out is None else out.dtype)
+        out, m = self._output(out, t, (*tokens.shape, cols), dtype, "out")
+        used = [t] if p is None else [t, p]
+        self._queue([*used, *given], given, L.lib.ttp_embedding, index, t.data_ptr(), scale,
+                    L.NO_TENSOR if p is None else position, _ptr(p), _matrix(m))
+        return out
+
+    def accumulate_embedding_grad(self, index, tokens, dy, *, scale=1.0):
+        """Add an embedding's gradient to the store's: row v of tensor `index` receives `scale`
+        times the sum of the rows of dy (*tokens.shape, cols), float32 or bfloat16, whose token is
+        v; tokens outside the table are passed over.  As accumulate_grad: a first gradient is
+        assigned (the rows that no token names become 0), a further one added in fp32 and
+        rounded once.  The same call takes a position table's gradient, with the positions for
+        tokens.  (ttp_accumulate_embedding_grad)"""
+        index, cols = self._table(index, "the table")
+        g = self._rows_of(dy, "dy")
+        if dy.shape[-1] != cols:
+            raise ValueError(f"dy has {dy.shape[-1]} columns, the table {cols}")
+        t = self._tokens(tokens, "the tokens")
+        if t.numel() != g.shape[0]:
+            raise ValueError(f"{t.numel()} tokens for {g.shape[0]} rows of dy")
+        if tokens.dim() > 1:
+            _check_row_order(dy, tokens)
+        self._queue((t, g), (), L.lib.ttp_accumulate_embedding_grad, index, t.data_ptr(), scale,
+                    _matrix(g))
+
+    def layer_norm(self, index, x, *, bias=None, eps=1e-5, dtype=None, out=None):
+        """Layer norm of x's rows (..., cols), float32 or bfloat16, with tensor `index` for the
+        weight and tensor `bias` (None: 1 and 0): a LayerNorm of y, in x's type or `dtype`, and the
+        rows' mean and rstd.  out: an earlier call's result to write again (out.y may be x).
+        (ttp_layer_norm)"""
+        w, b = self._index(index, "the weight"), self._index(bias, "the bias")
+        m = self._rows_of(x, "the input")
+        dtype = dtype or (x.dtype if out is None else out.y.dtype)
+        y, ym = self._output(out and out.y, x, x.shape, dtype, "out.y")
+        rows = x.shape[:-1]
+        mean = self._result(out and out.mean, x, rows, torch.float32, "out.mean")
+        rstd = self._result(out and out.rstd, x, rows, torch.float32, "out.rstd")
+        given = () if out is None else (y, mean, rstd)
+        self._queue((m,) + given, given, L.lib.ttp_layer_norm, w, b, _matrix(m), eps, _matrix(ym),
+                    mean.data_ptr(), rstd.data_ptr())
+        return LayerNorm(y, mean, rstd)
+
+    def layer_norm_backward(self, index, x, dy, mean, rstd, *, bias=None, add=None, out=None):
+        """The input's gradient of layer_norm, in x's type, plus `add` (like x: what a residual
+        connection brings); the weight's and the bias's are added to the store's gradients, as
+        accumulate_grad does.  mean, rstd: layer_norm's.  out: where to put it: dy, add or x
+        too.  (ttp_layer_norm_backward)"""
+        w, b = self._index(index, "the weight"), self._index(bias, "the bias")
+        m, g = self._rows_of(x, "the input"), self._rows_of(dy, "dy")
+        if dy.shape != x.shape:
+            raise ValueError(f"dy has shape {tuple(dy.shape)}, the input {tuple(x.shape)}")
+        rows = m.shape[0]
+        mean = self._vector_of(mean, rows, torch.float32, "mean")
+        rstd = self._vector_of(rstd, rows, torch.float32, "rstd")
+        _check_row_order(x, mean, rstd)
+        am = None if add is None else self._like(add, x, "add")
+        given = () if out is None else (out,)
+        out, d = self._output(out, x, x.shape, x.dtype, "out")
+        used = [t for t in (m, g, mean, rstd, am) if t is not None]
+        self._queue([*used, *given], given, L.lib.ttp_layer_norm_backward, w, b, _matrix(m),
+                    _matrix(g), mean.data_ptr(), rstd.data_ptr(),
+                    None if am is None else _matrix(am), _matrix(d))
+        return out
+
+    def _dropout_of(self, p, seed, stream):
+        """(ttp_dropout, the seed's tensor or None)."""
+        if not 0 <= p < 1:
+            raise ValueError("dropout's p must be in [0, 1)")
+        if not 0 <= stream < 2 ** 64:
+            raise ValueError("stream must be a whole number of 64 bits, 0 or more")
+        if isinstance(seed, torch.Tensor):
+            s = self._vector_of(seed, 1, torch.int64, "the seed")
+            return L.Dropout(p, 0, stream, s.data_ptr()), s
+        if not -2 ** 63 <= seed < 2 ** 64:
+            raise ValueError("the seed must be a whole number of 64 bits")
+        return L.Dropout(p, seed % 2 ** 64, stream, None), None
+
+    def dropout(self, x, p, seed, *, stream=0, residual=None, out=None):
+        """x (..., cols), float32 or bfloat16, with each element dropped (0) with probability p (a
+        multiple of 2^-16) and the others scaled by 1 / (1 - p); plus `residual` (like x).  Which
+        ones are dropped follows from (seed, stream, row, column) by a counter-based generator,
+        so nothing is kept for the backward: dropout(dy, p, seed, stream=stream).  seed: a whole
+        number, or an int64 tensor of one element on the GPU, which the kernel reads (a captured
+        graph then takes its present value at each launch).  out: x or the residual too.
+        (ttp_dropout_forward)"""
+        d, s = self._dropout_of(p, seed, stream)
+        m = self._rows_of(x, "the input")
+        rm = None if residual is None else self._like(residual, x, "the residual")
+        given = () if out is None else (out,)
+        out, ym = self._output(out, x, x.shape, x.dtype, "out")
+        used = [t for t in (m, rm, s) if t is not None]
+        self._queue([*used, *given], given, L.lib.ttp_dropout_forward, d, _matrix(m),
+                    None if rm is None else _matrix(rm), _matrix(ym))
+        return out
+
+    def linear(self, index, x, *, bias=None, activation=None, dropout=None, residual=None,
+               transposed=False, dtype=None, out=None):
+        """residual + dropout(activation(x W + bias)) for x (..., cols) of the store's parameter
+        type, with tensor `index` for W (cols, outs) (py/nn.py:36; transposed=True: (outs, cols),
+        torch.nn.Linear's) and tensor `bias`: (..., outs), of x's type or `dtype`.
+
+        activation: None, "relu", "gelu" or "gelu_tanh".  dropout: (p, seed, stream), as
+        dropout()'s and with its mask.  residual: like the result, which may be written over it
+        (out).  Sums are in fp32, rounded once.  (ttp_linear)"""
+        return self._multiply(index, x, bias, activation, dropout, residual, bool(transposed),
+                              dtype, out)
+
+    def linear_input_grad(self, index, dy, *, add=None, transposed=False, dtype=None, out=None):
+        """The input's gradient of linear(index, x, transposed=transposed): dy W^T, plus `add`
+        (like the result).  (ttp_linear)"""
+        return self._multiply(index, dy, None, None, None, add, not transposed, dtype, out)
+
+    def _multiply(self, index, x, bias, activation, dropout, residual, transposed, dtype, out):
+        act = _choice(_ACTIVATIONS, activation, "activation")
+        index, _ = self._table(index, "the weight")
+        shape = self.tensors[index].shape
+        b = self._index(bias, "the bias")
+        m = self._rows_of(x, "the input")
+        cols, outs = shape[::-1] if transposed else shape
+        if x.shape[-1] != cols:
+            raise ValueError(f"the input has {x.shape[-1]} columns, the weight {tuple(shape)} "
+                             f"takes {cols}")
+        if x.dtype != self._param_dtype():
+            raise ValueError(f"the input is {str(x.dtype)[6:]}, the store's weights "
+                             f"{str(self._param_dtype())[6:]}")
+        d, s = (None, None) if dropout is None else self._dropout_of(*dropout)
+        given = () if out is None else (out,)
+        dtype = dtype or (x.dtype if out is None else out.dtype)
+        out, ym = self._output(out, x, (*x.shape[:-1], outs), dtype, "out")
+        rm = None if residual is None else self._like(residual, out, "the residual")
+        mm, ymm = _matrix(m), _matrix(ym)
+        rmm = None if rm is None else _matrix(rm)
+        args = L.LinearArgs(C.addressof(mm), None if rmm is None else C.addressof(rmm),
+                            C.addressof(ymm), None if d is None else C.addressof(d), index, b,
+                            1 if transposed else 0, act)
+        used = [t for t in (m, rm, s) if t is not None]
+        self._queue([*used, *given], given, L.lib.ttp_linear, args)
+        return out
 
     def _like(self, out, x, what):
         """The matrix of a result that has x's shape and type."""
