@@ -10,7 +10,7 @@ import block_util as B
 from conftest import REPO
 from test_isa_cpu import HIPCC, PKG, scc_reads_live_into_a_block
 
-FILES = ("dropout", "layer_norm", "embedding", "linear")
+FILES = ("dropout", "layer_norm", "embedding", "linear", "linear_to_bf16", "linear_to_fp32")
 
 
 def test_struct_layouts_match_the_header(tmp_path):

@@ -142,18 +142,26 @@ def test_strides_and_places(mode, transposed, rows):
             _check(one[None], x[:1], w, transposed=transposed)
 
 
-def test_larger_products():
-    """Several tiles each way, long and short sums, sizes off every grid."""
+# several tiles each way, long and short sums, sizes on and off every grid
+LARGER = [(1025, 1600, 1601, "mixed"), (3000, 770, 523, "mixed"), (520, 6400, 1600, "mixed"),
+          (2304, 1280, 1280, "bf16"), (700, 1284, 900, "fp32"), (4100, 64, 4100, "mixed"),
+          (300, 50257, 100, "mixed"), (33, 768, 50257, "mixed"), (4099, 1288, 5128, "mixed"),
+          (8200, 200, 1288, "bf16"), (8190, 2568, 1280, "mixed"), (5, 5128, 1288, "mixed"),
+          (100, 5120, 1280, "mixed"), (1, 50264, 136, "mixed")]
+
+
+@pytest.mark.parametrize("rows,cols,outs,mode", LARGER)
+@pytest.mark.parametrize("transposed", [False, True])
+def test_larger_products(rows, cols, outs, mode, transposed):
     torch = torch_mod()
-    for rows, cols, outs, mode in ((1025, 1600, 1601, "mixed"), (3000, 770, 523, "mixed"),
-                                   (520, 6400, 1600, "mixed"), (2304, 1280, 1280, "bf16"),
-                                   (700, 1284, 900, "fp32"), (4100, 64, 4100, "mixed"),
-                                   (300, 50257, 100, "mixed"), (33, 768, 50257, "mixed")):
-        for transposed in (False, True):
-            x, w, b = _inputs(rows, cols, outs, mode, 13, transposed)
-            with B.store_of([w, b], mode) as store:
-                y = store.linear(1, x, bias=2, transposed=transposed)
-                _check(y, x, w, b, transposed=transposed)
+    x, w, b = _inputs(rows, cols, outs, mode, 13, transposed)
+    res = torch.randn(rows, outs, device="cuda").to(x.dtype)
+    with B.store_of([w, b], mode) as store:
+        y = store.linear(1, x, bias=2, transposed=transposed)
+        _check(y, x, w, b, transposed=transposed)
+        y = store.linear(1, x, bias=2, activation="gelu", dropout=(0.1, 3, 1), residual=res,
+                         transposed=transposed)
+        _check(y, x, w, b, "gelu", (0.1, 3, 1), res, transposed)
 
 
 @pytest.mark.parametrize("rows", [1, 9, 200])

@@ -19,7 +19,6 @@
 #include "device.hpp"
 
 namespace ttp {
-namespace {
 
 struct Dropout {
     uint64_t seed, stream;
@@ -27,6 +26,8 @@ struct Dropout {
     uint32_t threshold;  // of 2^16
     float factor;
 };
+
+namespace {
 
 __device__ __forceinline__ u32x4 philox(uint64_t seed, uint64_t stream, uint64_t group) {
     uint32_t c0 = (uint32_t)group, c1 = (uint32_t)(group >> 32);

@@ -7,73 +7,14 @@
 
 #include <algorithm>
 
-#include "columns8.hpp"
 #include "context.hpp"
-#include "dropout.hpp"
-#include "gelu.hpp"
+#include "linear.hpp"
 #include "matrix.hpp"
 #include "operand.hpp"
 #include "vector16.hpp"
 
 namespace ttp {
 namespace {
-
-struct LinearArgs {
-    const void *x, *w;
-    uint64_t x_stride, w_stride;
-    uint32_t rows, cols, outs;
-    uint32_t tiles_m, tiles_n;
-    // what follows the product
-    const void* bias;  // or null, of x's type
-    int activation;
-    bool has_dropout;
-    Dropout dropout;
-    const void* residual;  // or null, of y's type
-    void* y;
-    uint64_t residual_stride, y_stride;
-};
-
-// ---- what follows the product -----------------------------------------------------------------
-// 8 neighbouring sums of a row (column c a multiple of 8), on to y.
-template <class G, class Y>
-__device__ __forceinline__ void finish8(const LinearArgs& a, uint64_t seed, uint32_t row, uint32_t c,
-                                        float (&v)[8]) {
-    if (a.bias) {
-        float b[8];
-        load_cols((const G*)a.bias, c, a.outs, b);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += b[j];
-    }
-    if (a.activation == TTP_ACTIVATION_RELU) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = v[j] < 0.0f ? 0.0f : v[j];  // (NaN stays NaN)
-    } else if (a.activation == TTP_ACTIVATION_GELU_ERF) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = gelu<false>(v[j]);
-    } else if (a.activation == TTP_ACTIVATION_GELU_TANH) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = gelu<true>(v[j]);
-    }
-    float r[8];
-    if (a.residual) load_cols((const Y*)a.residual + row * a.residual_stride, c, a.outs, r);
-    if (a.has_dropout) {
-        const uint32_t groups = (a.outs + 7) / 8;
-        const u32x4 w = philox(seed, a.dropout.stream, (uint64_t)row * groups + c / 8);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const bool keep = keeps(w, j, a.dropout.threshold);
-            const float kept = v[j] * a.dropout.factor;
-            if (a.residual)
-                v[j] = keep ? r[j] + kept : r[j];
-            else
-                v[j] = keep ? kept : 0.0f;
-        }
-    } else if (a.residual) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = r[j] + v[j];
-    }
-    store_cols((Y*)a.y + row * a.y_stride, c, a.outs, v);
-}
 
 // ---- operands ---------------------------------------------------------------------------------
 // a and b as sums of three bf16 each (pairs packed): the first cut off, so that infinities and the
@@ -143,8 +84,11 @@ __global__ __launch_bounds__(256) void linear_kernel(LinearArgs a) {
     static_assert(2 * kBuffer * 2 >= 4 * 32 * kOutPitch * 4);
     __shared__ __align__(16) short lds[2 * kBuffer];
 
-    const uint32_t id = xcd_order(blockIdx.x, gridDim.x);
+    uint32_t id = xcd_order(blockIdx.x, gridDim.x);
+    const uint32_t part = id / (a.tiles_m * a.tiles_n);
+    id -= part * (a.tiles_m * a.tiles_n);
     const uint32_t m0 = id % a.tiles_m * kTile, n0 = id / a.tiles_m * kTile;
+    const uint32_t end = min((part + 1) * a.per, a.cols);  // of the summed index
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wm = wave / 2 * 64, wn = wave % 2 * 64;
@@ -155,28 +99,20 @@ __global__ __launch_bounds__(256) void linear_kernel(LinearArgs a) {
     struct Loads {
         Chunk8<G> a[2], b[2];
     };
-    const auto some = [](Chunk8<G>& c, const G* p, int n) {
-        if (n >= 8)
-            c.load(p);
-        else if (n > 0)
-            c.load_some(p, n);
-        else
-            c.clear();
-    };
     const auto load = [&](Loads& l, uint32_t k0) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint32_t m = m0 + rr + 64 * h, k = k0 + rk;
-            some(l.a[h], (const G*)a.x + m * a.x_stride + k,
-                 m < a.rows && k < a.cols ? (int)min(a.cols - k, 8u) : 0);
+            load_upto8(l.a[h], (const G*)a.x + m * a.x_stride + k,
+                 m < a.rows && k < end ? (int)min(end - k, 8u) : 0);
             if constexpr (kTransposed) {
                 const uint32_t n = n0 + rr + 64 * h;
-                some(l.b[h], (const G*)a.w + n * a.w_stride + k,
-                     n < a.outs && k < a.cols ? (int)min(a.cols - k, 8u) : 0);
+                load_upto8(l.b[h], (const G*)a.w + n * a.w_stride + k,
+                     n < a.outs && k < end ? (int)min(end - k, 8u) : 0);
             } else {
                 const uint32_t n = n0 + nn, kb = k0 + nk + 16 * h;
-                some(l.b[h], (const G*)a.w + kb * a.w_stride + n,
-                     kb < a.cols && n < a.outs ? (int)min(a.outs - n, 8u) : 0);
+                load_upto8(l.b[h], (const G*)a.w + kb * a.w_stride + n,
+                     kb < end && n < a.outs ? (int)min(a.outs - n, 8u) : 0);
             }
         }
     };
@@ -241,13 +177,13 @@ __global__ __launch_bounds__(256) void linear_kernel(LinearArgs a) {
             }
         }
     };
-    const uint32_t steps = (a.cols + kStep - 1) / kStep;
+    const uint32_t first = part * a.per, steps = (end - first + kStep - 1) / kStep;
     Loads l;
-    load(l, 0);
+    load(l, first);
     store(l, lds);
     __syncthreads();
     for (uint32_t s = 0; s < steps; ++s) {
-        if (s + 1 < steps) load(l, (s + 1) * kStep);
+        if (s + 1 < steps) load(l, first + (s + 1) * kStep);
         multiply(lds + (s & 1) * kBuffer);
         if (s + 1 < steps) store(l, lds + ((s + 1) & 1) * kBuffer);
         __syncthreads();
@@ -276,27 +212,107 @@ __global__ __launch_bounds__(256) void linear_kernel(LinearArgs a) {
                     for (int k = 0; k < 4; ++k) v[4 * q + k] = w[k];
                 }
                 const uint32_t row = m0 + wm + 32 * i + r, col = n0 + wn + 32 * j + c;
-                if (row < a.rows && col < a.outs) finish8<G, Y>(a, seed, row, col, v);
+                if (row >= a.rows || col >= a.outs) continue;
+                if (a.parts > 1) {
+                    put_part8(a, part, row, col, v);
+                } else {
+                    Chunk8<Y> res;
+                    load_residual(a, row, col, res);
+                    add_bias8<G>(a, col, v);
+                    finish8<Y>(a, seed, row, col, v, res);
+                }
             }
             __builtin_amdgcn_wave_barrier();
         }
 }
 
+// ---- parts ------------------------------------------------------------------------------------
+// The parts' sums in order, and what follows: a lane has 8 columns of a row.
+constexpr int kJoinBlock = 256;
 template <class G, class Y>
-int multiply(const ttpi::Op& op, LinearArgs a, bool transposed) {
-    a.tiles_m = (a.rows + kTile - 1) / kTile;
-    a.tiles_n = (a.outs + kTile - 1) / kTile;
-    const uint64_t blocks = (uint64_t)a.tiles_m * a.tiles_n;
-    if (blocks >= (1ull << 24))
-        return ttpi::fail(TTP_ERR_RANGE, "the product has too many tiles for one launch");
+__global__ __launch_bounds__(kJoinBlock) void join_parts_kernel(LinearArgs a, uint32_t groups,
+                                                                Divider by_groups) {
+    const uint32_t i = blockIdx.x * kJoinBlock + threadIdx.x;
+    if (i >= a.rows * groups) return;
+    const uint32_t row = divide(i, by_groups), c = (i - row * groups) * 8;
+    Chunk8<Y> res;
+    load_residual(a, row, c, res);
+    const uint64_t seed = a.has_dropout ? seed_of(a.dropout) : 0;
+    const float* p = a.partial + (uint64_t)row * a.pitch + c;
+    float v[8] = {};
+#pragma unroll 4
+    for (uint32_t k = 0; k < a.parts; ++k) {
+        float w[8];
+        load_cols(p + (uint64_t)k * a.rows * a.pitch, 0, 8, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += w[j];
+    }
+    add_bias8<G>(a, c, v);
+    finish8<Y>(a, seed, row, c, v, res);
+}
+
+// ---- launches ---------------------------------------------------------------------------------
+int check_blocks(uint64_t blocks) {
+    if (blocks < (1ull << 23)) return TTP_OK;  // (fewer than 2^32 work-items)
+    return ttpi::fail(TTP_ERR_RANGE, "the product has too many tiles for one launch");
+}
+
+// f(blocks) launches the tiles of a product whose arguments are complete but for the parts' memory.
+template <class G, class Y, class F>
+int launch_parts(ttp_ctx* ctx, const ttpi::Op& op, LinearArgs& a, F&& f) {
+    const uint64_t blocks = (uint64_t)a.tiles_m * a.tiles_n * a.parts;
+    int rc = check_blocks(blocks);
+    if (rc) return rc;
+    if (a.parts > 1) {
+        a.pitch = (a.outs + 7) / 8 * 8;
+        void* ws;
+        if ((rc = ttpi::workspace(ctx, (uint64_t)a.parts * a.rows * a.pitch * 4, &ws))) return rc;
+        a.partial = (float*)ws;
+    }
     (void)hipGetLastError();
-    const dim3 grid((uint32_t)blocks), block(256);
-    if (transposed)
-        hipLaunchKernelGGL((linear_kernel<G, Y, true>), grid, block, 0, op.stream, a);
-    else
-        hipLaunchKernelGGL((linear_kernel<G, Y, false>), grid, block, 0, op.stream, a);
+    f((uint32_t)blocks);
     TTPI_HIP(hipGetLastError());
+    if (a.parts > 1) {
+        const uint32_t groups = (a.outs + 7) / 8, n = a.rows * groups;  // (parts: of few tiles)
+        hipLaunchKernelGGL((join_parts_kernel<G, Y>), dim3((n + kJoinBlock - 1) / kJoinBlock),
+                           dim3(kJoinBlock), 0, op.stream, a, groups, divider(groups));
+        TTPI_HIP(hipGetLastError());
+    }
     return TTP_OK;
+}
+
+// Whether the loads that go straight into the LDS may be used: whole 16-byte chunks on their grid,
+// and a tile's rows within 31 bits of bytes.
+bool on_grid(const LinearArgs& a, bool transposed) {
+    return ((uintptr_t)a.x | (uintptr_t)a.w) % 16 == 0 && a.x_stride % 8 == 0 &&
+           a.w_stride % 8 == 0 && a.cols % 8 == 0 && (transposed || a.outs % 8 == 0) &&
+           a.x_stride < (1u << 22) && a.w_stride < (1u << 22);
+}
+
+template <class G, class Y>
+int multiply(ttp_ctx* ctx, const ttpi::Op& op, LinearArgs a, bool transposed) {
+    constexpr bool kBf16 = sizeof(G) == 2;
+    const bool direct = kBf16 && on_grid(a, transposed);
+    const LinearCut cut = choose_linear_cut(a.rows, a.cols, a.outs, direct, kBf16, transposed,
+                                            (uint64_t)op.num_cus);
+    a.tiles_m = (uint32_t)(((uint64_t)a.rows + cut.tile_rows - 1) / cut.tile_rows);
+    a.tiles_n = (uint32_t)(((uint64_t)a.outs + cut.tile_outs - 1) / cut.tile_outs);
+    a.parts = cut.parts;
+    a.per = cut.per;
+    return launch_parts<G, Y>(ctx, op, a, [&](uint32_t blocks) {
+        if (direct) {
+            if (sizeof(Y) == 2)
+                launch_direct_to_bf16(cut.shape, transposed, blocks, op.stream, a);
+            else
+                launch_direct_to_fp32(cut.shape, transposed, blocks, op.stream, a);
+        } else if (transposed) {
+            hipLaunchKernelGGL((linear_kernel<G, Y, true>), dim3(blocks), dim3(256), 0, op.stream,
+                               a);
+        } else {
+            hipLaunchKernelGGL((linear_kernel<G, Y, false>), dim3(blocks), dim3(256), 0, op.stream,
+                               a);
+        }
+    });
 }
 
 }  // namespace
@@ -366,9 +382,9 @@ extern "C" int ttp_linear(ttp_ctx* ctx, const ttp_linear_args* args) {
         a.y_stride = y->stride;
         const bool y16 = y->dtype == TTP_DTYPE_BF16;
         if (bf16)
-            return y16 ? multiply<uint16_t, uint16_t>(op, a, args->transposed)
-                       : multiply<uint16_t, float>(op, a, args->transposed);
-        return y16 ? multiply<float, uint16_t>(op, a, args->transposed)
-                   : multiply<float, float>(op, a, args->transposed);
+            return y16 ? multiply<uint16_t, uint16_t>(ctx, op, a, args->transposed)
+                       : multiply<uint16_t, float>(ctx, op, a, args->transposed);
+        return y16 ? multiply<float, uint16_t>(ctx, op, a, args->transposed)
+                   : multiply<float, float>(ctx, op, a, args->transposed);
     });
 }

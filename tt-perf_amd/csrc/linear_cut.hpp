@@ -1,0 +1,87 @@
+// linear_cut.hpp — how a linear product is cut into tiles and parts (host code, of numbers alone).
+#pragma once
+
+#include <stdint.h>
+
+#include <algorithm>
+
+namespace ttp {
+
+// The shapes of linear_direct_kernel and the one of any alignment.
+enum class LinearShape { kThin, kSmall, kWide, kLarge, kAny };
+
+namespace {
+
+// What a tile costs, fitted to measurements: ns per step of a block that has its CU to itself, and
+// of each where as many share it as fit; ns before its first step and behind its last one.
+struct LinearCost {
+    LinearShape shape;
+    uint32_t rows, outs, step, per_cu;
+    double alone, shared, ends;
+};
+
+struct LinearCut {
+    LinearShape shape;
+    uint32_t tile_rows, tile_outs;
+    uint32_t parts, per;  // parts of the summed index, and its elements in each
+    double ns;            // what it should take
+};
+
+constexpr uint32_t kThinRows = 32;  // a token or a few: a matrix is read for them
+
+// The number of parts that should take the least time.  A part has four steps or more; parts cost
+// their fp32 sums' way to memory and back at about 5 TB/s, and a launch.
+inline LinearCut cut_parts(uint64_t rows, uint64_t cols, uint64_t outs, const LinearCost& c,
+                           uint64_t cus) {
+    LinearCut best{c.shape, c.rows, c.outs, 0, 0, 0.0};
+    const uint64_t tiles = ((rows + c.rows - 1) / c.rows) * ((outs + c.outs - 1) / c.outs);
+    const uint64_t steps = (cols + c.step - 1) / c.step, slots = c.per_cu * cus;
+    const uint64_t most =
+        tiles >= slots ? 1 : std::max<uint64_t>(std::min<uint64_t>(steps / 4, 32), 1);
+    for (uint64_t n = 1; n <= most; ++n) {
+        const uint64_t per = (steps + n - 1) / n, parts = (steps + per - 1) / per;
+        const uint64_t blocks = tiles * parts, left = blocks % slots;
+        double ns = (double)(blocks / slots) * (c.shared * (double)per + c.ends);
+        if (left) {  // (as they are dealt out: some CUs have one more)
+            const double share =
+                left <= cus ? 0.0 : (double)(left - cus) / (double)(slots - cus);
+            ns += (c.alone + (c.shared - c.alone) * share) * (double)per + c.ends;
+        }
+        if (parts > 1) ns += 4000.0 + 8.0 * (double)parts * (double)rows * (double)outs / 5e3;
+        if (n == 1 || ns < best.ns) {
+            best.ns = ns;
+            best.parts = (uint32_t)parts;
+            best.per = (uint32_t)(per * c.step);
+        }
+    }
+    return best;
+}
+
+// The fastest shape of those that the operands allow.
+// Measured, bf16, us (W as it is / transposed): 8192 x 1280 x 5120 large 134 / 126, wide 117 / 127,
+// small 124 / 124, any alignment 167; 8192 x 5120 x 1280 large 100 / 89, wide 122 / 141, small 131 /
+// 125, any 181; 4096 x 1600 x 6400 large 108, wide 95, small 103; 100 x 5120 x 1280 small 56 in one
+// part, 17 in 4 and 16 in 8.
+inline LinearCut choose_linear_cut(uint64_t rows, uint64_t cols, uint64_t outs, bool direct,
+                                   bool bf16, bool transposed, uint64_t cus) {
+    using S = LinearShape;
+    if (!direct) {
+        const LinearCost any = bf16 ? LinearCost{S::kAny, 128, 128, 32, 2, 380.0, 680.0, 5000.0}
+                                    : LinearCost{S::kAny, 128, 128, 32, 1, 2000.0, 2000.0, 5000.0};
+        return cut_parts(rows, cols, outs, any, cus);
+    }
+    if (rows <= kThinRows)
+        return cut_parts(rows, cols, outs, {S::kThin, 32, 64, 64, 3, 150.0, 700.0, 4000.0}, cus);
+    LinearCut best =
+        cut_parts(rows, cols, outs, {S::kSmall, 128, 128, 64, 2, 540.0, 970.0, 5500.0}, cus);
+    for (const LinearCost& c :
+         {LinearCost{S::kWide, 128, 256, 32, 2, 450.0, transposed ? 1100.0 : 980.0, 7000.0},
+          LinearCost{S::kLarge, 256, 160, 64, 1, 1050.0, 1050.0, 12000.0}}) {
+        const LinearCut cut = cut_parts(rows, cols, outs, c, cus);
+        if (cut.ns < best.ns) best = cut;
+    }
+    return best;
+}
+
+}  // namespace
+}  // namespace ttp
