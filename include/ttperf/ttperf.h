@@ -647,7 +647,8 @@ int ttp_embedding(ttp_ctx* ctx, uint32_t table, const int64_t* tokens, double sc
 /* The table's gradient: row v (+)= scale times the sum of dy's rows whose token is v, in the order
  * of the rows, into the store's gradient as ttp_accumulate_grad puts it (no gradient yet: the
  * other rows become 0; else they are left as they are).  Tokens outside the table are passed
- * over.  dy of either type. */
+ * over.  dy of either type.  Tables of fewer than 2^30 rows; rows of dy / 16 times its columns / 256,
+ * each rounded up, below 2^25. */
 int ttp_accumulate_embedding_grad(ttp_ctx* ctx, uint32_t table, const int64_t* tokens, double scale,
                                   const ttp_matrix* dy);
 
