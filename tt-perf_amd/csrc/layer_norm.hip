@@ -3,7 +3,7 @@
 //   m = mean x,  r = 1 / sqrt(mean (x - m)^2 + eps),  y = (x - m) r w + b
 //   h = (x - m) r,  g = dy w,  dx = add + r (g - mean g - h mean(g h)),  dw = sum dy h,  db = sum dy
 //
-// Bound by memory.  A row of up to 2048 columns is a wave's, one of up to 8192 a block's of four:
+// Bound by memory.  A row of up to 1536 columns is a wave's, one of up to 8192 a block's:
 // it is read once, into registers, and its sums are taken there (the variance from the differences,
 // not from the squares, whose difference would lose what a mean far from 0 shares).  Longer rows are
 // read again for each sum.  The backward keeps the weight's and the bias's sums of its rows in
@@ -12,6 +12,7 @@
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "columns8.hpp"
 #include "context.hpp"
@@ -98,31 +99,112 @@ struct NormArgs {
 };
 
 // ---- rows in registers ------------------------------------------------------------------------
+// A lane's 8 columns of a step, from `first` on, of which the row's last lane may have fewer: it
+// takes the row's last 8 and counts those from `at + j >= first` on, a lane behind the row's end
+// none.  So every lane loads, without a branch, and the loads of a row are all under way before the
+// first is used.  (Rows of fewer than 8 columns, kShort, are read one by one.)
+struct Place8 {
+    uint32_t first, at;
+    __device__ __forceinline__ bool has(int j) const { return at + j >= first; }
+};
+__device__ __forceinline__ Place8 place8(uint32_t first, uint32_t cols) {
+    return {first, min(first, max(cols, 8u) - 8)};
+}
+template <class T>
+struct Raw8 {
+    u32x4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (uint32_t k = 0; k < sizeof(T) / 2; ++k) w[k] = load16(p + k * kPer<T>);
+    }
+    __device__ __forceinline__ void load_some(const T* p, uint32_t n) {  // the first n, then 0
+        float v[8];
+        load_cols(p, 0, n, v);
+#pragma unroll
+        for (uint32_t k = 0; k < sizeof(T) / 2; ++k) {
+            float q[kPer<T>];
+#pragma unroll
+            for (int j = 0; j < kPer<T>; ++j) q[j] = v[k * kPer<T> + j];
+            w[k] = pack(q, p);
+        }
+    }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+#pragma unroll
+        for (uint32_t k = 0; k < sizeof(T) / 2; ++k) {
+            float q[kPer<T>];
+            unpack(w[k], q, (const T*)nullptr);
+#pragma unroll
+            for (int j = 0; j < kPer<T>; ++j) v[k * kPer<T> + j] = q[j];
+        }
+    }
+};
+template <bool kShort, class T>
+__device__ __forceinline__ void load_place(Raw8<T>& r, const T* row, Place8 p, uint32_t cols) {
+    if constexpr (kShort)
+        r.load_some(row, p.first ? 0u : cols);
+    else
+        r.load(row + p.at);
+}
+template <bool kShort, class T>
+__device__ __forceinline__ void store_place(T* row, Place8 p, uint32_t cols, const float (&v)[8]) {
+    if (!kShort && p.first + 8 <= cols) {
+        store_cols(row, p.first, cols, v);
+    } else if (p.first < cols) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (p.has(j) && p.at + j < cols) narrow(v[j], row + p.at + j);
+    }
+}
+// The same of a vector of parameters (null: none).
+template <bool kShort, class W>
+__device__ __forceinline__ void load_param(Raw8<W>& r, const Vector& p, Place8 at, uint32_t cols) {
+    if (p.data) load_place<kShort>(r, (const W*)p.data, at, cols);
+}
+template <class W>
+__device__ __forceinline__ void param_values(const Raw8<W>& r, const Vector& p, float (&v)[8]) {
+    if (p.data) {
+        r.values(v);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = p.otherwise;
+    }
+}
+
 // kWaves waves have a row of up to kC steps of 512 kWaves columns.
-template <class T, class Y, int kWaves, int kC>
-__global__ __launch_bounds__(256) void norm_kernel(NormArgs a) {
-    __shared__ float lds[4];
-    const uint32_t lane = kWaves == 1 ? threadIdx.x & 63 : threadIdx.x;
+template <class T, class Y, class W, int kWaves, int kC, bool kShort>
+__global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void norm_kernel(NormArgs a) {
+    __shared__ float lds[kWaves];
+    const uint32_t lane = kWaves == 1 ? threadIdx.x & 63 : threadIdx.x, cols = a.cols;
     const uint64_t row =
         kWaves == 1 ? (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (uint64_t)blockIdx.x;
     if (row >= a.rows) return;  // (a wave, or the block, together)
+    const auto place = [&](int k) { return place8((k * 64 * kWaves + lane) * 8, cols); };
     const T* x = (const T*)a.x + row * a.x_stride;
+    Raw8<T> raw[kC];
+    Raw8<W> weight[kC], bias[kC];
+#pragma unroll
+    for (int k = 0; k < kC; ++k) load_place<kShort>(raw[k], x, place(k), cols);
+#pragma unroll
+    for (int k = 0; k < kC; ++k) load_param<kShort>(weight[k], a.weight, place(k), cols);
+#pragma unroll
+    for (int k = 0; k < kC; ++k) load_param<kShort>(bias[k], a.bias, place(k), cols);
     float v[kC][8];
     float s[1] = {0.0f};
 #pragma unroll
     for (int k = 0; k < kC; ++k) {
-        load_cols(x, (k * 64 * kWaves + lane) * 8, a.cols, v[k]);
+        raw[k].values(v[k]);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[0] += v[k][j];
+        for (int j = 0; j < 8; ++j) s[0] += place(k).has(j) ? v[k][j] : 0.0f;
     }
     row_sums<kWaves>(s, lds);
-    const float n = (float)a.cols, m = s[0] / n;
+    const float n = (float)cols, m = s[0] / n;
     s[0] = 0.0f;
 #pragma unroll
     for (int k = 0; k < kC; ++k)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            v[k][j] = (k * 64 * kWaves + lane) * 8 + j < a.cols ? v[k][j] - m : 0.0f;
+            const bool in = place(k).has(j) && (!kShort || j < (int)cols);
+            v[k][j] = in ? v[k][j] - m : 0.0f;
             s[0] += v[k][j] * v[k][j];
         }
     row_sums<kWaves>(s, lds);
@@ -134,105 +216,142 @@ __global__ __launch_bounds__(256) void norm_kernel(NormArgs a) {
     Y* y = (Y*)a.out + row * a.out_stride;
 #pragma unroll
     for (int k = 0; k < kC; ++k) {
-        const uint32_t c = (k * 64 * kWaves + lane) * 8;
-        if (c >= a.cols) break;
         float w[8], b[8];
-        load_vector(a.weight, c, a.cols, w);
-        load_vector(a.bias, c, a.cols, b);
+        param_values(weight[k], a.weight, w);
+        param_values(bias[k], a.bias, b);
 #pragma unroll
         for (int j = 0; j < 8; ++j) w[j] = v[k][j] * r * w[j] + b[j];
-        store_cols(y, c, a.cols, w);
+        store_place<kShort>(y, place(k), cols, w);
     }
 }
 
-// Rows of this block: a wave each (kWaves 1: eight waves), or the four waves' together.
-template <class T, class G, int kWaves, int kC>
-__global__ __launch_bounds__(kWaves == 1 ? 512 : 256) void norm_backward_kernel(NormArgs a,
-                                                                                uint64_t per) {
-    constexpr uint32_t kRows = kWaves == 1 ? 8 : 1;  // at a time
-    __shared__ float lds[kWaves == 1 ? 2 * kC * kWaveCols : 8];
-    const uint32_t lane = kWaves == 1 ? threadIdx.x & 63 : threadIdx.x;
+// Rows of this block: a wave each (kWaves 1), or all its waves' together; the next row's loads are
+// under way while a row is worked on.  A row's x and dy stay in their own type and are widened again
+// for dx, which leaves registers for that.
+constexpr int kBackwardWaves = 8;
+template <class T, class G, class W, int kWaves, int kC, bool kShort>
+__global__ __launch_bounds__(64 * (kWaves == 1 ? kBackwardWaves : kWaves))
+void norm_backward_kernel(NormArgs a, uint64_t per) {
+    constexpr uint32_t kRows = kWaves == 1 ? kBackwardWaves : 1;  // at a time
+    constexpr uint32_t kHalf = kRows / 2, kSums = kC * kWaveCols;
+    __shared__ float lds[kWaves == 1 ? kHalf * 2 * kSums : 2 * kWaves];
+    const uint32_t lane = kWaves == 1 ? threadIdx.x & 63 : threadIdx.x, cols = a.cols;
     const uint32_t wave = kWaves == 1 ? threadIdx.x >> 6 : 0;
     const uint64_t first = blockIdx.x * per, end = min(first + per, a.rows);
-    const float n = (float)a.cols;
-    float w[kC][8], sum_w[kC][8], sum_b[kC][8];
+    const float n = (float)cols;
+    const auto place = [&](int k) { return place8((k * 64 * kWaves + lane) * 8, cols); };
+    struct Row {
+        Raw8<T> x[kC];
+        Raw8<G> dy[kC];
+        float m, r;
+    } next;
+    const auto load_row = [&](uint64_t row) {
+        next.m = a.mean[row];
+        next.r = a.rstd[row];
+#pragma unroll
+        for (int k = 0; k < kC; ++k) {
+            load_place<kShort>(next.x[k], (const T*)a.x + row * a.x_stride, place(k), cols);
+            load_place<kShort>(next.dy[k], (const G*)a.in + row * a.in_stride, place(k), cols);
+        }
+    };
+    if (first + wave < end) load_row(first + wave);
+    Raw8<W> weight[kC];
+    float sum_w[kC][8], sum_b[kC][8];
 #pragma unroll
     for (int k = 0; k < kC; ++k) {
-        load_vector(a.weight, (k * 64 * kWaves + lane) * 8, a.cols, w[k]);
+        load_param<kShort>(weight[k], a.weight, place(k), cols);
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum_w[k][j] = sum_b[k][j] = 0.0f;
     }
     for (uint64_t row = first + wave; row < end; row += kRows) {
-        const T* x = (const T*)a.x + row * a.x_stride;
-        const G* dy = (const G*)a.in + row * a.in_stride;
-        const float m = a.mean[row], r = a.rstd[row];
-        float h[kC][8], g[kC][8], s[2] = {0.0f, 0.0f};
+        const Row now = next;
+        Raw8<T> add[kC];
+        if (a.add)
+#pragma unroll
+            for (int k = 0; k < kC; ++k)
+                load_place<kShort>(add[k], (const T*)a.add + row * a.add_stride, place(k), cols);
+        if (row + kRows < end) load_row(row + kRows);
+        // h and dy of step k, 0 where they are another lane's
+        const auto widen_step = [&](int k, float(&h)[8], float(&g)[8]) {
+            now.x[k].values(h);
+            now.dy[k].values(g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const bool in = place(k).has(j) && (!kShort || j < (int)cols);
+                h[j] = in ? (h[j] - now.m) * now.r : 0.0f;
+                g[j] = in ? g[j] : 0.0f;
+            }
+        };
+        float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < kC; ++k) {
-            const uint32_t c = (k * 64 * kWaves + lane) * 8;
-            load_cols(x, c, a.cols, h[k]);
-            load_cols(dy, c, a.cols, g[k]);
-        }
+            float h[8], g[8], w[8];
+            widen_step(k, h, g);
+            param_values(weight[k], a.weight, w);
 #pragma unroll
-        for (int k = 0; k < kC; ++k)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {  // (past the row's end dy is 0)
-                const bool in = (k * 64 * kWaves + lane) * 8 + j < a.cols;
-                h[k][j] = in ? (h[k][j] - m) * r : 0.0f;
-                sum_w[k][j] += g[k][j] * h[k][j];
-                sum_b[k][j] += g[k][j];
-                g[k][j] = in ? g[k][j] * w[k][j] : 0.0f;
-                s[0] += g[k][j];
-                s[1] += g[k][j] * h[k][j];
+            for (int j = 0; j < 8; ++j) {
+                sum_w[k][j] += g[j] * h[j];
+                sum_b[k][j] += g[j];
+                g[j] *= w[j];
+                s[0] += g[j];
+                s[1] += g[j] * h[j];
             }
+        }
         row_sums<kWaves>(s, lds);
         const float mean_g = s[0] / n, mean_gh = s[1] / n;
         T* dx = (T*)a.out + row * a.out_stride;
 #pragma unroll
         for (int k = 0; k < kC; ++k) {
-            const uint32_t c = (k * 64 * kWaves + lane) * 8;
-            if (c >= a.cols) break;
-            float o[8];
-            if (a.add) {
-                load_cols((const T*)a.add + row * a.add_stride, c, a.cols, o);
-            } else {
+            float h[8], g[8], w[8], o[8] = {};
+            widen_step(k, h, g);
+            param_values(weight[k], a.weight, w);
+            if (a.add) add[k].values(o);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = 0.0f;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) o[j] += r * (g[k][j] - mean_g - h[k][j] * mean_gh);
-            store_cols(dx, c, a.cols, o);
+            for (int j = 0; j < 8; ++j)
+                o[j] += now.r * (g[j] * w[j] - mean_g - h[j] * mean_gh);
+            store_place<kShort>(dx, place(k), cols, o);
         }
     }
-    float* part = a.parts + (uint64_t)blockIdx.x * 2 * a.cols;
-    if constexpr (kWaves == 1) {  // the waves' sums, in order
-        float* of_b = lds + kC * kWaveCols;
-        for (uint32_t t = 0; t < kRows; ++t) {
-            if (wave == t)
+    // (a lane's sums are of its columns from Place8::at on; those of another lane are 0)
+    float* part = a.parts + (uint64_t)blockIdx.x * 2 * cols;
+    if constexpr (kWaves == 1) {  // one half of the waves' sums, the other half's added, then in order
+#pragma unroll
+        for (uint32_t half = 0; half < 2; ++half) {
+            if (wave / kHalf == half)
 #pragma unroll
                 for (int k = 0; k < kC; ++k)
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const uint32_t at = k * kWaveCols + j * 64 + lane;  // a column's place
-                        lds[at] = t ? lds[at] + sum_w[k][j] : sum_w[k][j];
-                        of_b[at] = t ? of_b[at] + sum_b[k][j] : sum_b[k][j];
+                        float* p = lds + (wave % kHalf) * 2 * kSums + (k * 8 + j) * 64 + lane;
+                        p[0] = half ? p[0] + sum_w[k][j] : sum_w[k][j];
+                        p[kSums] = half ? p[kSums] + sum_b[k][j] : sum_b[k][j];
                     }
             __syncthreads();
         }
-        for (uint32_t c = threadIdx.x; c < a.cols; c += 512) {
-            const uint32_t at = c / kWaveCols * kWaveCols + c % 8 * 64 + c % kWaveCols / 8;
-            part[c] = lds[at];
-            part[a.cols + c] = of_b[at];
+        for (uint32_t c = threadIdx.x; c < cols; c += 64 * kRows) {
+            // column c is its lane's j-th, counted from where that lane's 8 begin
+            const uint32_t k = c / kWaveCols, l = c % kWaveCols / 8;
+            const uint32_t j = c - place8(c / 8 * 8, cols).at;
+            const float* p = lds + (k * 8 + j) * 64 + l;
+            float w = p[0], b = p[kSums];
+#pragma unroll
+            for (uint32_t t = 1; t < kHalf; ++t) {
+                w += p[t * 2 * kSums];
+                b += p[t * 2 * kSums + kSums];
+            }
+            part[c] = w;
+            part[cols + c] = b;
         }
     } else {
 #pragma unroll
         for (int k = 0; k < kC; ++k)
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const uint32_t c = (k * 64 * kWaves + lane) * 8 + j;
-                if (c < a.cols) {
+                const Place8 p = place(k);
+                const uint32_t c = p.at + j;
+                if (p.first < cols && p.has(j) && c < cols) {
                     part[c] = sum_w[k][j];
-                    part[a.cols + c] = sum_b[k][j];
+                    part[cols + c] = sum_b[k][j];
                 }
             }
     }
@@ -370,9 +489,17 @@ __global__ __launch_bounds__(1024) void join_columns_kernel(JoinArgs a) {
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint64_t c = (uint64_t)blockIdx.x * 64 + lane, all = 2ull * a.cols;
     const uint32_t per = (a.n + 15) / 16, end = min((wave + 1) * per, a.n);
+    const float* p = a.parts + min(c, all - 1);
     float v = 0.0f;
-    if (c < all)
-        for (uint32_t k = wave * per; k < end; ++k) v += a.parts[k * all + c];
+    uint32_t k = wave * per;
+    for (; k + 8 <= end; k += 8) {
+        float w[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = p[(k + j) * all];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v += w[j];
+    }
+    for (; k < end; ++k) v += p[k * all];
     lds[wave][lane] = v;
     __syncthreads();
     if (wave || c >= all) return;
@@ -389,28 +516,30 @@ __global__ __launch_bounds__(1024) void join_columns_kernel(JoinArgs a) {
 constexpr uint32_t kLongCols = 8192;  // rows longer than that are not kept in registers
 constexpr uint64_t kMostCols = 1u << 24;
 
-// f(waves of a row, steps): the shape that holds a row of `cols` <= kLongCols
+// f(waves of a row, steps, whether it is short): the shape that holds a row of `cols` <= kLongCols
 template <class F>
 void with_shape(uint32_t cols, F&& f) {
     using std::integral_constant;
-    if (cols <= kWaveCols)
-        f(integral_constant<int, 1>(), integral_constant<int, 1>());
+    if (cols < 8)
+        f(integral_constant<int, 1>(), integral_constant<int, 1>(), std::true_type());
+    else if (cols <= kWaveCols)
+        f(integral_constant<int, 1>(), integral_constant<int, 1>(), std::false_type());
     else if (cols <= 2 * kWaveCols)
-        f(integral_constant<int, 1>(), integral_constant<int, 2>());
+        f(integral_constant<int, 1>(), integral_constant<int, 2>(), std::false_type());
     else if (cols <= 3 * kWaveCols)
-        f(integral_constant<int, 1>(), integral_constant<int, 3>());
+        f(integral_constant<int, 1>(), integral_constant<int, 3>(), std::false_type());
     else if (cols <= 4 * kWaveCols)
-        f(integral_constant<int, 1>(), integral_constant<int, 4>());
+        f(integral_constant<int, 4>(), integral_constant<int, 1>(), std::false_type());
     else if (cols <= 8 * kWaveCols)
-        f(integral_constant<int, 4>(), integral_constant<int, 2>());
+        f(integral_constant<int, 8>(), integral_constant<int, 1>(), std::false_type());
     else
-        f(integral_constant<int, 4>(), integral_constant<int, 4>());
+        f(integral_constant<int, 8>(), integral_constant<int, 2>(), std::false_type());
 }
 
 // A launch has fewer than 2^32 work-items: f(first row, rows) over ranges of rows.
 template <class F>
 int for_row_ranges(uint64_t rows, F&& f) {
-    constexpr uint64_t kMost = (1u << 24) - 4;  // of 256 lanes each
+    constexpr uint64_t kMost = (1u << 23) - 8;  // of up to 512 lanes each
     for (uint64_t r = 0; r < rows; r += kMost) {
         (void)hipGetLastError();
         f(r, std::min(kMost, rows - r));
@@ -431,7 +560,7 @@ NormArgs from_row(NormArgs a, uint64_t r, uint64_t rows) {
     return a;
 }
 
-template <class T, class Y>
+template <class T, class Y, class W>
 int norm_rows(const ttpi::Op& op, const NormArgs& all) {
     return for_row_ranges(all.rows, [&](uint64_t r, uint64_t rows) {
         const NormArgs a = from_row<T, T, Y>(all, r, rows);
@@ -440,10 +569,11 @@ int norm_rows(const ttpi::Op& op, const NormArgs& all) {
                                op.stream, a);
             return;
         }
-        with_shape(a.cols, [&](auto waves, auto steps) {
+        with_shape(a.cols, [&](auto waves, auto steps, auto is_short) {
             const uint64_t blocks = waves == 1 ? (rows + 3) / 4 : rows;
-            hipLaunchKernelGGL((norm_kernel<T, Y, waves(), steps()>), dim3((uint32_t)blocks),
-                               dim3(256), 0, op.stream, a);
+            hipLaunchKernelGGL((norm_kernel<T, Y, W, waves(), steps(), is_short()>),
+                               dim3((uint32_t)blocks), dim3(waves == 1 ? 256 : 64 * waves), 0,
+                               op.stream, a);
         });
     });
 }
@@ -458,18 +588,18 @@ Parts parts_of(const ttpi::Op& op, uint64_t rows, uint32_t cols) {
     if (cols > kLongCols) {
         const uint64_t tiles = ((uint64_t)cols + 2047) / 2048;
         n = std::max<uint64_t>(4 * (uint64_t)op.num_cus / tiles, 1);
-    } else if (cols > 4 * kWaveCols) {
+    } else if (cols > 3 * kWaveCols) {
         n = 2 * (uint64_t)op.num_cus;
     } else {
         n = (uint64_t)op.num_cus;
-        step = 8;  // a row for each of the block's waves
+        step = kBackwardWaves;  // a row for each of the block's waves
     }
     const uint64_t per = std::max<uint64_t>((rows + n - 1) / n, 1);
     const uint64_t whole = (per + step - 1) / step * step;
     return {(uint32_t)((rows + whole - 1) / whole), whole};
 }
 
-template <class T, class G>
+template <class T, class G, class W>
 int norm_backward_rows(const ttpi::Op& op, const NormArgs& a, const Parts& p) {
     (void)hipGetLastError();
     if (a.cols > kLongCols) {
@@ -483,13 +613,27 @@ int norm_backward_rows(const ttpi::Op& op, const NormArgs& a, const Parts& p) {
         });
         if (rc) return rc;
     } else {
-        with_shape(a.cols, [&](auto waves, auto steps) {
-            hipLaunchKernelGGL((norm_backward_kernel<T, G, waves(), steps()>), dim3(p.n),
-                               dim3(waves == 1 ? 512 : 256), 0, op.stream, a, p.per);
+        with_shape(a.cols, [&](auto waves, auto steps, auto is_short) {
+            hipLaunchKernelGGL((norm_backward_kernel<T, G, W, waves(), steps(), is_short()>),
+                               dim3(p.n), dim3(64 * (waves == 1 ? kBackwardWaves : waves())), 0,
+                               op.stream, a, p.per);
         });
     }
     TTPI_HIP(hipGetLastError());
     return TTP_OK;
+}
+
+// f(a value of x's type, of y's or dy's, of the parameters')
+template <class F>
+int with_types(int x, int y, bool params_bf16, F&& f) {
+    const uint16_t h = 0;
+    const float s = 0.0f;
+    const auto with_params = [&](auto t, auto g) {
+        return params_bf16 ? f(t, g, h) : f(t, g, s);
+    };
+    if (x == TTP_DTYPE_BF16)
+        return y == TTP_DTYPE_BF16 ? with_params(h, h) : with_params(h, s);
+    return y == TTP_DTYPE_BF16 ? with_params(s, h) : with_params(s, s);
 }
 
 int check_cols(uint64_t cols) {
@@ -549,10 +693,10 @@ int ttp_layer_norm(ttp_ctx* ctx, uint32_t weight, uint32_t bias, const ttp_matri
         a.out_stride = y->stride;
         a.mean = mean;
         a.rstd = rstd;
-        const bool bf16 = y->dtype == TTP_DTYPE_BF16;
-        if (x->dtype == TTP_DTYPE_BF16)
-            return bf16 ? norm_rows<uint16_t, uint16_t>(op, a) : norm_rows<uint16_t, float>(op, a);
-        return bf16 ? norm_rows<float, uint16_t>(op, a) : norm_rows<float, float>(op, a);
+        return with_types(x->dtype, y->dtype, a.weight.bf16 || a.bias.bf16,
+                          [&](auto t, auto g, auto w) {
+                              return norm_rows<decltype(t), decltype(g), decltype(w)>(op, a);
+                          });
     });
 }
 
@@ -611,13 +755,9 @@ int ttp_layer_norm_backward(ttp_ctx* ctx, uint32_t weight, uint32_t bias, const 
         if (p.n && (rc = ttpi::workspace(ctx, (uint64_t)p.n * 2 * cols * 4, &ws))) return rc;
         a.parts = (float*)ws;
         if (p.n) {
-            const bool bf16 = dy->dtype == TTP_DTYPE_BF16;
-            if (x->dtype == TTP_DTYPE_BF16)
-                rc = bf16 ? norm_backward_rows<uint16_t, uint16_t>(op, a, p)
-                          : norm_backward_rows<uint16_t, float>(op, a, p);
-            else
-                rc = bf16 ? norm_backward_rows<float, uint16_t>(op, a, p)
-                          : norm_backward_rows<float, float>(op, a, p);
+            rc = with_types(x->dtype, dy->dtype, a.weight.bf16, [&](auto t, auto g, auto w) {
+                return norm_backward_rows<decltype(t), decltype(g), decltype(w)>(op, a, p);
+            });
             if (rc) return rc;
         }
         if (has_weight || has_bias) {
