@@ -508,7 +508,7 @@ int table_param(ttp_ctx* ctx, ttpi::Buffers& b, uint32_t index, uint64_t cols, c
         return ttpi::fail(TTP_ERR_RANGE, "tensor " + std::to_string(index) + " has " +
                                              std::to_string(p->numel) + " elements, not rows of " +
                                              std::to_string(cols));
-    return b.array(p->data, p->numel, p->bf16 ? 2 : 4, what, false);
+    return b.own(p->data, p->numel, p->bf16 ? 2 : 4, what, false);
 }
 
 int check_scale(double scale) {
@@ -583,7 +583,7 @@ int ttp_accumulate_embedding_grad(ttp_ctx* ctx, uint32_t table, const int64_t* t
         ttpi::Buffers b(ctx);
         if ((rc = b.array(tokens, rows, 8, "the tokens", false))) return rc;
         if ((rc = b.matrix(dy, rows, cols, "the output's gradient", false))) return rc;
-        if ((rc = b.array(g.data, g.numel, g.bf16 ? 2 : 4, "the table's gradient", true)))
+        if ((rc = b.own(g.data, g.numel, g.bf16 ? 2 : 4, "the table's gradient", true)))
             return rc;
         GradArgs a{};
         a.tokens = tokens;

@@ -654,7 +654,7 @@ int vector_param(ttp_ctx* ctx, ttpi::Buffers& b, uint32_t index, uint64_t cols, 
                                              std::to_string(p.numel) + " elements, not " +
                                              std::to_string(cols));
     *out = {p.data, p.bf16, otherwise};
-    return b.array(p.data, cols, p.bf16 ? 2 : 4, what, false);
+    return b.own(p.data, cols, p.bf16 ? 2 : 4, what, false);
 }
 
 }  // namespace
@@ -727,9 +727,9 @@ int ttp_layer_norm_backward(ttp_ctx* ctx, uint32_t weight, uint32_t bias, const 
         if ((rc = vector_param(ctx, b, weight, cols, 1.0f, "the weight", &a.weight))) return rc;
         if ((rc = vector_param(ctx, b, bias, cols, 0.0f, "the bias", &ignored))) return rc;
         const uint64_t size = w.bf16 || s.bf16 ? 2 : 4;
-        if (has_weight && (rc = b.array(w.data, cols, size, "the weight's gradient", true)))
+        if (has_weight && (rc = b.own(w.data, cols, size, "the weight's gradient", true)))
             return rc;
-        if (has_bias && (rc = b.array(s.data, cols, size, "the bias's gradient", true))) return rc;
+        if (has_bias && (rc = b.own(s.data, cols, size, "the bias's gradient", true))) return rc;
         const ttp_matrix* place = !dx                            ? x
                                   : add && dx->data == add->data ? add
                                   : dy->data == dx->data         ? dy

@@ -63,7 +63,9 @@ __device__ __forceinline__ bf16x8 finite(bf16x8 v) {
 }
 
 // ---- operands of any alignment, through registers ---------------------------------------------
-// 128 x 128 of y per block, 32 of the summed index per step, through two LDS buffers.
+// 128 x 128 of y per block, 32 of the summed index per step; bf16 through two LDS buffers, the three
+// parts of fp32 through one, so that two blocks share a CU and one's products run beside the other's
+// splitting (3585 x 384 x 1536: 56 us with two buffers and one block, 44 now).
 constexpr uint32_t kTile = 128, kStep = 32;
 constexpr int kPitchK = kStep + 8;  // LDS rows along the summed index, padded against conflicts
 constexpr int kPitchN = kTile + 32;
@@ -75,14 +77,15 @@ __device__ __forceinline__ bf16x8 row_fragment(const short* lds, int n, int f) {
 }
 
 template <class G, class Y, bool kTransposed>
-__global__ __launch_bounds__(256) void linear_kernel(LinearArgs a) {
+__global__ __launch_bounds__(256, 2) void linear_kernel(LinearArgs a) {
     constexpr int kPlanes = sizeof(G) == 2 ? 1 : 3;
     constexpr int kSizeA = kTile * kPitchK;
     constexpr int kSizeB = kTransposed ? kTile * kPitchK : kStep * kPitchN;
     constexpr int kBuffer = kPlanes * (kSizeA + kSizeB);
     constexpr int kOutPitch = 36;  // floats; a wave's 32 x 32 of y on its way out
-    static_assert(2 * kBuffer * 2 >= 4 * 32 * kOutPitch * 4);
-    __shared__ __align__(16) short lds[2 * kBuffer];
+    constexpr int kBuffers = kPlanes == 1 ? 2 : 1;
+    static_assert(kBuffers * kBuffer * 2 >= 4 * 32 * kOutPitch * 4);
+    __shared__ __align__(16) short lds[kBuffers * kBuffer];
 
     uint32_t id = xcd_order(blockIdx.x, gridDim.x);
     const uint32_t part = id / (a.tiles_m * a.tiles_n);
@@ -99,7 +102,29 @@ __global__ __launch_bounds__(256) void linear_kernel(LinearArgs a) {
     struct Loads {
         Chunk8<G> a[2], b[2];
     };
+    // Whole steps load without a branch: rows and columns past the end are any there are, as they only
+    // reach sums that are not written; a row's last chunk of W as it is reaches into the next row,
+    // where there is one.  (With a branch for each chunk of the tiles at the edges, whose loads then
+    // wait for each other, 500 x 2176 x 4726 took 163 us, now 44.)
+    const auto whole = [&](uint32_t k0) {
+        return k0 + kStep <= end &&
+               (kTransposed || a.outs % 8 == 0 || (a.outs >= 8 && k0 + kStep < a.cols));
+    };
+    const uint32_t column = n0 + nn < a.outs ? n0 + nn : 0;
     const auto load = [&](Loads& l, uint32_t k0) {
+        if (whole(k0)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t m = min(m0 + rr + 64 * h, a.rows - 1);
+                l.a[h].load((const G*)a.x + m * a.x_stride + k0 + rk);
+                if constexpr (kTransposed)
+                    l.b[h].load((const G*)a.w + min(n0 + rr + 64 * h, a.outs - 1) * a.w_stride +
+                                k0 + rk);
+                else
+                    l.b[h].load((const G*)a.w + (k0 + nk + 16 * h) * a.w_stride + column);
+            }
+            return;
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const uint32_t m = m0 + rr + 64 * h, k = k0 + rk;
@@ -180,14 +205,19 @@ __global__ __launch_bounds__(256) void linear_kernel(LinearArgs a) {
     const uint32_t first = part * a.per, steps = (end - first + kStep - 1) / kStep;
     Loads l;
     load(l, first);
-    store(l, lds);
-    __syncthreads();
+    if constexpr (kBuffers == 2) store(l, lds);
     for (uint32_t s = 0; s < steps; ++s) {
-        if (s + 1 < steps) load(l, first + (s + 1) * kStep);
-        multiply(lds + (s & 1) * kBuffer);
-        if (s + 1 < steps) store(l, lds + ((s + 1) & 1) * kBuffer);
+        if constexpr (kBuffers == 1) {
+            __syncthreads();  // the step before has been read
+            store(l, lds);
+        }
         __syncthreads();
+        if (s + 1 < steps) load(l, first + (s + 1) * kStep);
+        multiply(lds + (kBuffers == 2 ? s & 1 : 0) * kBuffer);
+        if constexpr (kBuffers == 2)
+            if (s + 1 < steps) store(l, lds + ((s + 1) & 1) * kBuffer);
     }
+    __syncthreads();
 
     // out, 32 x 32 at a time through this wave's LDS
     const uint64_t seed = a.has_dropout ? seed_of(a.dropout) : 0;
@@ -354,8 +384,8 @@ extern "C" int ttp_linear(ttp_ctx* ctx, const ttp_linear_args* args) {
                                              (w.bf16 ? "bfloat16" : "float32") + ")");
         ttpi::Buffers b(ctx);
         if ((rc = b.matrix(x, rows, cols, "the input", false))) return rc;
-        if ((rc = b.array(w.data, w.numel, bf16 ? 2 : 4, "the weight", false))) return rc;
-        if (has_bias && (rc = b.array(bias.data, outs, bf16 ? 2 : 4, "the bias", false))) return rc;
+        if ((rc = b.own(w.data, w.numel, bf16 ? 2 : 4, "the weight", false))) return rc;
+        if (has_bias && (rc = b.own(bias.data, outs, bf16 ? 2 : 4, "the bias", false))) return rc;
         if (res && (rc = b.matrix(res, rows, outs, "the residual", false))) return rc;
         if (args->dropout && args->dropout->device_seed &&
             (rc = b.array(args->dropout->device_seed, 1, 8, "the seed", false)))

@@ -67,7 +67,7 @@ inline LinearCut choose_linear_cut(uint64_t rows, uint64_t cols, uint64_t outs, 
     using S = LinearShape;
     if (!direct) {
         const LinearCost any = bf16 ? LinearCost{S::kAny, 128, 128, 32, 2, 380.0, 680.0, 5000.0}
-                                    : LinearCost{S::kAny, 128, 128, 32, 1, 2000.0, 2000.0, 5000.0};
+                                    : LinearCost{S::kAny, 128, 128, 32, 2, 1500.0, 2000.0, 5000.0};
         return cut_parts(rows, cols, outs, any, cus);
     }
     if (rows <= kThinRows)

@@ -45,6 +45,12 @@ class Buffers {
         return add({(uintptr_t)p, n * size, n * size, n * size, written, false, what});
     }
 
+    // an array of the context's own memory, whose place and size are known (asking the runtime about
+    // it takes a microsecond)
+    int own(const void* p, uint64_t n, uint64_t size, const char* what, bool written) {
+        return add({(uintptr_t)p, n * size, n * size, n * size, written, false, what});
+    }
+
     // a matrix of `rows` x `cols`; it may be exactly `same_as` (a result in its input's place)
     int matrix(const ttp_matrix* m, uint64_t rows, uint64_t cols, const char* what, bool written,
                const ttp_matrix* same_as = nullptr) {
