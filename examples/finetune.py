@@ -1,15 +1,17 @@
 """Fine-tuning a small next-token model on a ParamStore: preferences first, then a policy step.
 
 The model scores the next token from the current one: an embedding, one MLP block with a residual
-connection, and an output layer.  Its forward and backward are plain products in torch on the
-store's own weights; everything around them is the store's:
+connection, and an output layer.  All of it runs on the store's own weights:
 
+  * the embedding, the linear layers with their biases and the residual, and the inputs' gradients
+    are the store's products (embedding, linear, linear_input_grad);
   * the losses give the logits' gradient, already scaled by the store's loss scale
     (preference_loss, policy_loss; token_logprobs for the reference and the rollout's scores);
   * the backward needs each linear layer's input and GELU's: they are kept in 8 bits
     (checkpoint8, gelu_checkpoint8), a quarter of fp32 or half of bf16;
   * weight and bias gradients go from the kept inputs into the store's gradient buffer
-    (accumulate_linear_grad8), which AdamW steps with loss scaling and clipping.
+    (accumulate_linear_grad8), the embedding's from its tokens (accumulate_embedding_grad), and
+    AdamW steps them with loss scaling and clipping.
 
 Run: python examples/finetune.py [--steps N]
 """
@@ -42,36 +44,33 @@ class Model:
         for t, s in zip(self.store.tensors, shapes):
             if len(s) == 2:
                 t.set_data((torch.randn(s, generator=gen) * s[0] ** -0.5).numpy())
-        # the weights the forward reads: views of the store's bf16 copies
+        # views of the bf16 weights that the forward reads
         self.w = [t.torch_view() for t in self.store.tensors]
 
     def forward(self, tokens, keep=True):
         """Logits (tokens, vocab), and what the backward needs, in 8 bits."""
-        store, w = self.store, self.w
-        e = w[EMB][tokens]
-        h = torch.addmm(w[B1], e, w[W1])
-        if not keep:
+        store = self.store
+        e = store.embedding(EMB, tokens)
+        h = store.linear(W1, e, bias=B1)
+        if not keep:  # (GELU on the same rounded h: a reference gives the model's own scores)
             a = torch.nn.functional.gelu(h, approximate="tanh")
-            y = e + torch.addmm(w[B2], a, w[W2])
-            return torch.addmm(w[BO], y, w[WO]), None
+            return store.linear(WO, store.linear(W2, a, bias=B2, residual=e), bias=BO), None
         a, h8 = store.gelu_checkpoint8(h, fmt=self.fmt, approximate="tanh")
-        y = e + torch.addmm(w[B2], a, w[W2])
+        y = store.linear(W2, a, bias=B2, residual=e)
         kept = (tokens, store.checkpoint8(e, fmt=self.fmt), h8,
                 store.checkpoint8(a, fmt=self.fmt), store.checkpoint8(y, fmt=self.fmt))
-        return torch.addmm(w[BO], y, w[WO]), kept
+        return store.linear(WO, y, bias=BO), kept
 
     def backward(self, grad, kept):
         """The gradients of all weights into the store, from the logits'."""
-        store, w = self.store, self.w
+        store = self.store
         tokens, e8, h8, a8, y8 = kept
         store.accumulate_linear_grad8(WO, y8, grad, bias=BO)
-        dy = grad @ w[WO].t().contiguous()
+        dy = store.linear_input_grad(WO, grad)
         store.accumulate_linear_grad8(W2, a8, dy, bias=B2)
-        dh = store.gelu_backward8(h8, dy @ w[W2].t().contiguous(), approximate="tanh")
+        dh = store.gelu_backward8(h8, store.linear_input_grad(W2, dy), approximate="tanh")
         store.accumulate_linear_grad8(W1, e8, dh, bias=B1)
-        de = dy + dh @ w[W1].t().contiguous()
-        demb = torch.zeros(w[EMB].shape, device=de.device)
-        store.accumulate_grad(EMB, demb.index_add_(0, tokens, de.float()))
+        store.accumulate_embedding_grad(EMB, tokens, store.linear_input_grad(W1, dh, add=dy))
 
 
 def sequences(count, length, vocab, gen):
