@@ -63,9 +63,10 @@ __device__ __forceinline__ bf16x8 finite(bf16x8 v) {
 }
 
 // ---- operands of any alignment, through registers ---------------------------------------------
-// 128 x 128 of y per block, 32 of the summed index per step; bf16 through two LDS buffers, the three
-// parts of fp32 through one, so that two blocks share a CU and one's products run beside the other's
-// splitting (3585 x 384 x 1536: 56 us with two buffers and one block, 44 now).
+// 128 x 128 of y per block of four waves, 32 of the summed index per step; bf16 through two LDS
+// buffers, the three parts of fp32 through one, so that two blocks share a CU and one's products run
+// beside the other's splitting (3585 x 384 x 1536: 56 us with two buffers and one block, 44 so; 53
+// with eight waves, half of which split while the others multiply).
 constexpr uint32_t kTile = 128, kStep = 32;
 constexpr int kPitchK = kStep + 8;  // LDS rows along the summed index, padded against conflicts
 constexpr int kPitchN = kTile + 32;
@@ -76,14 +77,17 @@ __device__ __forceinline__ bf16x8 row_fragment(const short* lds, int n, int f) {
     return *reinterpret_cast<const bf16x8*>(lds + (f + (lane & 31)) * kPitchK + n + (lane >> 5) * 8);
 }
 
+constexpr int kAnyThreads = 256;
 template <class G, class Y, bool kTransposed>
-__global__ __launch_bounds__(256, 2) void linear_kernel(LinearArgs a) {
-    constexpr int kPlanes = sizeof(G) == 2 ? 1 : 3;
+__global__ __launch_bounds__(kAnyThreads, 2) void linear_kernel(LinearArgs a) {
+    constexpr int kPlanes = sizeof(G) == 2 ? 1 : 3, kBuffers = kPlanes == 1 ? 2 : 1;
+    constexpr int FB = 2;          // 32 x 32 fragments of a wave: 2 x FB
+    constexpr int kChunks = 2;     // of x, and of W, that a lane loads in a step
+    constexpr uint32_t kRows = kTile / kChunks, kRowsN = kStep / kChunks;  // that a load covers
     constexpr int kSizeA = kTile * kPitchK;
     constexpr int kSizeB = kTransposed ? kTile * kPitchK : kStep * kPitchN;
     constexpr int kBuffer = kPlanes * (kSizeA + kSizeB);
     constexpr int kOutPitch = 36;  // floats; a wave's 32 x 32 of y on its way out
-    constexpr int kBuffers = kPlanes == 1 ? 2 : 1;
     static_assert(kBuffers * kBuffer * 2 >= 4 * 32 * kOutPitch * 4);
     __shared__ __align__(16) short lds[kBuffers * kBuffer];
 
@@ -96,16 +100,16 @@ __global__ __launch_bounds__(256, 2) void linear_kernel(LinearArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int wm = wave / 2 * 64, wn = wave % 2 * 64;
 
-    // this lane's chunks of a step: two of x (rows along the summed index), two of W
-    const uint32_t rk = t % 4 * 8, rr = t / 4;            // of 32 columns x 128 rows
-    const uint32_t nn = t % 16 * 8, nk = t / 16;          // of 128 columns x 32 rows
+    // this lane's chunks of a step: of x (rows along the summed index), of W
+    const uint32_t rk = t % 4 * 8, rr = t / 4;    // of 32 columns x 128 rows
+    const uint32_t nn = t % 16 * 8, nk = t / 16;  // of 128 columns x 32 rows
     struct Loads {
-        Chunk8<G> a[2], b[2];
+        Chunk8<G> a[kChunks], b[kChunks];
     };
     // Whole steps load without a branch: rows and columns past the end are any there are, as they only
     // reach sums that are not written; a row's last chunk of W as it is reaches into the next row,
     // where there is one.  (With a branch for each chunk of the tiles at the edges, whose loads then
-    // wait for each other, 500 x 2176 x 4726 took 163 us, now 44.)
+    // wait for each other, 500 x 2176 x 4726 bf16 took 163 us, now 44.)
     const auto whole = [&](uint32_t k0) {
         return k0 + kStep <= end &&
                (kTransposed || a.outs % 8 == 0 || (a.outs >= 8 && k0 + kStep < a.cols));
@@ -114,86 +118,86 @@ __global__ __launch_bounds__(256, 2) void linear_kernel(LinearArgs a) {
     const auto load = [&](Loads& l, uint32_t k0) {
         if (whole(k0)) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t m = min(m0 + rr + 64 * h, a.rows - 1);
+            for (int h = 0; h < kChunks; ++h) {
+                const uint32_t m = min(m0 + rr + kRows * h, a.rows - 1);
                 l.a[h].load((const G*)a.x + m * a.x_stride + k0 + rk);
                 if constexpr (kTransposed)
-                    l.b[h].load((const G*)a.w + min(n0 + rr + 64 * h, a.outs - 1) * a.w_stride +
+                    l.b[h].load((const G*)a.w + min(n0 + rr + kRows * h, a.outs - 1) * a.w_stride +
                                 k0 + rk);
                 else
-                    l.b[h].load((const G*)a.w + (k0 + nk + 16 * h) * a.w_stride + column);
+                    l.b[h].load((const G*)a.w + (k0 + nk + kRowsN * h) * a.w_stride + column);
             }
             return;
         }
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint32_t m = m0 + rr + 64 * h, k = k0 + rk;
+        for (int h = 0; h < kChunks; ++h) {
+            const uint32_t m = m0 + rr + kRows * h, k = k0 + rk;
             load_upto8(l.a[h], (const G*)a.x + m * a.x_stride + k,
-                 m < a.rows && k < end ? (int)min(end - k, 8u) : 0);
+                       m < a.rows && k < end ? (int)min(end - k, 8u) : 0);
             if constexpr (kTransposed) {
-                const uint32_t n = n0 + rr + 64 * h;
+                const uint32_t n = n0 + rr + kRows * h;
                 load_upto8(l.b[h], (const G*)a.w + n * a.w_stride + k,
-                     n < a.outs && k < end ? (int)min(end - k, 8u) : 0);
+                           n < a.outs && k < end ? (int)min(end - k, 8u) : 0);
             } else {
-                const uint32_t n = n0 + nn, kb = k0 + nk + 16 * h;
+                const uint32_t n = n0 + nn, kb = k0 + nk + kRowsN * h;
                 load_upto8(l.b[h], (const G*)a.w + kb * a.w_stride + n,
-                     kb < end && n < a.outs ? (int)min(a.outs - n, 8u) : 0);
+                           kb < end && n < a.outs ? (int)min(a.outs - n, 8u) : 0);
             }
         }
     };
     const auto store = [&](const Loads& l, short* buffer) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < kChunks; ++h) {
             u32x4 w[kPlanes];
             planes_of(l.a[h], w);
 #pragma unroll
             for (int p = 0; p < kPlanes; ++p)
-                *reinterpret_cast<u32x4*>(buffer + p * kSizeA + (rr + 64 * h) * kPitchK + rk) =
+                *reinterpret_cast<u32x4*>(buffer + p * kSizeA + (rr + kRows * h) * kPitchK + rk) =
                     w[p];
             planes_of(l.b[h], w);
             short* b = buffer + kPlanes * kSizeA;
 #pragma unroll
             for (int p = 0; p < kPlanes; ++p)
                 *reinterpret_cast<u32x4*>(
-                    b + p * kSizeB +
-                    (kTransposed ? (rr + 64 * h) * kPitchK + rk : (nk + 16 * h) * kPitchN + nn)) =
-                    w[p];
+                    b + p * kSizeB + (kTransposed ? (rr + kRows * h) * kPitchK + rk
+                                                  : (nk + kRowsN * h) * kPitchN + nn)) = w[p];
         }
     };
 
-    f32x16 acc[2][2];
+    f32x16 acc[2][FB];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = f32x16{};
+        for (int j = 0; j < FB; ++j) acc[i][j] = f32x16{};
     const auto multiply = [&](const short* buffer) {
 #pragma unroll
         for (int k = 0; k < (int)kStep; k += 16) {
-            bf16x8 fa[kPlanes][2], fb[kPlanes][2];
+            bf16x8 fa[kPlanes][2], fb[kPlanes][FB];
 #pragma unroll
-            for (int p = 0; p < kPlanes; ++p)
+            for (int p = 0; p < kPlanes; ++p) {
+                const short* b = buffer + kPlanes * kSizeA + p * kSizeB;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
+                for (int i = 0; i < 2; ++i)
                     fa[p][i] = row_fragment(buffer + p * kSizeA, k, wm + 32 * i);
-                    const short* b = buffer + kPlanes * kSizeA + p * kSizeB;
-                    fb[p][i] = kTransposed ? row_fragment(b, k, wn + 32 * i)
-                                           : fragment(b, kPitchN, k, wn + 32 * i);
-                }
-            const auto products = [&](const bf16x8(&u)[2], const bf16x8(&v)[2]) {
+#pragma unroll
+                for (int j = 0; j < FB; ++j)
+                    fb[p][j] = kTransposed ? row_fragment(b, k, wn + 32 * j)
+                                           : fragment(b, kPitchN, k, wn + 32 * j);
+            }
+            const auto products = [&](const bf16x8(&u)[2], const bf16x8(&v)[FB]) {
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int j = 0; j < 2; ++j)
+                    for (int j = 0; j < FB; ++j)
                         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[i], v[j], acc[i][j],
                                                                             0, 0, 0);
             };
             products(fa[0], fb[0]);
             if constexpr (kPlanes == 3) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    fa[0][i] = finite(fa[0][i]);
-                    fb[0][i] = finite(fb[0][i]);
-                }
+                for (int i = 0; i < 2; ++i) fa[0][i] = finite(fa[0][i]);
+#pragma unroll
+                for (int j = 0; j < FB; ++j) fb[0][j] = finite(fb[0][j]);
                 products(fa[0], fb[1]);
                 products(fa[1], fb[0]);
                 products(fa[0], fb[2]);
@@ -205,19 +209,26 @@ __global__ __launch_bounds__(256, 2) void linear_kernel(LinearArgs a) {
     const uint32_t first = part * a.per, steps = (end - first + kStep - 1) / kStep;
     Loads l;
     load(l, first);
-    if constexpr (kBuffers == 2) store(l, lds);
-    for (uint32_t s = 0; s < steps; ++s) {
-        if constexpr (kBuffers == 1) {
+    if constexpr (kBuffers == 2) {
+        store(l, lds);
+        if (steps > 1) load(l, first + kStep);
+        __syncthreads();
+        for (uint32_t s = 0; s < steps; ++s) {
+            multiply(lds + (s & 1) * kBuffer);
+            if (s + 1 < steps) store(l, lds + ((s + 1) & 1) * kBuffer);
+            if (s + 2 < steps) load(l, first + (s + 2) * kStep);
+            __syncthreads();
+        }
+    } else {
+        for (uint32_t s = 0; s < steps; ++s) {
             __syncthreads();  // the step before has been read
             store(l, lds);
+            __syncthreads();
+            if (s + 1 < steps) load(l, first + (s + 1) * kStep);
+            multiply(lds);
         }
         __syncthreads();
-        if (s + 1 < steps) load(l, first + (s + 1) * kStep);
-        multiply(lds + (kBuffers == 2 ? s & 1 : 0) * kBuffer);
-        if constexpr (kBuffers == 2)
-            if (s + 1 < steps) store(l, lds + ((s + 1) & 1) * kBuffer);
     }
-    __syncthreads();
 
     // out, 32 x 32 at a time through this wave's LDS
     const uint64_t seed = a.has_dropout ? seed_of(a.dropout) : 0;
@@ -225,13 +236,13 @@ __global__ __launch_bounds__(256, 2) void linear_kernel(LinearArgs a) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < FB; ++j) {
 #pragma unroll
             for (int k = 0; k < 16; ++k)
                 out[(8 * (k / 4) + 4 * (lane >> 5) + k % 4) * kOutPitch + (lane & 31)] =
                     acc[i][j][k];
             __builtin_amdgcn_wave_barrier();
-#pragma unroll
+#pragma unroll 1
             for (int h = 0; h < 2; ++h) {
                 const uint32_t r = lane / 4 + 16 * h, c = lane % 4 * 8;
                 float v[8];
@@ -336,11 +347,11 @@ int multiply(ttp_ctx* ctx, const ttpi::Op& op, LinearArgs a, bool transposed) {
             else
                 launch_direct_to_fp32(cut.shape, transposed, blocks, op.stream, a);
         } else if (transposed) {
-            hipLaunchKernelGGL((linear_kernel<G, Y, true>), dim3(blocks), dim3(256), 0, op.stream,
-                               a);
+            hipLaunchKernelGGL((linear_kernel<G, Y, true>), dim3(blocks), dim3(kAnyThreads), 0,
+                               op.stream, a);
         } else {
-            hipLaunchKernelGGL((linear_kernel<G, Y, false>), dim3(blocks), dim3(256), 0, op.stream,
-                               a);
+            hipLaunchKernelGGL((linear_kernel<G, Y, false>), dim3(blocks), dim3(kAnyThreads), 0,
+                               op.stream, a);
         }
     });
 }
