@@ -116,7 +116,7 @@ GRADS = [(1, 1, 1, "same"), (1, 768, 300, "uniform"), (31, 8, 5, "zipf"), (32, 1
          (33, 64, 3, "same"), (64, 257, 1000, "zipf"), (100, 33, 65, "uniform"),
          (1025, 384, 65, "zipf"), (4099, 48, 50257, "zipf"), (3000, 20, 3000, "positions"),
          (2048, 100, 128, "positions"), (5000, 36, 700, "same"), (2500, 768, 300, "zipf"),
-         (700, 5, 20000, "uniform")]
+         (700, 5, 20000, "uniform"), (20011, 8, 65, "zipf"), (40001, 12, 900, "zipf")]
 
 
 @pytest.mark.parametrize("rows,cols,vocab,kind", GRADS)

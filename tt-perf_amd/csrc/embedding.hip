@@ -1,6 +1,7 @@
 // embedding.hip — embedding lookup, and its gradient by sorted tokens.
 //
-// The lookup is bound by memory: a lane has 8 columns of a row.
+// The lookup is bound by memory: a lane has 8 columns of a row (16384 x 768 bf16 with a table of
+// positions: 10.8 us).
 //
 // The gradient's row v is the sum of the rows of dy whose token is v, in their order.  Three launches:
 // sort_tokens_kernel puts the tokens in order (equal ones by their rows), sum_rows_kernel walks the
@@ -9,14 +10,16 @@
 // ends goes to scratch memory, and join_runs_kernel adds these up in order, while its first blocks
 // write zeros where no token is.  No sum depends on when a block runs.
 // Measured, 16384 x 768 bf16 into 50257 rows: sort 12 us, sums 15 (5 of them to find their rows),
-// joins beside 77 MB of zeros 17; added to a gradient that is there 12, 13 and 8.
+// joins beside 77 MB of zeros 17; added to a gradient that is there 12, 13 and 8.  4099 x 384 fp32
+// into 65 rows: 7, 4 and 5 us.
 //
 // The sort: block p has the tokens p, p + parts, p + 2 parts ..., at most kMostKeys of the table's.
 // It counts the tokens of all rows that are another block's before its own, which is where its own
 // begin, so the blocks need nothing of each other; for that it reads the list of tokens (128 KB of
 // a batch of 16384) from the L2.  Its own it lists in the order of the rows; each wave counts an
 // equal share of the list by token, the counts' sums say where each wave's entries of each token
-// go, and within 64 entries ballots tell how many equal ones stand before.
+// go, and within 64 entries ballots tell how many equal ones stand before.  A block of one token has
+// its entries in order as soon as they are listed (65 tokens, 4099 rows: 7.0 us instead of 8.8).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -192,7 +195,9 @@ __global__ __launch_bounds__(kSortBlock) void sort_tokens_kernel(GradArgs a) {
             if (mine(k)) {
                 const uint32_t to = at + __popcll(m & below);
                 const Entry e{v[k], (uint32_t)r0 + wave * (kRounds * 64) + k * 64 + lane};
-                if (to < kListed)
+                if (a.keys == 1)
+                    a.sorted[base + to] = e;
+                else if (to < kListed)
                     list[to] = e;
                 else
                     a.listed[base + to] = e;
@@ -202,6 +207,10 @@ __global__ __launch_bounds__(kSortBlock) void sort_tokens_kernel(GradArgs a) {
         n += b.all;
     }
     if (part == in_part && t == 0) *a.count = base + n;
+    if (a.keys == 1) {  // (the order of the rows is all)
+        if (t == 0) a.named[part] = n != 0;
+        return;
+    }
     __syncthreads();  // (the list in memory, too: this block alone writes and reads its part)
     const auto entry = [&](uint32_t i) { return i < kListed ? list[i] : a.listed[base + i]; };
 
