@@ -672,7 +672,8 @@ int ttp_layer_norm_backward(ttp_ctx* ctx, uint32_t weight, uint32_t bias, const 
  * y either, the residual y's.  The input's gradient of y = x W is this call on dy with
  * `transposed` the other way round.  Products of bf16 are exact, sums in fp32.  fp32 operands go
  * in as three bf16 parts each, of whose products the six largest are taken: what is left out is
- * below 2^-22 of a product (of an operand below 2^-110 the bits below 2^-133 are lost).
+ * below 2^-22 of a product (of an operand below 2^-110 the bits below 2^-133 are lost).  An fp32
+ * infinity gives what fp32 arithmetic does with factors below 2^12, with larger ones that or NaN.
  * y may be exactly the residual. */
 #define TTP_ACTIVATION_NONE 0
 #define TTP_ACTIVATION_RELU 1

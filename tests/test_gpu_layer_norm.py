@@ -322,3 +322,19 @@ def test_refusals():
             store.layer_norm_backward(1, x3, dy.view(2, 4, 16), r.mean.view(4, 2), r.rstd, bias=2)
         assert all(torch.equal(u, v) for u, v in zip((x, dy, *r), kept))
         assert not any(store.has_grad(i) for i in range(4))
+
+
+def test_a_place_that_is_read_as_another_type():
+    """dx in add's place, where dy lies too, of as many bytes in all but other rows."""
+    torch = torch_mod()
+    rows, cols = 3, 8
+    memory = torch.zeros(64, device="cuda")
+    dy = memory[:rows * cols].view(rows, cols)  # 96 bytes: 2 x 32 + 32
+    add = memory.view(torch.bfloat16).as_strided((rows, cols), (20, 1))  # 2 x 40 + 16
+    x, _ = _inputs(rows, cols, torch.bfloat16, 3)
+    w, b = _weights(cols, "fp32")
+    with B.store_of([w, b], "fp32") as store:
+        r = store.layer_norm(1, x, bias=2)
+        with pytest.raises(ValueError, match="overlap"):
+            store.layer_norm_backward(1, x, dy, r.mean, r.rstd, bias=2, add=add, out=add)
+        assert not memory.any() and not store.has_grad(1)

@@ -93,11 +93,17 @@ class Buffers {
         return true;
     }
 
+    // the same bytes in every row
+    static bool same_rows(const Span& a, const Span& b) {
+        return a.at == b.at && a.bytes == b.bytes && a.width == b.width &&
+               (a.pitch == b.pitch || a.bytes == a.width);
+    }
+
     int add(const Span& s) {
         for (int k = 0; k < n_; ++k) {
             const Span& o = spans_[k];
             if (!(s.written || o.written) || !overlap(s, o)) continue;
-            if (s.in_place && !o.written && s.at == o.at && s.bytes == o.bytes) continue;
+            if (s.in_place && !o.written && same_rows(s, o)) continue;
             return fail(TTP_ERR_INVALID, std::string(s.what) + " overlaps " + o.what);
         }
         if (n_ < kMax) spans_[n_++] = s;
