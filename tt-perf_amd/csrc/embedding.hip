@@ -3,7 +3,8 @@
 // The lookup is bound by memory: a lane has 8 columns of a row (16384 x 768 bf16 with a table of
 // positions: 10.8 us).
 //
-// The gradient's row v is the sum of the rows of dy whose token is v, in their order.  Three launches:
+// The gradient's row v is the sum of the rows of dy whose token is v, in their order.  Up to 512 rows
+// few_rows_kernel looks for them itself.  For more there are three launches:
 // sort_tokens_kernel puts the tokens in order (equal ones by their rows), sum_rows_kernel walks the
 // sorted list in chunks of equal length, so that frequent tokens cost no more than rare ones, and
 // writes every run of one token that lies within a chunk; what a chunk has of a run that crosses its
@@ -484,6 +485,110 @@ __global__ __launch_bounds__(256) void join_runs_kernel(GradArgs a, uint32_t wav
     put_row(p, a.cols, a.scale, a.first, c, (s0 + s1) + (s2 + s3), old);
 }
 
+// Few tokens, in one launch: a wave has `keys` rows of the gradient and a slab of their columns, and
+// looks through all tokens for those rows.  Where there are none, the waves of these rows share their
+// zeros; else each row's list goes through the LDS, and its rows of dy are added up 16 at a time, in
+// eight sums.  Up to 512 tokens, us (sorted / so): 500 x 768 into 50257 rows bf16 31.5 / 19.5 and fp32
+// 40.1 / 33.0 (the zeros alone 13.0 and 29.1), 300 x 1600 into 5000 rows 23.8 / 11.7, 200 x 384 into 65
+// rows 18.2 / 11.7; slower only where most of them are one token, whose list is one wave's a slab
+// (512 x 384 in full: 18 / 25).
+constexpr uint32_t kFewTokens = 512, kFewWords = kFewTokens / 64;
+template <class G, class O, bool kNarrow>
+__global__ __launch_bounds__(64 * kSumWaves) void few_rows_kernel(GradArgs a, uint32_t waves) {
+    __shared__ uint32_t lists[kSumWaves][kFewTokens];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t w = blockIdx.x * kSumWaves + wave;
+    if (w >= waves) return;
+    const uint32_t lane = threadIdx.x & 63, slab = w % a.slabs;
+    const uint32_t row0 = w / a.slabs * a.keys, n = min(a.keys, a.vocab - row0);
+    const Columns c = columns_of(slab * kSlab + lane * 4, a.cols);
+    uint32_t* const list = lists[wave];
+    int64_t token[kFewWords];
+#pragma unroll
+    for (uint32_t k = 0; k < kFewWords; ++k)
+        token[k] = k * 64 + lane < a.rows ? a.tokens[k * 64 + lane] : -1;
+    uint32_t key[kFewWords];  // of this wave's rows; n: none of them
+#pragma unroll
+    for (uint32_t k = 0; k < kFewWords; ++k)
+        key[k] = token[k] >= (int64_t)row0 && token[k] < (int64_t)(row0 + n)
+                     ? (uint32_t)token[k] - row0
+                     : n;
+    bool any = false;
+#pragma unroll
+    for (uint32_t k = 0; k < kFewWords; ++k) any |= key[k] != n;
+    O* p = (O*)a.grad + (uint64_t)row0 * a.cols;
+    if (!__ballot(any)) {  // (so in the other slabs of these rows: each has a share of them all)
+        if (!a.first) return;
+        const uint64_t all = (uint64_t)n * a.cols;
+        const float zeros[8] = {};
+        for (uint64_t at = ((uint64_t)slab * 64 + lane) * 8; at < all; at += (uint64_t)a.slabs * 512)
+            store_cols(p + at, 0, (uint32_t)min(all - at, 8ul), zeros);
+        return;
+    }
+    const G* const dy = (const G*)a.dy + c.at;
+    p += c.at;
+    for (uint32_t i = 0; i < n; ++i, p += a.cols) {
+        uint32_t count = 0;
+#pragma unroll
+        for (uint32_t k = 0; k < kFewWords; ++k) {
+            const uint64_t m = __ballot(key[k] == i);
+            if (key[k] == i) list[count + __popcll(m & ((1ull << lane) - 1))] = k * 64 + lane;
+            count += __popcll(m);
+        }
+        if (!count && !a.first) continue;
+        __builtin_amdgcn_wave_barrier();
+        Raw4<O> old;
+        if (!a.first) old_row(old, p, a.cols);
+        f32x4 sums[8] = {};
+        for (uint32_t k0 = 0; k0 < count; k0 += 16) {
+            const uint32_t mine = list[min(k0 + (lane & 15), count - 1)];
+            Raw4<G> v[16];
+#pragma unroll
+            for (uint32_t k = 0; k < 16; ++k) {
+                const G* q = dy + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)mine, k) *
+                                      a.dy_stride;
+                if constexpr (kNarrow)
+                    v[k].load_some(q, a.cols);
+                else
+                    v[k].load(q);
+            }
+#pragma unroll
+            for (uint32_t k = 0; k < 16; ++k) v[k].here();
+            if (k0 + 16 <= count) {
+#pragma unroll
+                for (uint32_t k = 0; k < 16; ++k) sums[k % 8] += v[k].values();
+            } else {
+#pragma unroll
+                for (uint32_t k = 0; k < 16; ++k)
+                    if (k0 + k < count) sums[k % 8] += v[k].values();
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+        if (c.skip < 4)
+            put_row(p, a.cols, a.scale, a.first, c,
+                    ((sums[0] + sums[1]) + (sums[2] + sums[3])) +
+                        ((sums[4] + sums[5]) + (sums[6] + sums[7])),
+                    old);
+    }
+}
+
+template <class G, class O>
+int add_few_rows(const ttpi::Op& op, GradArgs a) {
+    // rows of a wave: as many as leave the CUs 16 waves each, up to 8 (with 16, 256 neighbouring tokens
+    // of 50257 took 28 us instead of 17)
+    const uint64_t all = (uint64_t)a.vocab * a.slabs / (16 * (uint64_t)op.num_cus);
+    a.keys = (uint32_t)std::max<uint64_t>(std::min<uint64_t>(all, 8), 1);
+    const uint32_t waves = (a.vocab + a.keys - 1) / a.keys * a.slabs;
+    const dim3 grid((waves + kSumWaves - 1) / kSumWaves), block(64 * kSumWaves);
+    (void)hipGetLastError();
+    if (a.cols < 4)
+        hipLaunchKernelGGL((few_rows_kernel<G, O, true>), grid, block, 0, op.stream, a, waves);
+    else
+        hipLaunchKernelGGL((few_rows_kernel<G, O, false>), grid, block, 0, op.stream, a, waves);
+    TTPI_HIP(hipGetLastError());
+    return TTP_OK;
+}
+
 template <class G, class O>
 int add_rows(const ttpi::Op& op, const GradArgs& a) {
     (void)hipGetLastError();
@@ -611,6 +716,17 @@ int ttp_accumulate_embedding_grad(ttp_ctx* ctx, uint32_t table, const int64_t* t
         a.scale = (float)scale;
         a.grad = g.data;
         a.first = g.first;
+        const bool bf16 = dy->dtype == TTP_DTYPE_BF16;
+        if (rows <= kFewTokens) {
+            if (g.bf16)
+                rc = bf16 ? add_few_rows<uint16_t, uint16_t>(op, a)
+                          : add_few_rows<float, uint16_t>(op, a);
+            else
+                rc = bf16 ? add_few_rows<uint16_t, float>(op, a) : add_few_rows<float, float>(op, a);
+            if (rc) return rc;
+            ttpi::grad_written(ctx, table);
+            return TTP_OK;
+        }
         const uint64_t chunks = (rows + kChunk - 1) / kChunk;
         if (chunks * a.slabs >= (1ull << 25))
             return fail(TTP_ERR_RANGE, "the output's gradient is too large for one launch");
@@ -627,7 +743,6 @@ int ttp_accumulate_embedding_grad(ttp_ctx* ctx, uint32_t table, const int64_t* t
         a.count = (uint32_t*)(a.named + named);
         if (a.first) a.fills = (uint32_t)((named + 3) / 4 * 4);
         a.groups_in_all = (uint32_t)named;
-        const bool bf16 = dy->dtype == TTP_DTYPE_BF16;
         if (g.bf16)
             rc = bf16 ? add_rows<uint16_t, uint16_t>(op, a) : add_rows<float, uint16_t>(op, a);
         else
