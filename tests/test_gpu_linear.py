@@ -147,7 +147,9 @@ LARGER = [(1025, 1600, 1601, "mixed"), (3000, 770, 523, "mixed"), (520, 6400, 16
           (2304, 1280, 1280, "bf16"), (700, 1284, 900, "fp32"), (4100, 64, 4100, "mixed"),
           (300, 50257, 100, "mixed"), (33, 768, 50257, "mixed"), (4099, 1288, 5128, "mixed"),
           (8200, 200, 1288, "bf16"), (8190, 2568, 1280, "mixed"), (5, 5128, 1288, "mixed"),
-          (100, 5120, 1280, "mixed"), (1, 50264, 136, "mixed")]
+          (100, 5120, 1280, "mixed"), (1, 50264, 136, "mixed"), (17, 4001, 1201, "mixed"),
+          (1, 768, 50257, "fp32"), (64, 6401, 300, "fp32"), (65, 6400, 301, "fp32"),
+          (3, 40, 70001, "bf16")]
 
 
 @pytest.mark.parametrize("rows,cols,outs,mode", LARGER)

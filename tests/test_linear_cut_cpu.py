@@ -22,7 +22,7 @@ int main() {
     }
 }
 """
-THIN, SMALL, WIDE, LARGE, ANY = range(5)
+THIN, SMALL, WIDE, LARGE, THIN_ANY, ANY = range(6)
 
 
 @pytest.fixture(scope="module")
@@ -50,10 +50,13 @@ def test_the_gpu_tests_reach_every_shape_and_parts(cut):
     shapes = [(r, c, o, int(_direct(c, o, tr)), 1, tr) for tr in (0, 1)
               for r, c, o in [*gpu.SHAPES, *[s[:3] for s in gpu.LARGER if s[3] != "fp32"]]]
     got = cut(shapes)
-    assert {g[0] for g in got} == {THIN, SMALL, WIDE, LARGE, ANY}
+    assert {g[0] for g in got} == {THIN, SMALL, WIDE, LARGE, THIN_ANY, ANY}
     assert {(g[0], g[3] > 1) for g in got} >= {(THIN, False), (THIN, True), (SMALL, False),
-                                               (SMALL, True), (ANY, False), (ANY, True)}
-    assert {g[3] > 1 for g in cut([(r, c, o, 0, 0, 0) for r, c, o in gpu.SHAPES])} == {False, True}
+                                               (SMALL, True), (ANY, False), (ANY, True),
+                                               (THIN_ANY, False), (THIN_ANY, True)}
+    full = cut([(r, c, o, 0, 0, 0) for r, c, o in gpu.SHAPES])
+    assert {(g[0], g[3] > 1) for g in full} == {(s, p) for s in (THIN_ANY, ANY)
+                                                for p in (False, True)}
 
 
 def test_parts_cover_the_summed_index(cut):
@@ -65,10 +68,10 @@ def test_parts_cover_the_summed_index(cut):
         shapes.append((*size, direct, 1 if direct else rng.randrange(2), rng.randrange(2)))
     for s, (shape, tile_rows, tile_outs, parts, per) in zip(shapes, cut(shapes)):
         rows, cols, outs, direct, bf16, _ = s
-        step = 32 if shape in (WIDE, ANY) else 64
-        assert (shape == ANY) == (not direct) and per % step == 0, s
+        step = 32 if shape in (WIDE, THIN_ANY, ANY) else 64
+        assert (shape in (THIN_ANY, ANY)) == (not direct) and per % step == 0, s
         assert 1 <= parts <= 32 and (parts - 1) * per < cols <= parts * per, (s, parts, per)
         if parts > 1:  # parts of four steps or more, of few tiles
             assert per >= 4 * step
             tiles = -(-rows // tile_rows) * -(-outs // tile_outs)
-            assert tiles < 3 * 256
+            assert tiles < (4 if shape == THIN_ANY else 3) * 256

@@ -63,10 +63,11 @@ __device__ __forceinline__ bf16x8 finite(bf16x8 v) {
 }
 
 // ---- operands of any alignment, through registers ---------------------------------------------
-// 128 x 128 of y per block of four waves, 32 of the summed index per step; bf16 through two LDS
-// buffers, the three parts of fp32 through one, so that two blocks share a CU and one's products run
-// beside the other's splitting (3585 x 384 x 1536: 56 us with two buffers and one block, 44 so; 53
-// with eight waves, half of which split while the others multiply).
+// 128 x 128 of y per block of four waves, or 32 x 128 where rows are few and W is what is read (a
+// token's 768 x 50257 fp32: 35 us, of 30 for its 154 MB, instead of 64); 32 of the summed index per
+// step; bf16 through two LDS buffers, the three parts of fp32 through one, so that blocks share a CU
+// and one's products run beside another's splitting (3585 x 384 x 1536: 56 us with two buffers and one
+// block, 44 so; 53 with eight waves, half of which split while the others multiply).
 constexpr uint32_t kTile = 128, kStep = 32;
 constexpr int kPitchK = kStep + 8;  // LDS rows along the summed index, padded against conflicts
 constexpr int kPitchN = kTile + 32;
@@ -78,13 +79,14 @@ __device__ __forceinline__ bf16x8 row_fragment(const short* lds, int n, int f) {
 }
 
 constexpr int kAnyThreads = 256;
-template <class G, class Y, bool kTransposed>
-__global__ __launch_bounds__(kAnyThreads, 2) void linear_kernel(LinearArgs a) {
+template <class G, class Y, bool kTransposed, uint32_t kM>
+__global__ __launch_bounds__(kAnyThreads, kM == kTile ? 2 : 4) void linear_kernel(LinearArgs a) {
     constexpr int kPlanes = sizeof(G) == 2 ? 1 : 3, kBuffers = kPlanes == 1 ? 2 : 1;
-    constexpr int FB = 2;          // 32 x 32 fragments of a wave: 2 x FB
-    constexpr int kChunks = 2;     // of x, and of W, that a lane loads in a step
+    constexpr int FA = kM == kTile ? 2 : 1, FB = FA;  // 32 x 32 fragments of a wave
+    constexpr int kChunks = 2;  // of W, that a lane loads in a step
+    constexpr int kChunksA = kM == kTile ? 2 : 1;  // of x (kM 32: the first 128 lanes)
     constexpr uint32_t kRows = kTile / kChunks, kRowsN = kStep / kChunks;  // that a load covers
-    constexpr int kSizeA = kTile * kPitchK;
+    constexpr int kSizeA = kM * kPitchK;
     constexpr int kSizeB = kTransposed ? kTile * kPitchK : kStep * kPitchN;
     constexpr int kBuffer = kPlanes * (kSizeA + kSizeB);
     constexpr int kOutPitch = 36;  // floats; a wave's 32 x 32 of y on its way out
@@ -94,17 +96,18 @@ __global__ __launch_bounds__(kAnyThreads, 2) void linear_kernel(LinearArgs a) {
     uint32_t id = xcd_order(blockIdx.x, gridDim.x);
     const uint32_t part = id / (a.tiles_m * a.tiles_n);
     id -= part * (a.tiles_m * a.tiles_n);
-    const uint32_t m0 = id % a.tiles_m * kTile, n0 = id / a.tiles_m * kTile;
+    const uint32_t m0 = id % a.tiles_m * kM, n0 = id / a.tiles_m * kTile;
     const uint32_t end = min((part + 1) * a.per, a.cols);  // of the summed index
     const int t = threadIdx.x, lane = t & 63;
     const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int wm = wave / 2 * 64, wn = wave % 2 * 64;
+    const int wm = kM == kTile ? wave / 2 * 64 : 0, wn = kM == kTile ? wave % 2 * 64 : wave * 32;
+    const bool has_a = kM == kTile || wave < 2;
 
     // this lane's chunks of a step: of x (rows along the summed index), of W
     const uint32_t rk = t % 4 * 8, rr = t / 4;    // of 32 columns x 128 rows
     const uint32_t nn = t % 16 * 8, nk = t / 16;  // of 128 columns x 32 rows
     struct Loads {
-        Chunk8<G> a[kChunks], b[kChunks];
+        Chunk8<G> a[kChunksA], b[kChunks];
     };
     // Whole steps load without a branch: rows and columns past the end are any there are, as they only
     // reach sums that are not written; a row's last chunk of W as it is reaches into the next row,
@@ -117,10 +120,14 @@ __global__ __launch_bounds__(kAnyThreads, 2) void linear_kernel(LinearArgs a) {
     const uint32_t column = n0 + nn < a.outs ? n0 + nn : 0;
     const auto load = [&](Loads& l, uint32_t k0) {
         if (whole(k0)) {
+            if (has_a)
+#pragma unroll
+                for (int h = 0; h < kChunksA; ++h) {
+                    const uint32_t m = min(m0 + rr + kRows * h, a.rows - 1);
+                    l.a[h].load((const G*)a.x + m * a.x_stride + k0 + rk);
+                }
 #pragma unroll
             for (int h = 0; h < kChunks; ++h) {
-                const uint32_t m = min(m0 + rr + kRows * h, a.rows - 1);
-                l.a[h].load((const G*)a.x + m * a.x_stride + k0 + rk);
                 if constexpr (kTransposed)
                     l.b[h].load((const G*)a.w + min(n0 + rr + kRows * h, a.outs - 1) * a.w_stride +
                                 k0 + rk);
@@ -129,11 +136,15 @@ __global__ __launch_bounds__(kAnyThreads, 2) void linear_kernel(LinearArgs a) {
             }
             return;
         }
+        const uint32_t k = k0 + rk;
+#pragma unroll
+        for (int h = 0; h < kChunksA; ++h) {
+            const uint32_t m = m0 + rr + kRows * h;
+            load_upto8(l.a[h], (const G*)a.x + m * a.x_stride + k,
+                       has_a && m < a.rows && k < end ? (int)min(end - k, 8u) : 0);
+        }
 #pragma unroll
         for (int h = 0; h < kChunks; ++h) {
-            const uint32_t m = m0 + rr + kRows * h, k = k0 + rk;
-            load_upto8(l.a[h], (const G*)a.x + m * a.x_stride + k,
-                       m < a.rows && k < end ? (int)min(end - k, 8u) : 0);
             if constexpr (kTransposed) {
                 const uint32_t n = n0 + rr + kRows * h;
                 load_upto8(l.b[h], (const G*)a.w + n * a.w_stride + k,
@@ -146,14 +157,19 @@ __global__ __launch_bounds__(kAnyThreads, 2) void linear_kernel(LinearArgs a) {
         }
     };
     const auto store = [&](const Loads& l, short* buffer) {
+        if (has_a)
+#pragma unroll
+            for (int h = 0; h < kChunksA; ++h) {
+                u32x4 w[kPlanes];
+                planes_of(l.a[h], w);
+#pragma unroll
+                for (int p = 0; p < kPlanes; ++p)
+                    *reinterpret_cast<u32x4*>(buffer + p * kSizeA + (rr + kRows * h) * kPitchK +
+                                              rk) = w[p];
+            }
 #pragma unroll
         for (int h = 0; h < kChunks; ++h) {
             u32x4 w[kPlanes];
-            planes_of(l.a[h], w);
-#pragma unroll
-            for (int p = 0; p < kPlanes; ++p)
-                *reinterpret_cast<u32x4*>(buffer + p * kSizeA + (rr + kRows * h) * kPitchK + rk) =
-                    w[p];
             planes_of(l.b[h], w);
             short* b = buffer + kPlanes * kSizeA;
 #pragma unroll
@@ -164,29 +180,29 @@ __global__ __launch_bounds__(kAnyThreads, 2) void linear_kernel(LinearArgs a) {
         }
     };
 
-    f32x16 acc[2][FB];
+    f32x16 acc[FA][FB];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < FA; ++i)
 #pragma unroll
         for (int j = 0; j < FB; ++j) acc[i][j] = f32x16{};
     const auto multiply = [&](const short* buffer) {
 #pragma unroll
         for (int k = 0; k < (int)kStep; k += 16) {
-            bf16x8 fa[kPlanes][2], fb[kPlanes][FB];
+            bf16x8 fa[kPlanes][FA], fb[kPlanes][FB];
 #pragma unroll
             for (int p = 0; p < kPlanes; ++p) {
                 const short* b = buffer + kPlanes * kSizeA + p * kSizeB;
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < FA; ++i)
                     fa[p][i] = row_fragment(buffer + p * kSizeA, k, wm + 32 * i);
 #pragma unroll
                 for (int j = 0; j < FB; ++j)
                     fb[p][j] = kTransposed ? row_fragment(b, k, wn + 32 * j)
                                            : fragment(b, kPitchN, k, wn + 32 * j);
             }
-            const auto products = [&](const bf16x8(&u)[2], const bf16x8(&v)[FB]) {
+            const auto products = [&](const bf16x8(&u)[FA], const bf16x8(&v)[FB]) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < FA; ++i)
 #pragma unroll
                     for (int j = 0; j < FB; ++j)
                         acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(u[i], v[j], acc[i][j],
@@ -195,7 +211,7 @@ __global__ __launch_bounds__(kAnyThreads, 2) void linear_kernel(LinearArgs a) {
             products(fa[0], fb[0]);
             if constexpr (kPlanes == 3) {
 #pragma unroll
-                for (int i = 0; i < 2; ++i) fa[0][i] = finite(fa[0][i]);
+                for (int i = 0; i < FA; ++i) fa[0][i] = finite(fa[0][i]);
 #pragma unroll
                 for (int j = 0; j < FB; ++j) fb[0][j] = finite(fb[0][j]);
                 products(fa[0], fb[1]);
@@ -234,7 +250,7 @@ __global__ __launch_bounds__(kAnyThreads, 2) void linear_kernel(LinearArgs a) {
     const uint64_t seed = a.has_dropout ? seed_of(a.dropout) : 0;
     float* out = reinterpret_cast<float*>(lds) + wave * 32 * kOutPitch;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < FA; ++i)
 #pragma unroll
         for (int j = 0; j < FB; ++j) {
 #pragma unroll
@@ -330,6 +346,16 @@ bool on_grid(const LinearArgs& a, bool transposed) {
            a.x_stride < (1u << 22) && a.w_stride < (1u << 22);
 }
 
+template <class G, class Y, uint32_t kM>
+void launch_any(bool transposed, uint32_t blocks, hipStream_t stream, const LinearArgs& a) {
+    if (transposed)
+        hipLaunchKernelGGL((linear_kernel<G, Y, true, kM>), dim3(blocks), dim3(kAnyThreads), 0, stream,
+                           a);
+    else
+        hipLaunchKernelGGL((linear_kernel<G, Y, false, kM>), dim3(blocks), dim3(kAnyThreads), 0,
+                           stream, a);
+}
+
 template <class G, class Y>
 int multiply(ttp_ctx* ctx, const ttpi::Op& op, LinearArgs a, bool transposed) {
     constexpr bool kBf16 = sizeof(G) == 2;
@@ -346,12 +372,10 @@ int multiply(ttp_ctx* ctx, const ttpi::Op& op, LinearArgs a, bool transposed) {
                 launch_direct_to_bf16(cut.shape, transposed, blocks, op.stream, a);
             else
                 launch_direct_to_fp32(cut.shape, transposed, blocks, op.stream, a);
-        } else if (transposed) {
-            hipLaunchKernelGGL((linear_kernel<G, Y, true>), dim3(blocks), dim3(kAnyThreads), 0,
-                               op.stream, a);
+        } else if (cut.shape == LinearShape::kThinAny) {
+            launch_any<G, Y, kThinRows>(transposed, blocks, op.stream, a);
         } else {
-            hipLaunchKernelGGL((linear_kernel<G, Y, false>), dim3(blocks), dim3(kAnyThreads), 0,
-                               op.stream, a);
+            launch_any<G, Y, kTile>(transposed, blocks, op.stream, a);
         }
     });
 }

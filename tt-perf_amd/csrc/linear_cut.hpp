@@ -7,8 +7,8 @@
 
 namespace ttp {
 
-// The shapes of linear_direct_kernel and the one of any alignment.
-enum class LinearShape { kThin, kSmall, kWide, kLarge, kAny };
+// The shapes of linear_direct_kernel and the two of any alignment.
+enum class LinearShape { kThin, kSmall, kWide, kLarge, kThinAny, kAny };
 
 namespace {
 
@@ -66,6 +66,14 @@ inline LinearCut choose_linear_cut(uint64_t rows, uint64_t cols, uint64_t outs, 
                                    bool bf16, bool transposed, uint64_t cus) {
     using S = LinearShape;
     if (!direct) {
+        // (1 x 768 x 50257 transposed fp32: thin 35 us, the other 64; 64 rows 56 and 67, 96 rows 73 and
+        // 67; bf16 769 columns, 32 rows: 20 and 25, 33 rows 30 and 25)
+        if (rows <= (bf16 ? kThinRows : 2 * kThinRows)) {
+            const LinearCost thin =
+                bf16 ? LinearCost{S::kThinAny, 32, 128, 32, 4, 250.0, 600.0, 4000.0}
+                     : LinearCost{S::kThinAny, 32, 128, 32, 4, 600.0, 1500.0, 4000.0};
+            return cut_parts(rows, cols, outs, thin, cus);
+        }
         const LinearCost any = bf16 ? LinearCost{S::kAny, 128, 128, 32, 2, 380.0, 680.0, 5000.0}
                                     : LinearCost{S::kAny, 128, 128, 32, 2, 1500.0, 2000.0, 5000.0};
         return cut_parts(rows, cols, outs, any, cus);

@@ -396,6 +396,7 @@ void launch_direct(LinearShape shape, bool transposed, uint32_t blocks, hipStrea
             return launch_shape<128, 8, 2, 32, 3, Y>(transposed, blocks, stream, a);
         case LinearShape::kLarge:
             return launch_shape<256, 5, 2, 64, 3, Y>(transposed, blocks, stream, a);
+        case LinearShape::kThinAny:
         case LinearShape::kAny: break;
     }
 }
