@@ -71,7 +71,7 @@ def test_parts_cover_the_summed_index(cut):
         step = 32 if shape in (WIDE, THIN_ANY, ANY) else 64
         assert (shape in (THIN_ANY, ANY)) == (not direct) and per % step == 0, s
         assert 1 <= parts <= 32 and (parts - 1) * per < cols <= parts * per, (s, parts, per)
-        if parts > 1:  # parts of four steps or more, of few tiles
-            assert per >= 4 * step
+        if parts > 1:  # parts of three steps or more, of few tiles
+            assert per >= 3 * step
             tiles = -(-rows // tile_rows) * -(-outs // tile_outs)
             assert tiles < (4 if shape == THIN_ANY else 3) * 256
