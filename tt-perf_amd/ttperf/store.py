@@ -559,8 +559,9 @@ class ParamStore(_StepSlots, Operators):
     def torch_view(self, which=L.BUF_PARAM, index=L.ALL_TENSORS):
         """Zero-copy torch tensor over a contiguously stored buffer (PARAM, GRAD, MOMENTUM;
         MASTER in fp32 mode): the whole flat buffer, or one tensor's slice as a 1-D tensor.
-        bf16 buffers come back as torch.bfloat16.  The view aliases the store's memory for the
-        store's lifetime.  Torch work on it is ordered on torch's current stream and the
+        bf16 buffers come back as torch.bfloat16.  The view aliases the store's memory, which
+        lasts until the store is closed (a view keeps a store alive that nothing else
+        names).  Torch work on it is ordered on torch's current stream and the
         store's on its own: share one stream (set_stream(torch.cuda.current_stream())) or
         synchronise between them.  Writes to BUF_GRAD through a view need mark_grads()."""
         import torch
@@ -576,7 +577,9 @@ class ParamStore(_StepSlots, Operators):
                                         "typestr": "<u2" if two else "<f4", "strides": None,
                                         "version": 3}
 
-        t = torch.as_tensor(_Device(), device=f"cuda:{self.device}")
+        wrapped = _Device()
+        wrapped.store = self  # torch keeps what it wraps for as long as the memory has a tensor
+        t = torch.as_tensor(wrapped, device=f"cuda:{self.device}")
         if t.data_ptr() != ptr:
             raise RuntimeError("torch copied the buffer instead of wrapping it")
         return t.view(torch.bfloat16) if two else t
