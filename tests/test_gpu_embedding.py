@@ -256,6 +256,25 @@ def test_captured(rows):
         store.end_capture(discard=True)
 
 
+def test_a_table_of_many_rows():
+    """More rows than one launch has waves for their zeros."""
+    import ttperf
+    torch = torch_mod()
+    vocab, cols = (1 << 24) + 1003, 4
+    with ttperf.ParamStore([(vocab, cols)], mode="bf16") as store:
+        store.torch_view(ttperf.BUF_GRAD).fill_(3.0)
+        g = torch.Generator(device="cuda").manual_seed(4)
+        t = torch.randperm(vocab, generator=g, device="cuda")[:700]
+        t[:3] = torch.tensor([0, vocab - 1, (1 << 24) + 17], device="cuda")
+        t = t.unique()
+        dy = torch.randn(t.numel(), cols, generator=g, device="cuda").bfloat16()
+        store.accumulate_embedding_grad(0, t, dy)
+        grad = store.torch_view(ttperf.BUF_GRAD)[:vocab * cols].view(vocab, cols)
+        assert torch.equal(grad[t], dy)
+        grad[t] = 0
+        assert not grad.any()
+
+
 def test_a_table_past_2_to_the_32_elements():
     """Rows at the table's far end: lookup, gradient, zeros where no token is."""
     import ttperf
@@ -273,13 +292,16 @@ def test_a_table_past_2_to_the_32_elements():
     y = store.embedding(0, t)
     assert torch.equal(y[1:4], rows[1:4]) and torch.equal(y[0], rows[2]) and y[4].isnan().all()
     grad = B.grad(store, 0)
-    grad[-2000:] = 9.0
-    store.accumulate_embedding_grad(0, t, rows)
-    assert torch.equal(grad[vocab - 1], (rows[0].float() + rows[2].float()).bfloat16())
-    assert torch.equal(grad[t[1]], rows[1]) and torch.equal(grad[t[3]], rows[3])
-    last = grad[-2000:].clone()
-    last[t[3] - (vocab - 2000)] = 0
-    assert (last[:-1] == 0).all()
+    for more in (0, 600):  # tokens of padding: in one launch, and sorted
+        grad[-2000:] = 9.0
+        store.zero_grad(set_to_none=True, fill=False)
+        store.accumulate_embedding_grad(0, torch.cat([t, t.new_full((more,), -1)]),
+                                        torch.cat([rows, rows.new_ones(more, cols)]))
+        assert torch.equal(grad[vocab - 1], (rows[0].float() + rows[2].float()).bfloat16())
+        assert torch.equal(grad[t[1]], rows[1]) and torch.equal(grad[t[3]], rows[3])
+        last = grad[-2000:].clone()
+        last[t[3] - (vocab - 2000)] = 0
+        assert (last[:-1] == 0).all()
     del w, grad
     store.close()
 

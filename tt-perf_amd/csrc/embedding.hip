@@ -8,11 +8,11 @@
 // sort_tokens_kernel puts the tokens in order (equal ones by their rows), sum_rows_kernel walks the
 // sorted list in chunks of equal length, so that frequent tokens cost no more than rare ones, and
 // writes every run of one token that lies within a chunk; what a chunk has of a run that crosses its
-// ends goes to scratch memory, and join_runs_kernel adds these up in order, while its first blocks
+// ends goes to scratch memory, and join_runs_kernel adds these up in order, while its other blocks
 // write zeros where no token is.  No sum depends on when a block runs.
 // Measured, 16384 x 768 bf16 into 50257 rows: sort 12 us, sums 15 (5 of them to find their rows),
-// joins beside 77 MB of zeros 17; added to a gradient that is there 12, 13 and 8.  4099 x 384 fp32
-// into 65 rows: 7, 4 and 5 us.
+// joins beside 77 MB of zeros 14; added to a gradient that is there 12, 13 and 6.  4099 x 384 fp32
+// into 65 rows: 7, 4 and 6 us.
 //
 // The sort: block p has the tokens p, p + parts, p + 2 parts ..., at most kMostKeys of the table's.
 // It counts the tokens of all rows that are another block's before its own, which is where its own
@@ -116,8 +116,7 @@ struct GradArgs {
     float scale;
     void* grad;
     bool first;       // assign, zeros where no token is
-    uint32_t fills;   // waves that write those zeros: one for 64 tokens of a block of the sort,
-    uint32_t groups_in_all;  // and how many have any
+    uint32_t fills;   // waves that write those zeros
     Entry* listed;    // a block's tokens in the order of the rows, where the LDS does not hold them
     Entry* sorted;
     uint64_t* named;  // for each block of the sort, a bit for each of its tokens
@@ -328,20 +327,26 @@ __device__ __forceinline__ void put_row(O* p, uint32_t cols, float scale, bool f
     }
 }
 
-// Zeros in the rows that no token names, of 64 tokens of a block of the sort.
+// Zeros in those of 16 rows that no token names, runs of them in one.
+constexpr uint32_t kFillRows = 16;
 template <class O>
-__device__ __forceinline__ void fill_zeros(const GradArgs& a, uint32_t which) {
-    if (which >= a.groups_in_all) return;
-    const uint32_t groups = (a.keys + 63) / 64, part = which / groups, key0 = which % groups * 64;
-    uint64_t none = ~a.named[which];
-    for (; none; none &= none - 1) {
-        const uint32_t key = key0 + (uint32_t)__builtin_ctzll(none);
-        const uint64_t row = ((uint64_t)key << a.parts_log2) + part;
-        if (key >= a.keys || row >= a.vocab) break;
-        O* p = (O*)a.grad + row * a.cols;
+__device__ __forceinline__ void fill_zeros(const GradArgs& a, uint32_t row0) {
+    const uint32_t lane = threadIdx.x & 63, row = row0 + lane;
+    bool none = false;
+    if (lane < kFillRows && row < a.vocab) {
+        const uint32_t part = row & ((1u << a.parts_log2) - 1), key = row >> a.parts_log2;
+        none = !(a.named[part * ((a.keys + 63) / 64) + key / 64] >> (key % 64) & 1);
+    }
+    uint32_t left = (uint32_t)__ballot(none);
+    while (left) {
+        const uint32_t first = (uint32_t)__builtin_ctz(left);
+        const uint32_t n = (uint32_t)__builtin_ctz(~(left >> first));  // (16 bits: there is a 0)
+        left &= ~(((1u << n) - 1) << first);
+        O* p = (O*)a.grad + (uint64_t)(row0 + first) * a.cols;
+        const uint64_t all = (uint64_t)n * a.cols;
         const float zeros[8] = {};
-        for (uint64_t c = (threadIdx.x & 63) * 8; c < a.cols; c += 512)
-            store_cols(p, (uint32_t)c, a.cols, zeros);
+        for (uint64_t at = lane * 8; at < all; at += 512)
+            store_cols(p + at, 0, (uint32_t)min(all - at, 8ul), zeros);
     }
 }
 
@@ -431,16 +436,19 @@ __global__ __launch_bounds__(64 * kSumWaves) void sum_rows_kernel(GradArgs a, ui
     }
 }
 
-// The first blocks write the zeros.  The others, the runs that leave the chunk in which they begin: a
-// wave of that chunk adds up what the chunks have, in order, four sums in turn.
+// The first blocks have the runs that leave the chunk in which they begin: a wave of that chunk adds up
+// what the chunks have, in order, four sums in turn.  The others write the zeros.
 template <class O>
 __global__ __launch_bounds__(256) void join_runs_kernel(GradArgs a, uint32_t waves) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (blockIdx.x < a.fills / 4) {
-        fill_zeros<O>(a, blockIdx.x * 4 + wave);
+    const uint32_t joins = (waves + 3) / 4;
+    if (blockIdx.x >= joins) {
+        for (uint64_t row = ((blockIdx.x - joins) * 4 + wave) * kFillRows; row < a.vocab;
+             row += (uint64_t)a.fills * kFillRows)
+            fill_zeros<O>(a, (uint32_t)row);
         return;
     }
-    const uint32_t w = (blockIdx.x - a.fills / 4) * 4 + wave;
+    const uint32_t w = blockIdx.x * 4 + wave;
     if (w >= waves) return;
     const uint32_t lane = threadIdx.x & 63, chunk = w / a.slabs, slab = w % a.slabs;
     const uint32_t end = (chunk + 1) * kChunk;
@@ -467,7 +475,7 @@ __global__ __launch_bounds__(256) void join_runs_kernel(GradArgs a, uint32_t wav
         const bool goes_on = i < count && a.sorted[min(i, (uint64_t)a.rows - 1)].token == token;
         const uint32_t n = __ffsll(~__ballot(goes_on)) ? __ffsll(~__ballot(goes_on)) - 1 : 64;
         uint32_t k = 0;
-#pragma unroll 2
+#pragma unroll 4
         for (; k + 8 <= n; k += 8) {
             const uint32_t i = k0 + k;
             const f32x4 v0 = at(i, 0), v1 = at(i + 1, 0), v2 = at(i + 2, 0), v3 = at(i + 3, 0);
@@ -741,8 +749,8 @@ int ttp_accumulate_embedding_grad(ttp_ctx* ctx, uint32_t table, const int64_t* t
         a.sorted = a.listed + rows;
         a.named = (uint64_t*)(a.sorted + rows);
         a.count = (uint32_t*)(a.named + named);
-        if (a.first) a.fills = (uint32_t)((named + 3) / 4 * 4);
-        a.groups_in_all = (uint32_t)named;
+        const uint64_t fills = (vocab + 4 * kFillRows - 1) / (4 * kFillRows) * 4;
+        if (a.first) a.fills = (uint32_t)std::min<uint64_t>(fills, 1u << 20);
         if (g.bf16)
             rc = bf16 ? add_rows<uint16_t, uint16_t>(op, a) : add_rows<float, uint16_t>(op, a);
         else
