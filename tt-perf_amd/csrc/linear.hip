@@ -418,7 +418,8 @@ extern "C" int ttp_linear(ttp_ctx* ctx, const ttp_linear_args* args) {
             return fail(TTP_ERR_INVALID, std::string("the input has another type than the weight (") +
                                              (w.bf16 ? "bfloat16" : "float32") + ")");
         ttpi::Buffers b(ctx);
-        if ((rc = b.matrix(x, rows, cols, "the input", false))) return rc;
+        // (y may be the residual, but never what x is: other tiles read x's rows when one is written)
+        if ((rc = b.matrix(x, rows, cols, "the input", false, nullptr, true))) return rc;
         if ((rc = b.own(w.data, w.numel, bf16 ? 2 : 4, "the weight", false))) return rc;
         if (has_bias && (rc = b.own(bias.data, outs, bf16 ? 2 : 4, "the bias", false))) return rc;
         if (res && (rc = b.matrix(res, rows, outs, "the residual", false))) return rc;

@@ -42,18 +42,20 @@ class Buffers {
         if ((uintptr_t)p % size) return misaligned(what);
         const int rc = device_buffer(c_, p, n * size, what, &seen_);
         if (rc) return rc;
-        return add({(uintptr_t)p, n * size, n * size, n * size, written, false, what});
+        return add({(uintptr_t)p, n * size, n * size, n * size, written, false, true, what});
     }
 
     // an array of the context's own memory, whose place and size are known (asking the runtime about
     // it takes a microsecond)
     int own(const void* p, uint64_t n, uint64_t size, const char* what, bool written) {
-        return add({(uintptr_t)p, n * size, n * size, n * size, written, false, what});
+        return add({(uintptr_t)p, n * size, n * size, n * size, written, false, true, what});
     }
 
-    // a matrix of `rows` x `cols`; it may be exactly `same_as` (a result in its input's place)
+    // a matrix of `rows` x `cols`; it may be exactly `same_as` (a result in its input's place), and
+    // with it every other input of the same bytes but those that are `shared`: what one of their rows
+    // or elements says is read for results elsewhere, too (a product's input; every array)
     int matrix(const ttp_matrix* m, uint64_t rows, uint64_t cols, const char* what, bool written,
-               const ttp_matrix* same_as = nullptr) {
+               const ttp_matrix* same_as = nullptr, bool shared = false) {
         const int rc0 = check_matrix(m, what);
         if (rc0) return rc0;
         if (m->rows != rows || m->cols != cols)
@@ -68,14 +70,14 @@ class Buffers {
         const bool in_place = same_as && m->data == same_as->data &&
                               m->stride == same_as->stride && m->dtype == same_as->dtype;
         return add({(uintptr_t)m->data, bytes, m->stride * size, cols * size, written, in_place,
-                    what});
+                    shared, what});
     }
 
   private:
     struct Span {
         uintptr_t at;
         uint64_t bytes, pitch, width;  // of the whole, from row to row, of a row
-        bool written, in_place;
+        bool written, in_place, shared;
         const char* what;
     };
 
@@ -103,7 +105,7 @@ class Buffers {
         for (int k = 0; k < n_; ++k) {
             const Span& o = spans_[k];
             if (!(s.written || o.written) || !overlap(s, o)) continue;
-            if (s.in_place && !o.written && same_rows(s, o)) continue;
+            if (s.in_place && !o.written && !o.shared && same_rows(s, o)) continue;
             return fail(TTP_ERR_INVALID, std::string(s.what) + " overlaps " + o.what);
         }
         if (n_ < kMax) spans_[n_++] = s;
