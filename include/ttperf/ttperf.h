@@ -655,10 +655,11 @@ int ttp_accumulate_embedding_grad(ttp_ctx* ctx, uint32_t table, const int64_t* t
 /* Layer norm over each row: m the mean, r = 1 / sqrt(mean((x - m)^2) + eps),
  *   y = (x - m) r weight + bias     (weight, bias: tensor indices or TTP_NO_TENSOR: 1 and 0)
  * mean and rstd (rows each): m and r, for the backward.  y of either type; of x's type it may be
- * exactly x.  At most 2^24 columns; eps 0 or more. */
+ * exactly x.  At most 2^24 columns; eps 0 or more.  y is made from the differences from the row's
+ * mean as it is, not as `mean` holds it, rounded to fp32: rows far from 0 lose nothing. */
 int ttp_layer_norm(ttp_ctx* ctx, uint32_t weight, uint32_t bias, const ttp_matrix* x, double eps,
                    const ttp_matrix* y, float* mean, float* rstd);
-/* With h = (x - m) r and g = dy weight:
+/* With h = (x - m) r, of m and r as given, and g = dy weight:
  *   dx = add + r (g - mean(g) - h mean(g h))    weight (+)= sum dy h,   bias (+)= sum dy
  * over the rows, into the store's gradients as ttp_accumulate_grad puts them.  add (null: none)
  * and dx have x's type; dy either.  dx may be exactly dy, add or x. */

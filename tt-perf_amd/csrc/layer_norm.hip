@@ -4,11 +4,15 @@
 //   h = (x - m) r,  g = dy w,  dx = add + r (g - mean g - h mean(g h)),  dw = sum dy h,  db = sum dy
 //
 // Bound by memory.  A row of up to 1536 columns is a wave's, one of up to 8192 a block's of four or
-// eight waves: it is read once, into registers, and its sums are taken there (the variance from the differences,
-// not from the squares, whose difference would lose what a mean far from 0 shares).  Longer rows are
-// read again for each sum.  The backward keeps the weight's and the bias's sums of its rows in
-// registers too: a block has a range of rows, writes one partial sum per column, and
-// join_columns_kernel adds those up in order.
+// eight waves: it is read once, into registers, and its sums are taken there.  Longer rows are read
+// again for each sum.  The backward keeps the weight's and the bias's sums of its rows in registers
+// too: a block has a range of rows, writes one partial sum per column, and join_columns_kernel adds
+// those up in order.
+//
+// Rows far from 0: a sum in fp32, rounded to the mean m', is off by some units of the mean, which in
+// the variance and beside small deviations is much (1e4 with a deviation of 0.1: y 1e-2 off).  So the
+// variance is that of the differences d = x - m', exact to their own unit, and what they still have
+// in common, c = mean d, is taken off: m = m' + c, variance = mean d^2 - c^2, y from d - c (4e-7 off).
 //
 // bf16, us: 8192 x 1280 forward 10.8 and backward, with a gradient to add, 18.7 (4.5 TB/s) + 3.9;
 // 16384 x 1600 27 and 40 (5.3 TB/s) + 4.8; 8192 x 1280 fp32 18 and 31 (5.4 TB/s) + 4.  At 1280 columns
@@ -50,12 +54,8 @@ __device__ __forceinline__ void load_vector(const Vector& p, uint32_t c, uint32_
 
 // the wave's sum in every lane, by a butterfly without LDS permutes (see wave_sum)
 __device__ __forceinline__ double wave_total(double x) { return wave_sum(x); }
-__device__ __forceinline__ float wave_total(float x) {
-    {
-        const uint32_t u = __float_as_uint(x);
-        const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-        x = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-    }
+// (the steps within 32 lanes)
+__device__ __forceinline__ float half_total(float x) {
     {
         const uint32_t u = __float_as_uint(x);
         const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
@@ -68,18 +68,38 @@ __device__ __forceinline__ float wave_total(float x) {
     add(__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), 0xB1, 0xF, 0xF, true));
     return x;
 }
+// a's sum in the lower 32 lanes, b's in the upper: two sums for the steps of one
+__device__ __forceinline__ float wave_totals(float a, float b) {
+    const auto s =
+        __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+    return half_total(__uint_as_float(s[0]) + __uint_as_float(s[1]));
+}
+__device__ __forceinline__ float wave_total(float x) { return wave_totals(x, x); }
 
-// The sums of N numbers over the kWaves waves of a row, in every lane.
+// The sums of N numbers (fp32: one or two) over the kWaves waves of a row, in every lane.
 template <int kWaves, int N, class F>
 __device__ __forceinline__ void row_sums(F (&x)[N], F* lds) {
+    constexpr bool kPair = N == 2 && sizeof(F) == 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if constexpr (kPair) {
+        x[0] = wave_totals(x[0], x[1]);
+        if constexpr (kWaves == 1) {
+            const int u = (int)__float_as_uint(x[0]);
+            x[0] = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(u, 0));
+            x[1] = __uint_as_float((uint32_t)__builtin_amdgcn_readlane(u, 32));
+        }
+    } else {
 #pragma unroll
-    for (int n = 0; n < N; ++n) x[n] = wave_total(x[n]);
+        for (int n = 0; n < N; ++n) x[n] = wave_total(x[n]);
+    }
     if constexpr (kWaves > 1) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
         __syncthreads();  // the last sums have been read
-        if (lane == 0)
+        if constexpr (kPair) {
+            if (lane % 32 == 0) lds[wave * 2 + lane / 32] = x[0];
+        } else if (lane == 0) {
 #pragma unroll
             for (int n = 0; n < N; ++n) lds[wave * N + n] = x[n];
+        }
         __syncthreads();
 #pragma unroll
         for (int n = 0; n < N; ++n) {
@@ -179,7 +199,7 @@ __device__ __forceinline__ void param_values(const Raw8<W>& r, const Vector& p, 
 // kWaves waves have a row of up to kC steps of 512 kWaves columns.
 template <class T, class Y, class W, int kWaves, int kC, bool kShort>
 __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void norm_kernel(NormArgs a) {
-    __shared__ float lds[kWaves];
+    __shared__ float lds[2 * kWaves];
     const uint32_t lane = kWaves == 1 ? threadIdx.x & 63 : threadIdx.x, cols = a.cols;
     const uint64_t row =
         kWaves == 1 ? (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (uint64_t)blockIdx.x;
@@ -194,6 +214,7 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void norm_kernel(N
     for (int k = 0; k < kC; ++k) load_param<kShort>(weight[k], a.weight, place(k), cols);
 #pragma unroll
     for (int k = 0; k < kC; ++k) load_param<kShort>(bias[k], a.bias, place(k), cols);
+    const float share = 1.0f / (float)cols;
     float v[kC][8];
     float s[1] = {0.0f};
 #pragma unroll
@@ -203,20 +224,23 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void norm_kernel(N
         for (int j = 0; j < 8; ++j) s[0] += place(k).has(j) ? v[k][j] : 0.0f;
     }
     row_sums<kWaves>(s, lds);
-    const float n = (float)cols, m = s[0] / n;
-    s[0] = 0.0f;
+    const float m = s[0] / (float)cols;
+    float d[2] = {0.0f, 0.0f};  // the sums of the differences and of their squares
 #pragma unroll
     for (int k = 0; k < kC; ++k)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const bool in = place(k).has(j) && (!kShort || j < (int)cols);
             v[k][j] = in ? v[k][j] - m : 0.0f;
-            s[0] += v[k][j] * v[k][j];
+            d[0] += v[k][j];
+            d[1] = __builtin_fmaf(v[k][j], v[k][j], d[1]);
         }
-    row_sums<kWaves>(s, lds);
-    const float r = 1.0f / sqrtf(s[0] / n + (float)a.eps);
+    row_sums<kWaves>(d, lds);
+    const float c = d[0] * share, var = __builtin_fmaf(-c, c, d[1] * share);
+    const float r = 1.0f / sqrtf((var < 0.0f ? 0.0f : var) + (float)a.eps);  // (NaN stays NaN)
+    const float cr = c * r;
     if (lane == 0) {
-        a.mean[row] = m;
+        a.mean[row] = m + c;
         a.rstd[row] = r;
     }
     Y* y = (Y*)a.out + row * a.out_stride;
@@ -226,7 +250,8 @@ __global__ __launch_bounds__(kWaves == 1 ? 256 : 64 * kWaves) void norm_kernel(N
         param_values(weight[k], a.weight, w);
         param_values(bias[k], a.bias, b);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = v[k][j] * r * w[j] + b[j];
+        for (int j = 0; j < 8; ++j)
+            w[j] = __builtin_fmaf(__builtin_fmaf(v[k][j], r, -cr), w[j], b[j]);
         store_place<kShort>(y, place(k), cols, w);
     }
 }
@@ -364,7 +389,8 @@ void norm_backward_kernel(NormArgs a, uint64_t per) {
 }
 
 // ---- rows that registers do not hold -----------------------------------------------------------
-// A block per row, which reads it once for each sum and once more; the sums in 64 bits.
+// A block per row, which reads it once for each sum and once more; the sums in 64 bits, the mean as
+// fp32 and what its rounding left.
 template <class T, class Y>
 __global__ __launch_bounds__(256) void norm_long_kernel(NormArgs a) {
     __shared__ double lds[8];
@@ -378,7 +404,7 @@ __global__ __launch_bounds__(256) void norm_long_kernel(NormArgs a) {
         for (int j = 0; j < 8; ++j) s[0] += v[j];
     }
     row_sums<4>(s, lds);
-    const float m = (float)(s[0] / a.cols);
+    const float m = (float)(s[0] / a.cols), left = (float)(s[0] / a.cols - m);
     s[0] = 0.0;
     for (uint64_t c = threadIdx.x * 8; c < a.cols; c += 2048) {
         float v[8];
@@ -390,7 +416,8 @@ __global__ __launch_bounds__(256) void norm_long_kernel(NormArgs a) {
         }
     }
     row_sums<4>(s, lds);
-    const float r = (float)(1.0 / sqrt(s[0] / a.cols + a.eps));
+    const double var = s[0] / a.cols - (double)left * left;
+    const float r = (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + a.eps)), left_r = left * r;
     if (threadIdx.x == 0) {
         a.mean[row] = m;
         a.rstd[row] = r;
@@ -402,7 +429,8 @@ __global__ __launch_bounds__(256) void norm_long_kernel(NormArgs a) {
         load_vector(a.weight, (uint32_t)c, a.cols, w);
         load_vector(a.bias, (uint32_t)c, a.cols, b);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = (v[j] - m) * r * w[j] + b[j];
+        for (int j = 0; j < 8; ++j)
+            v[j] = __builtin_fmaf(__builtin_fmaf(v[j] - m, r, -left_r), w[j], b[j]);
         store_cols(y, (uint32_t)c, a.cols, v);
     }
 }
