@@ -28,6 +28,7 @@
 
 #include "columns8.hpp"
 #include "context.hpp"
+#include "embedding_cut.hpp"
 #include "matrix.hpp"
 #include "vector16.hpp"
 
@@ -111,7 +112,8 @@ struct GradArgs {
     const void* dy;
     uint64_t dy_stride;
     uint32_t rows, cols, vocab;
-    uint32_t parts_log2, keys;  // blocks of the sort; tokens of each
+    uint32_t parts_log2, keys;  // blocks of the sort; tokens of each (few tokens: of a wave)
+    uint32_t row0;              // few tokens: the launch's first row of the table
     uint32_t slabs;
     float scale;
     void* grad;
@@ -493,13 +495,13 @@ __global__ __launch_bounds__(256) void join_runs_kernel(GradArgs a, uint32_t wav
     put_row(p, a.cols, a.scale, a.first, c, (s0 + s1) + (s2 + s3), old);
 }
 
-// Few tokens, in one launch: a wave has `keys` rows of the gradient and a slab of their columns, and
-// looks through all tokens for those rows.  Where there are none, the waves of these rows share their
-// zeros; else each row's list goes through the LDS, and its rows of dy are added up 16 at a time, in
-// eight sums.  Up to 512 tokens, us (sorted / so): 500 x 768 into 50257 rows bf16 31.5 / 19.5 and fp32
-// 40.1 / 33.0 (the zeros alone 13.0 and 29.1), 300 x 1600 into 5000 rows 23.8 / 11.7, 200 x 384 into 65
-// rows 18.2 / 11.7; slower only where most of them are one token, whose list is one wave's a slab
-// (512 x 384 in full: 18 / 25).
+// Few tokens, in one launch (embedding_cut.hpp): a wave has `keys` rows of the gradient and a slab of
+// their columns, and looks through all tokens for those rows.  Where there are none, the waves of these
+// rows share their zeros; else each row's list goes through the LDS, and its rows of dy are added up 16
+// at a time, in eight sums.  Up to 512 tokens, us (sorted / so): 500 x 768 into 50257 rows bf16 31.5 /
+// 19.5 and fp32 40.1 / 33.0 (the zeros alone 13.0 and 29.1), 300 x 1600 into 5000 rows 23.8 / 11.7, 200 x
+// 384 into 65 rows 18.2 / 11.7; slower only where most of them are one token, whose list is one wave's a
+// slab (512 x 384 in full: 18 / 25).
 constexpr uint32_t kFewTokens = 512, kFewWords = kFewTokens / 64;
 template <class G, class O, bool kNarrow>
 __global__ __launch_bounds__(64 * kSumWaves) void few_rows_kernel(GradArgs a, uint32_t waves) {
@@ -508,7 +510,7 @@ __global__ __launch_bounds__(64 * kSumWaves) void few_rows_kernel(GradArgs a, ui
     const uint32_t w = blockIdx.x * kSumWaves + wave;
     if (w >= waves) return;
     const uint32_t lane = threadIdx.x & 63, slab = w % a.slabs;
-    const uint32_t row0 = w / a.slabs * a.keys, n = min(a.keys, a.vocab - row0);
+    const uint32_t row0 = a.row0 + w / a.slabs * a.keys, n = min(a.keys, a.vocab - row0);
     const Columns c = columns_of(slab * kSlab + lane * 4, a.cols);
     uint32_t* const list = lists[wave];
     int64_t token[kFewWords];
@@ -582,18 +584,20 @@ __global__ __launch_bounds__(64 * kSumWaves) void few_rows_kernel(GradArgs a, ui
 
 template <class G, class O>
 int add_few_rows(const ttpi::Op& op, GradArgs a) {
-    // rows of a wave: as many as leave the CUs 16 waves each, up to 8 (with 16, 256 neighbouring tokens
-    // of 50257 took 28 us instead of 17)
-    const uint64_t all = (uint64_t)a.vocab * a.slabs / (16 * (uint64_t)op.num_cus);
-    a.keys = (uint32_t)std::max<uint64_t>(std::min<uint64_t>(all, 8), 1);
-    const uint32_t waves = (a.vocab + a.keys - 1) / a.keys * a.slabs;
-    const dim3 grid((waves + kSumWaves - 1) / kSumWaves), block(64 * kSumWaves);
-    (void)hipGetLastError();
-    if (a.cols < 4)
-        hipLaunchKernelGGL((few_rows_kernel<G, O, true>), grid, block, 0, op.stream, a, waves);
-    else
-        hipLaunchKernelGGL((few_rows_kernel<G, O, false>), grid, block, 0, op.stream, a, waves);
-    TTPI_HIP(hipGetLastError());
+    const FewRowsCut cut = cut_few_rows(a.vocab, a.slabs, (uint64_t)op.num_cus);
+    a.keys = cut.keys;
+    for (uint64_t r = 0; r < a.vocab; r += cut.rows) {
+        const uint64_t rows = std::min<uint64_t>(cut.rows, a.vocab - r);
+        a.row0 = (uint32_t)r;
+        const uint32_t waves = (uint32_t)((rows + a.keys - 1) / a.keys) * a.slabs;
+        const dim3 grid((waves + kSumWaves - 1) / kSumWaves), block(64 * kSumWaves);
+        (void)hipGetLastError();
+        if (a.cols < 4)
+            hipLaunchKernelGGL((few_rows_kernel<G, O, true>), grid, block, 0, op.stream, a, waves);
+        else
+            hipLaunchKernelGGL((few_rows_kernel<G, O, false>), grid, block, 0, op.stream, a, waves);
+        TTPI_HIP(hipGetLastError());
+    }
     return TTP_OK;
 }
 
