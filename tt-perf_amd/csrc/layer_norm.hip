@@ -799,6 +799,7 @@ int ttp_layer_norm_backward(ttp_ctx* ctx, uint32_t weight, uint32_t bias, const 
         if (has_weight || has_bias) {
             const JoinArgs j{a.parts, p.n, a.cols, w.data, s.data, size == 2, w.first, s.first};
             const uint32_t blocks = (uint32_t)((2 * cols + 63) / 64);
+            (void)hipGetLastError();
             hipLaunchKernelGGL(join_columns_kernel, dim3(blocks), dim3(1024), 0, op.stream, j);
             TTPI_HIP(hipGetLastError());
         }
