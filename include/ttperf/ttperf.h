@@ -644,11 +644,12 @@ int ttp_dropout_forward(ttp_ctx* ctx, const ttp_dropout* dropout, const ttp_matr
  * null): none.  y of either type. */
 int ttp_embedding(ttp_ctx* ctx, uint32_t table, const int64_t* tokens, double scale,
                   uint32_t position_table, const int64_t* positions, const ttp_matrix* y);
-/* The table's gradient: row v (+)= scale times the sum of dy's rows whose token is v, in the order
- * of the rows, into the store's gradient as ttp_accumulate_grad puts it (no gradient yet: the
- * other rows become 0; else they are left as they are).  Tokens outside the table are passed
- * over.  dy of either type.  Tables of fewer than 2^30 rows; rows of dy / 16 times its columns / 256,
- * each rounded up, below 2^25. */
+/* The table's gradient: row v (+)= scale times the sum of dy's rows whose token is v, into the
+ * store's gradient as ttp_accumulate_grad puts it (no gradient yet: the other rows become 0; else
+ * they are left as they are).  Tokens outside the table are passed over.  dy of either type.  The
+ * order of the additions is fixed by the list of tokens and its length: the same call gives the same
+ * bits, another list may add the same rows in another order.  Tables of fewer than 2^30 rows; rows of
+ * dy / 16 times its columns / 256, each rounded up, below 2^25. */
 int ttp_accumulate_embedding_grad(ttp_ctx* ctx, uint32_t table, const int64_t* tokens, double scale,
                                   const ttp_matrix* dy);
 

@@ -3,13 +3,14 @@
 // The lookup is bound by memory: a lane has 8 columns of a row (16384 x 768 bf16 with a table of
 // positions: 10.8 us).
 //
-// The gradient's row v is the sum of the rows of dy whose token is v, in their order.  Up to 512 rows
-// few_rows_kernel looks for them itself.  For more there are three launches:
+// The gradient's row v is the sum of the rows of dy whose token is v.  Up to 512 rows few_rows_kernel
+// looks for them itself, in eight sums that take them in turn.  For more there are three launches:
 // sort_tokens_kernel puts the tokens in order (equal ones by their rows), sum_rows_kernel walks the
 // sorted list in chunks of equal length, so that frequent tokens cost no more than rare ones, and
 // writes every run of one token that lies within a chunk; what a chunk has of a run that crosses its
-// ends goes to scratch memory, and join_runs_kernel adds these up in order, while its other blocks
-// write zeros where no token is.  No sum depends on when a block runs.
+// ends goes to scratch memory, and join_runs_kernel adds these up, four sums in turn, while its other
+// blocks write zeros where no token is.  The order of a sum follows from the list of tokens (which other
+// tokens there are says where a run is cut), never from when a block runs.
 // Measured, 16384 x 768 bf16 into 50257 rows: sort 12 us, sums 15 (5 of them to find their rows),
 // joins beside 77 MB of zeros 14; added to a gradient that is there 12, 13 and 6.  4099 x 384 fp32
 // into 65 rows: 7, 4 and 6 us.
