@@ -676,6 +676,10 @@ int ttp_layer_norm_backward(ttp_ctx* ctx, uint32_t weight, uint32_t bias, const 
  * in as three bf16 parts each, of whose products the six largest are taken: what is left out is
  * below 2^-22 of a product (of an operand below 2^-110 the bits below 2^-133 are lost).  An fp32
  * infinity gives what fp32 arithmetic does with factors below 2^12, with larger ones that or NaN.
+ * How a product is cut, and so the order of its sums, follows from its sizes, its types and whether
+ * its operands lie on the 16-byte grid: the same inputs at another alignment or row stride may give
+ * other last bits.  A result has fewer than 2^23 tiles, of 32 x 64 at least for up to 64 rows and of
+ * 128 x 128 for more.
  * y may be exactly the residual (but not where x is the same memory, too). */
 #define TTP_ACTIVATION_NONE 0
 #define TTP_ACTIVATION_RELU 1

@@ -1,7 +1,8 @@
 // embedding.hip — embedding lookup, and its gradient by sorted tokens.
 //
-// The lookup is bound by memory: a lane has 8 columns of a row (16384 x 768 bf16 with a table of
-// positions: 10.8 us).
+// The lookup is bound by memory and by how little of it a lane has under way: its token, then 8 columns
+// of that token's row, then the result (16384 x 768 bf16 with a table of positions: 10.6 us for the 36 MB
+// of a batch with 5,900 different tokens, 3.4 TB/s).
 //
 // The gradient's row v is the sum of the rows of dy whose token is v.  Up to 512 rows few_rows_kernel
 // looks for them itself, in eight sums that take them in turn.  For more there are three launches:
@@ -12,7 +13,7 @@
 // blocks write zeros where no token is.  The order of a sum follows from the list of tokens (which other
 // tokens there are says where a run is cut), never from when a block runs.
 // Measured, 16384 x 768 bf16 into 50257 rows: sort 12 us, sums 15 (5 of them to find their rows),
-// joins beside 77 MB of zeros 14; added to a gradient that is there 12, 13 and 6.  4099 x 384 fp32
+// joins beside 77 MB of zeros 14 (40 in all, as called); added to a gradient that is there 12, 13 and 6.  4099 x 384 fp32
 // into 65 rows: 7, 4 and 6 us.
 //
 // The sort: block p has the tokens p, p + parts, p + 2 parts ..., at most kMostKeys of the table's.

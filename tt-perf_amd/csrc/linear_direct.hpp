@@ -4,11 +4,15 @@
 // kM x 32 F of y per block of four waves, kK of the summed index per step, through kStages LDS
 // buffers that the loads fill without passing through registers.
 //
-// What bounds it: power.  At these sizes the clock falls to 1.7 GHz, and the matrix instructions alone,
-// on random operands in registers, reach 2.0 PFLOP/s as 16 x 16 x 32 and 1.7 as 32 x 32 x 16, which is
-// why the former are used.  8192 x 1280 x 5120 with GELU takes 118 us (0.91 PFLOP/s, the instructions
-// busy half of the cycles) and 8192 x 5120 x 1280 with dropout and a residual 103 (1.04).  A token's
-// 768 x 50257 is bound by W's 77 MB: 14.5 us, 5.3 TB/s.
+// What bounds it: in the steps, power.  The clock falls to 1.7 GHz, and the matrix instructions alone, on
+// random operands in registers, reach 2.0 PFLOP/s as 16 x 16 x 32 and 1.7 as 32 x 32 x 16, which is why
+// the former are used; steps go at 1.3 PFLOP/s in 128 x 256 tiles and 1.47 in 256 x 160.  The rest is
+// what lies before a tile's first step and behind its last, and uneven rounds of tiles: 8192 x 1280 x
+// 5120 with GELU takes 118 us (0.91 PFLOP/s), two rounds of 128 x 256 tiles and a half one, 10.8 us of
+// each round's 44 outside the steps; 8192 x 5120 x 1280 with dropout and a residual 103 (1.04), one
+// round of 256 x 160, 13 us outside; 8192 x 768 x 50257 transposed 850 (0.74), with 24 steps to a
+// tile (the library's product alone 575).  A token's 768 x 50257 is bound by W's 77 MB: 14.5 us, 5.3
+// TB/s.
 //
 // Four shapes, since no tile is best for every grid of 256 CUs (linear_cut.hpp has the choice and the
 // figures): 256 x 160 moves the fewest bytes through the LDS for a product, one block to a CU; 128 x 256

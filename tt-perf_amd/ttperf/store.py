@@ -562,9 +562,10 @@ class ParamStore(_StepSlots, Operators):
         bf16 buffers come back as torch.bfloat16.  The view aliases the store's memory, which
         lasts until the store is closed (a view keeps a store alive that nothing else
         names; one that the store itself reaches, as an attribute of it, keeps it until close():
-        the collector does not see what torch's storage holds).  Torch work on it is ordered on torch's current stream and the
-        store's on its own: share one stream (set_stream(torch.cuda.current_stream())) or
-        synchronise between them.  Writes to BUF_GRAD through a view need mark_grads()."""
+        the collector does not see what torch's storage holds).  Torch work on it is ordered on
+        torch's current stream and the store's on its own: share one stream
+        (set_stream(torch.cuda.current_stream())) or synchronise between them.  Writes to
+        BUF_GRAD through a view need mark_grads()."""
         import torch
         ptr = self.ptr(which, index)
         n = self._numel(index)
